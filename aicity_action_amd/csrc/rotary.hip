@@ -1,0 +1,269 @@
+// Rotary positions with several axes (time, height, width): each head's channels are cut into one section per axis, a section's channels
+// into pairs (a, b), and the pair i of axis A turns by the angle p_A * f_i where p_A is the token's place on that axis:
+//     y_a = x_a cos - x_b sin,     y_b = x_a sin + x_b cos;
+// the scores q . k of rotated queries and keys then depend on the differences of places alone.  The transposed map is the turn by the
+// negative angle, so the backward pass is the same kernel with the sine's sign flipped.  Channels behind the sections pass through; with
+// an addend the result is rot(x) + add, rounded once.
+//
+// Bound by HBM: 2 * itemsize bytes and six operations per channel.  The angle is not read from a table: the place times the frequency (in
+// turns) is one product in 64 bits -- a place of a million turns the fastest pair 160,000 times, which 32 bits would round to a hundredth
+// of a turn -- whose fraction goes to sincospif in 32 bits (angle off by at most 2^-24 of half a turn).  That costs about 40 VALU cycles
+// per pair and wave, half of what the memory time of the pair's row leaves free, and is shared by all heads that a thread walks.
+#include "common.h"
+
+struct RotaryArgs {
+    mvit_rotary_tensor t[2];
+    uint32_t first_block_1;        // blocks of t[1] begin here
+    uint32_t blocks_per_group[2];  // blocks that cover L tokens x tasks of one (batch, head group)
+    uint32_t groups[2];            // head groups per batch
+    int heads_per_thread[2];
+    int dim, pairs, axes;          // channels, rotated pairs of a head
+    int tasks;                     // threads per token: pair chunks, then chunks of the channels that pass through
+    int sec[MVIT_ROTARY_AXES];     // channels of each section
+    float sign;
+    double turns[MVIT_ROTARY_PAIRS];
+};
+
+template <typename T, int V> struct RotVec { typedef T type __attribute__((ext_vector_type(V))); };
+template <typename T> struct RotVec<T, 1> { typedef T type; };
+
+template <typename T, int V>
+__device__ __forceinline__ void rot_load(const T* p, float (&f)[V]) {
+    const typename RotVec<T, V>::type v = *reinterpret_cast<const typename RotVec<T, V>::type*>(p);
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        T e;
+        if constexpr (V == 1) e = v;
+        else e = v[j];
+        if constexpr (sizeof(T) == 2) f[j] = bf16_to_f32(e);
+        else f[j] = e;
+    }
+}
+template <typename T, int V>
+__device__ __forceinline__ void rot_store(T* p, const float (&f)[V]) {
+    typename RotVec<T, V>::type v;
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        T e;
+        if constexpr (sizeof(T) == 2) e = f32_to_bf16(f[j]);
+        else e = f[j];
+        if constexpr (V == 1) v = e;
+        else v[j] = e;
+    }
+    *reinterpret_cast<typename RotVec<T, V>::type*>(p) = v;
+}
+
+// A thread owns V pairs of one token (2 V channels: two vectors of V) in up to heads_per_thread heads.  INTER: the pairs are (2i, 2i + 1),
+// else (i, i + s / 2) within a section of s.  V divides what the host checked: every vector is aligned and none crosses a section's half
+// (interleaved: pairs of two sections may share a thread, each pair looks up its own axis).
+template <typename T, int V, bool INTER>
+__global__ __launch_bounds__(256) void rotary_kernel(const RotaryArgs a) {
+    const int which = blockIdx.x >= a.first_block_1 ? 1 : 0;
+    const mvit_rotary_tensor& t = a.t[which];
+    const uint32_t blk = blockIdx.x - (which ? a.first_block_1 : 0u);
+    const uint32_t row = blk / a.blocks_per_group[which], in_row = blk - row * a.blocks_per_group[which];
+    const uint32_t item = in_row * 256u + threadIdx.x;
+    const uint32_t l = item / (uint32_t)a.tasks, task = item - l * (uint32_t)a.tasks;
+    if ((int64_t)l >= t.L) return;
+    const uint32_t b = row / a.groups[which], grp = row - b * a.groups[which];
+    const int h0 = (int)grp * a.heads_per_thread[which];
+    const int h1 = min(h0 + a.heads_per_thread[which], t.H);
+
+    const T* x = static_cast<const T*>(t.x) + (int64_t)b * t.xs[0] + (int64_t)l * t.xs[2];
+    T* y = static_cast<T*>(t.y) + (int64_t)b * t.ys[0] + (int64_t)l * t.ys[2];
+    const T* add = t.add ? static_cast<const T*>(t.add) + (int64_t)b * t.as[0] + (int64_t)l * t.as[2] : nullptr;
+    const int p0 = (int)task * V;           // first pair of this thread
+    const int chunks = a.pairs / V;
+
+    if ((int)task >= chunks) {              // channels that pass through
+        const int c0 = 2 * a.pairs + ((int)task - chunks) * 2 * V;
+        for (int h = h0; h < h1; ++h) {
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                const int c = c0 + half * V;
+                if (c >= a.dim) break;
+                float f[V];
+                rot_load<T, V>(x + (int64_t)h * t.xs[1] + c, f);
+                if (add) {
+                    float g[V];
+                    rot_load<T, V>(add + (int64_t)h * t.as[1] + c, g);
+#pragma unroll
+                    for (int j = 0; j < V; ++j) f[j] += g[j];
+                }
+                rot_store<T, V>(y + (int64_t)h * t.ys[1] + c, f);
+            }
+        }
+        return;
+    }
+
+    // the place on every axis
+    double place[MVIT_ROTARY_AXES];
+    if (t.pos) {
+        const int64_t at = (int64_t)b * t.ps[0] + (int64_t)l * t.ps[1];
+#pragma unroll
+        for (int n = 0; n < MVIT_ROTARY_AXES; ++n) {
+            if (n >= a.axes) break;
+            const int64_t i = at + n * t.ps[2];
+            place[n] = t.pos_type == MVIT_POS_I32 ? (double)static_cast<const int32_t*>(t.pos)[i]
+                     : t.pos_type == MVIT_POS_I64 ? (double)static_cast<const int64_t*>(t.pos)[i]
+                                                  : (double)static_cast<const float*>(t.pos)[i];
+        }
+    } else {
+        uint32_t rest = l;
+#pragma unroll
+        for (int n = MVIT_ROTARY_AXES - 1; n >= 0; --n) {
+            if (n >= a.axes) continue;
+            const uint32_t q = rest / (uint32_t)t.grid[n];
+            place[n] = t.origin[n] + t.step[n] * (double)(rest - q * (uint32_t)t.grid[n]);
+            rest = q;
+        }
+    }
+    float cs[V], sn[V];
+    int ca = 0, cb = 0;                     // channels of the thread's two vectors
+    int axis = 0, first = 0;                // axis of the pair, first channel of its section
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        const int p = p0 + j;
+#pragma unroll
+        for (int n = 0; n < MVIT_ROTARY_AXES - 1; ++n)
+            if (axis == n && 2 * p >= first + a.sec[n] && n + 1 < a.axes) { first += a.sec[n]; axis = n + 1; }
+        double at = place[0];
+#pragma unroll
+        for (int n = 1; n < MVIT_ROTARY_AXES; ++n) at = axis == n ? place[n] : at;
+        const double turn = at * a.turns[p];
+        const float r = (float)(turn - __builtin_rint(turn));
+        sincospif(2.0f * r, &sn[j], &cs[j]);
+        sn[j] *= a.sign;
+        if (j == 0) {
+            if (INTER) { ca = 2 * p0; cb = 2 * p0 + V; }
+            else { ca = first + (p0 - first / 2); cb = ca + a.sec[axis] / 2; }
+        }
+    }
+    for (int h = h0; h < h1; ++h) {
+        float u[V], w[V];
+        const T* xh = x + (int64_t)h * t.xs[1];
+        rot_load<T, V>(xh + ca, u);
+        rot_load<T, V>(xh + cb, w);
+        float yu[V], yw[V];
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            if (INTER) {                    // flat channel 2j, 2j + 1 of the 2 V in (u, w)
+                const float xa = 2 * j < V ? u[(2 * j) % V] : w[(2 * j) % V];
+                const float xb = 2 * j + 1 < V ? u[(2 * j + 1) % V] : w[(2 * j + 1) % V];
+                const float ya = xa * cs[j] - xb * sn[j], yb = xa * sn[j] + xb * cs[j];
+                if (2 * j < V) yu[(2 * j) % V] = ya; else yw[(2 * j) % V] = ya;
+                if (2 * j + 1 < V) yu[(2 * j + 1) % V] = yb; else yw[(2 * j + 1) % V] = yb;
+            } else {
+                yu[j] = u[j] * cs[j] - w[j] * sn[j];
+                yw[j] = u[j] * sn[j] + w[j] * cs[j];
+            }
+        }
+        if (add) {
+            rot_load<T, V>(add + (int64_t)h * t.as[1] + ca, u);
+            rot_load<T, V>(add + (int64_t)h * t.as[1] + cb, w);
+#pragma unroll
+            for (int j = 0; j < V; ++j) { yu[j] += u[j]; yw[j] += w[j]; }
+        }
+        T* yh = y + (int64_t)h * t.ys[1];
+        rot_store<T, V>(yh + ca, yu);
+        rot_store<T, V>(yh + cb, yw);
+    }
+}
+
+template <typename T, int V>
+static void rotary_launch(const RotaryArgs& a, uint32_t blocks, int layout, hipStream_t st) {
+    if (layout) hipLaunchKernelGGL((rotary_kernel<T, V, true>), dim3(blocks), dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((rotary_kernel<T, V, false>), dim3(blocks), dim3(256), 0, st, a);
+}
+
+extern "C" int mvit_rotary_tensor_bytes(void) { return (int)sizeof(mvit_rotary_tensor); }
+
+extern "C" int mvit_rotary(const mvit_rotary_tensor* tensors, int ntensors, int dim, int axes, const int* sections, const double* turns,
+                           int layout, int inverse, int act_dtype, void* stream) {
+    if (!tensors || ntensors < 1 || ntensors > 2 || dim < 1 || axes < 0 || axes > MVIT_ROTARY_AXES || (axes && (!sections || !turns)) ||
+        (layout & ~1))
+        return MVIT_EINVAL;
+    if (act_dtype != MVIT_F32 && act_dtype != MVIT_BF16) return MVIT_EDTYPE;
+    RotaryArgs a;
+    a.dim = dim;
+    a.axes = axes;
+    a.sign = inverse ? -1.0f : 1.0f;
+    const int itemsize = act_dtype == MVIT_F32 ? 4 : 2;
+    int channels = 0;
+    uint64_t fit = 16 / itemsize;           // a power of two: what every extent below has to be a multiple of
+    auto narrow = [&fit](uint64_t v) { while (fit > 1 && v % fit) fit >>= 1; };
+    for (int n = 0; n < MVIT_ROTARY_AXES; ++n) {
+        a.sec[n] = n < axes ? sections[n] : 0;
+        if (n < axes && (sections[n] < 2 || sections[n] % 2)) return MVIT_EINVAL;
+        channels += a.sec[n];
+        // pairs (i, i + s/2): a vector stays in its half, and every half begins at a multiple of it.  Interleaved pairs: only the sum counts
+        if (!layout && n < axes) narrow(a.sec[n] / 2);
+    }
+    if (channels > dim || channels / 2 > MVIT_ROTARY_PAIRS) return MVIT_EINVAL;
+    a.pairs = channels / 2;
+    for (int p = 0; p < a.pairs; ++p) a.turns[p] = turns[p];
+    narrow(a.pairs);
+    narrow(dim - channels);
+    uint64_t total_blocks = 0;
+    for (int i = 0; i < 2; ++i) {
+        a.first_block_1 = (uint32_t)total_blocks;
+        a.blocks_per_group[i] = 1; a.groups[i] = 1; a.heads_per_thread[i] = 1;
+        if (i >= ntensors) { a.t[i] = a.t[0]; a.first_block_1 = 0xffffffffu; continue; }
+        const mvit_rotary_tensor& t = a.t[i] = tensors[i];
+        if (t.B < 0 || t.H < 0 || t.L < 0) return MVIT_EINVAL;
+        if (t.B == 0 || t.H == 0 || t.L == 0) continue;
+        if (!t.x || !t.y || (t.pos && (t.pos_type < MVIT_POS_I32 || t.pos_type > MVIT_POS_F32))) return MVIT_EINVAL;
+        if (!t.pos && axes) {
+            int64_t n = 1;
+            for (int k = 0; k < axes; ++k) {
+                if (t.grid[k] < 1) return MVIT_EINVAL;
+                n *= t.grid[k];
+                if (n > t.L) return MVIT_EINVAL;
+            }
+            if (n != t.L) return MVIT_EINVAL;
+        }
+        const void* ptrs[3] = {t.x, t.y, t.add};
+        const int64_t* strides[3] = {t.xs, t.ys, t.as};
+        const int64_t extent[3] = {t.B, t.H, t.L};
+        for (int k = 0; k < 3; ++k) {
+            if (!ptrs[k]) continue;
+            if (reinterpret_cast<uintptr_t>(ptrs[k]) % itemsize) return MVIT_EINVAL;
+            narrow(reinterpret_cast<uintptr_t>(ptrs[k]) / itemsize);
+            for (int d = 0; d < 3; ++d)     // (the stride of a single row is never used)
+                if (extent[d] > 1) narrow((uint64_t)(strides[k][d] < 0 ? -strides[k][d] : strides[k][d]));
+        }
+    }
+    a.tasks = a.pairs / (int)fit + (dim - channels + 2 * (int)fit - 1) / (2 * (int)fit);
+    // Heads per thread: one head each until there are two rounds of full workgroups on the 256 CUs, then more, so that a turn serves
+    // several heads (up to 8)
+    for (int i = 0; i < ntensors; ++i) {
+        const mvit_rotary_tensor& t = a.t[i];
+        if (i == 1) a.first_block_1 = (uint32_t)total_blocks;
+        if (t.B == 0 || t.H == 0 || t.L == 0) continue;
+        const uint64_t items = (uint64_t)t.L * a.tasks;
+        if (items > 0xffffff00u) return MVIT_EUNSUPPORTED;
+        const uint64_t per = (items + 255) / 256;
+        int hpt = 1;
+        while (hpt < 8 && hpt < t.H && per * t.B * ((t.H + 2 * hpt - 1) / (2 * hpt)) >= 4096) hpt *= 2;
+        a.heads_per_thread[i] = hpt;
+        a.groups[i] = (uint32_t)((t.H + hpt - 1) / hpt);
+        a.blocks_per_group[i] = (uint32_t)per;
+        total_blocks += per * a.groups[i] * (uint64_t)t.B;
+        if (total_blocks > 0x7fffffffu) return MVIT_EUNSUPPORTED;
+    }
+    if (!total_blocks) return MVIT_OK;
+    const uint32_t blocks = (uint32_t)total_blocks;
+    hipStream_t st = as_stream(stream);
+    if (act_dtype == MVIT_F32) {
+        if (fit == 4) rotary_launch<float, 4>(a, blocks, layout, st);
+        else if (fit == 2) rotary_launch<float, 2>(a, blocks, layout, st);
+        else rotary_launch<float, 1>(a, blocks, layout, st);
+    } else {
+        if (fit == 8) rotary_launch<bf16_t, 8>(a, blocks, layout, st);
+        else if (fit == 4) rotary_launch<bf16_t, 4>(a, blocks, layout, st);
+        else if (fit == 2) rotary_launch<bf16_t, 2>(a, blocks, layout, st);
+        else rotary_launch<bf16_t, 1>(a, blocks, layout, st);
+    }
+    MVIT_LAUNCH_CHECK();
+    return MVIT_OK;
+}

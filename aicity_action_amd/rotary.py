@@ -1,0 +1,211 @@
+"""Rotary positions with several axes (time, height, width) for the queries and keys of video and image tokens.
+
+The reference model knows positions from the learned embeddings of its stem alone (slowfast/models/video_model_builder.py:1196-1223); a
+rotary position instead turns pairs of channels of every query and key by an angle proportional to the token's place on one axis, so
+that scores depend on differences of places and a model meets other grid sizes without interpolated tables.  ``HIP.ROTARY`` turns it on
+in the model (models/mvit.py); this module is the operator itself::
+
+    rot = AxialRotary(96)                                            # 32 channels for each of t, h, w
+    q, k = rot(q, TokenGrid((8, 28, 28)), k, TokenGrid((8, 14, 14), step=(1, 2, 2)))
+
+One kernel launch (csrc/rotary.hip) serves both tensors in each direction, on the tensors' device and its current stream; there is no
+CPU fallback.
+"""
+import ctypes
+import math
+
+import torch
+
+from . import _hip
+
+_MAX_AXES, _MAX_PAIRS = 4, 256
+_POS = {torch.int32: 1, torch.int64: 2, torch.float32: 3}
+_LAYOUTS = {"half": 0, "interleaved": 1}
+_i3 = ctypes.c_int64 * 3
+
+
+class _Tensor(ctypes.Structure):
+    """mvit_rotary_tensor of include/mvit_hip.h."""
+    _fields_ = [("x", ctypes.c_void_p), ("y", ctypes.c_void_p), ("add", ctypes.c_void_p), ("pos", ctypes.c_void_p),
+                ("xs", _i3), ("ys", _i3), ("as_", _i3), ("ps", _i3), ("L", ctypes.c_int64), ("B", ctypes.c_int32), ("H", ctypes.c_int32),
+                ("pos_type", ctypes.c_int32), ("grid", ctypes.c_int32 * 4), ("origin", ctypes.c_double * 4), ("step", ctypes.c_double * 4)]
+
+
+class TokenGrid(object):
+    """Tokens in order on a grid, the last axis fastest (the model's token order: t, h, w).  Token (i_0, i_1, ...) stands at
+    ``origin + step * i`` on each axis: keys pooled with stride s stand at every s-th place of the queries' grid (``step=(1, s, s)``)."""
+
+    def __init__(self, sizes, step=None, origin=None):
+        self.sizes = tuple(int(n) for n in sizes)
+        self.step = tuple(float(s) for s in step) if step is not None else (1.0,) * len(self.sizes)
+        self.origin = tuple(float(s) for s in origin) if origin is not None else (0.0,) * len(self.sizes)
+        if not 1 <= len(self.sizes) <= _MAX_AXES or any(n < 1 or n >= 1 << 31 for n in self.sizes):
+            raise ValueError("TokenGrid: 1 to %d axes of at least one token each, got %s" % (_MAX_AXES, self.sizes))
+        if len(self.step) != len(self.sizes) or len(self.origin) != len(self.sizes):
+            raise ValueError("TokenGrid: step and origin need one value for each of the %d axes" % len(self.sizes))
+        if not all(math.isfinite(v) for v in self.step + self.origin):
+            raise ValueError("TokenGrid: step and origin must be finite")
+        self.tokens = math.prod(self.sizes)
+
+    def __repr__(self):
+        return "TokenGrid(%s, step=%s, origin=%s)" % (self.sizes, self.step, self.origin)
+
+
+class AxialRotary(object):
+    """The plan of a head: which channels turn by which axis, and how fast.
+
+    ``sections``: channels per axis, even; default: three axes of ``head_dim // 6 * 2`` channels.  Channels behind the sections pass
+    through.  Pair i of a section of s channels turns by ``place * base ** (-2 i / s)``.  ``layout``: "half" pairs channel i of a section
+    with i + s / 2, "interleaved" pairs 2i with 2i + 1."""
+
+    def __init__(self, head_dim, sections=None, base=10000.0, layout="half"):
+        self.head_dim = int(head_dim)
+        self.sections = tuple(int(s) for s in sections) if sections is not None else (self.head_dim // 6 * 2,) * 3
+        self.base, self.layout = float(base), layout
+        if layout not in _LAYOUTS:
+            raise ValueError("AxialRotary: layout must be 'half' or 'interleaved', got %r" % (layout,))
+        if not 1 <= len(self.sections) <= _MAX_AXES or any(s < 2 or s % 2 for s in self.sections):
+            raise ValueError("AxialRotary: 1 to %d sections of an even number of channels each, got %s" % (_MAX_AXES, self.sections))
+        if sum(self.sections) > self.head_dim or sum(self.sections) > 2 * _MAX_PAIRS:
+            raise ValueError("AxialRotary: sections %s need more than the %d channels of a head (at most %d turn)"
+                             % (self.sections, self.head_dim, 2 * _MAX_PAIRS))
+        if not (math.isfinite(self.base) and self.base > 0.0):
+            raise ValueError("AxialRotary: base must be positive, got %r" % (base,))
+        turns = [self.base ** (-2.0 * i / s) / (2.0 * math.pi) for s in self.sections for i in range(s // 2)]
+        self._turns = (ctypes.c_double * len(turns))(*turns)
+        self._sections = (ctypes.c_int * len(self.sections))(*self.sections)
+
+    def __call__(self, x, positions, k=None, k_positions=None):
+        """Turned copies of ``x`` (and ``k``), differentiable.  Tensors [batch, heads, tokens, head_dim], float32 / bfloat16 / float16, any
+        strides with contiguous channels (a token-major buffer goes in as its transposed view).  Positions: a TokenGrid, or a tensor
+        [tokens, axes] or [batch, tokens, axes] of int32 / int64 / float32 on the same device."""
+        xs, ps = self._arguments(x, positions, k, k_positions)
+        if torch.is_grad_enabled() and any(t.requires_grad for t in xs):
+            held = [_leaf_on_one_stream(t) for t in xs]
+            ys = _RotaryFn.apply(self, ps, *xs)
+            del held                                # the graph holds the nodes now
+        else:
+            ys = self.turn(xs, ps)
+        return tuple(ys) if k is not None else ys[0]
+
+    def rotate_(self, x, positions, k=None, k_positions=None, inverse=False):
+        """The same in place, without a graph (serving: queries and keys are turned where they stand;
+        they must not overlap each other)."""
+        xs, ps = self._arguments(x, positions, k, k_positions)
+        for t in xs:
+            if torch.is_grad_enabled() and t.requires_grad:
+                raise RuntimeError("AxialRotary.rotate_: the tensor requires a gradient; use the plan's call, which makes a turned copy")
+            if any(s == 0 and n > 1 for s, n in zip(t.stride(), t.shape)):
+                raise ValueError("AxialRotary.rotate_: an expanded tensor (stride 0) cannot be turned in place")
+        if k is not None and x.numel() and x.data_ptr() == k.data_ptr():
+            raise ValueError("AxialRotary.rotate_: x and k are the same memory; they must not overlap")
+        self.turn(xs, ps, outs=xs, inverse=inverse)
+        return tuple(xs) if k is not None else x
+
+    # ---- checks ----------------------------------------------------------------------------------------------------------------------
+    def _arguments(self, x, positions, k, k_positions):
+        if (k is None) != (k_positions is None):
+            raise ValueError("AxialRotary: k and k_positions go together")
+        xs, ps = ([x], [positions]) if k is None else ([x, k], [positions, k_positions])
+        for t, p in zip(xs, ps):
+            self._check(t, p)
+            if t.dtype != x.dtype or t.device != x.device:
+                raise ValueError("AxialRotary: x and k must have one dtype and one device, got %s on %s and %s on %s"
+                                 % (x.dtype, x.device, t.dtype, t.device))
+        return xs, ps
+
+    def _check(self, t, p):
+        if t.dim() != 4 or t.shape[3] != self.head_dim:
+            raise ValueError("AxialRotary: expected [batch, heads, tokens, %d], got %s" % (self.head_dim, tuple(t.shape)))
+        if t.dtype not in (torch.float32, torch.bfloat16, torch.float16):
+            raise TypeError("AxialRotary: float32, bfloat16 or float16, got %s" % t.dtype)
+        if t.stride(3) != 1:
+            raise ValueError("AxialRotary: the channels of a head must be contiguous (stride %d)" % t.stride(3))
+        if isinstance(p, TokenGrid):
+            if len(p.sizes) != len(self.sections) or p.tokens != t.shape[2]:
+                raise ValueError("AxialRotary: %r does not describe %d tokens on %d axes" % (p, t.shape[2], len(self.sections)))
+        elif isinstance(p, torch.Tensor):
+            if p.dtype not in _POS:
+                raise TypeError("AxialRotary: positions must be int32, int64 or float32, got %s" % p.dtype)
+            want = (t.shape[2], len(self.sections))
+            if tuple(p.shape) != want and tuple(p.shape) not in ((t.shape[0],) + want, (1,) + want):
+                raise ValueError("AxialRotary: positions must be [%d, %d] or [%d, %d, %d], got %s" % (want + (t.shape[0],) + want + (tuple(p.shape),)))
+            if p.device != t.device:
+                raise ValueError("AxialRotary: positions on %s, the tensor on %s" % (p.device, t.device))
+        else:
+            raise TypeError("AxialRotary: positions must be a TokenGrid or a tensor, got %s" % type(p).__name__)
+        if not t.is_cuda:
+            raise RuntimeError("AxialRotary needs its tensors on a gfx950 device; there is no CPU fallback")
+
+    # ---- the launch --------------------------------------------------------------------------------------------------------------------
+    def turn(self, xs, ps, outs=None, adds=None, inverse=False):
+        """One launch over one or two checked tensors: outs[i] = rot(xs[i]) (+ adds[i]); fresh outputs where ``outs`` is None."""
+        if outs is None:
+            outs = [torch.empty_like(t) for t in xs]
+            outs = [y if y.stride(3) == 1 else torch.empty(y.shape, dtype=y.dtype, device=y.device) for y in outs]
+        _launch(xs, outs, adds, ps, self.head_dim, len(self.sections), self._sections, self._turns, _LAYOUTS[self.layout], inverse)
+        return list(outs)
+
+
+def add_(out, add):
+    """out += add for two [batch, heads, tokens, channels] views of any strides with contiguous channels: the rotary kernel with no axis."""
+    _launch([out], [out], [add], [None], out.shape[3], 0, None, None, 0, False)
+    return out
+
+
+def _launch(xs, outs, adds, ps, dim, axes, sections, turns, layout, inverse):
+    x = xs[0]
+    rec = (_Tensor * len(xs))()
+    for i, (t, y, p) in enumerate(zip(xs, outs, ps)):
+        r = rec[i]
+        r.x, r.y = t.data_ptr(), y.data_ptr()
+        r.xs[:], r.ys[:] = t.stride()[:3], y.stride()[:3]
+        if adds is not None and adds[i] is not None:
+            r.add = adds[i].data_ptr()
+            r.as_[:] = adds[i].stride()[:3]
+        r.B, r.H, r.L = t.shape[0], t.shape[1], t.shape[2]
+        if isinstance(p, TokenGrid):
+            n = len(p.sizes)
+            r.grid[:n], r.origin[:n], r.step[:n] = p.sizes, p.origin, p.step
+        elif p is not None:
+            r.pos, r.pos_type = p.data_ptr(), _POS[p.dtype]
+            r.ps[:] = (p.stride(0) if p.dim() == 3 and p.shape[0] > 1 else 0,) + tuple(p.stride()[-2:])
+    L = _hip.lib("fp16" if x.dtype == torch.float16 else "bf16")
+    with torch.cuda.device(x.device):
+        _hip.check(L.mvit_rotary(rec, len(xs), dim, axes, sections, turns, layout, 1 if inverse else 0,
+                                 _hip.F32 if x.dtype == torch.float32 else _hip.BF16, torch.cuda.current_stream().cuda_stream), "rotary")
+
+
+def _leaf_on_one_stream(t):
+    """A leaf's gradient node belongs to the stream it was made on and lives as long as any graph of the leaf.  A backward pass that is
+    captured into a HIP graph while an eager graph of the same leaf is alive would make the capture wait for a stream outside it, which
+    ends the process when the capture ends: refused here, as far as this operator has seen the leaf."""
+    if not (t.is_leaf and t.requires_grad):
+        return None
+    node = torch.autograd.graph.get_gradient_edge(t).node
+    stream = torch.cuda.current_stream(t.device).cuda_stream
+    if torch.cuda.is_current_stream_capturing() and node.metadata.get("rotary_stream", stream) != stream:
+        raise RuntimeError("AxialRotary: an eager graph of this leaf tensor is still alive while its backward pass is being captured; "
+                           "drop it (its outputs, its loss) before the capture")
+    node.metadata["rotary_stream"] = stream
+    return node
+
+
+class _RotaryFn(torch.autograd.Function):
+    """The turn is orthogonal: the gradient is turned back by the same angles.  Nothing of the input is kept."""
+
+    @staticmethod
+    def forward(ctx, plan, ps, *xs):
+        ctx.plan = plan
+        ctx.grids = [p if isinstance(p, TokenGrid) else None for p in ps]
+        ctx.save_for_backward(*[p for p in ps if not isinstance(p, TokenGrid)])
+        ctx.n = len(xs)
+        return tuple(plan.turn(xs, ps))
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, *grads):
+        saved = iter(ctx.saved_tensors)
+        ps = [g if g is not None else next(saved) for g in ctx.grids]
+        gs = [g if g.stride(3) == 1 else g.contiguous() for g in grads]
+        return (None, None) + tuple(ctx.plan.turn(gs, ps, inverse=True))

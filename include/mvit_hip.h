@@ -353,6 +353,39 @@ int mvit_cast_transpose_f32_to_bf16(const float* src, void* dst, void* dst_t, in
 int mvit_cast_desc_bytes(void);
 int mvit_cast_transpose_multi(const void* desc_table, int ntensors, int total_tiles, void* stream);
 
+/* ------------------------------------------------------------------------------------------------
+ * Operators beside the reference's own: rotary positions, Newton-Schulz orthogonalisation, the Muon step.
+ * ------------------------------------------------------------------------------------------------ */
+
+/* Rotary positions with up to four axes (csrc/rotary.hip): y = rot(x) (+ add), every head's channels cut into one section per axis.
+ *   tensors: HOST array of 1 or 2 records (a query and a key tensor share one launch); x, y, add are act-typed device tensors
+ *            [B][H][L][dim] with the element strides of batch, head and token given and channels contiguous; add may be NULL; y may be x
+ *            itself (same strides), any other overlap is the caller's error.
+ *   places:  pos = NULL: token l stands on the grid grid[0] x ... (last axis fastest, product = L) at origin[n] + step[n] * index;
+ *            else device places [B][L][axes] of pos_type with element strides ps (0 = shared by the batch).
+ *   sections: HOST, channels per axis, even, sum <= dim (the rest passes through); axes may be 0 (y = x + add).
+ *   turns:   HOST, one per pair: turns (angle / 2 pi) per unit of place; the product with the place is taken in 64 bits.
+ *   layout:  0 pairs (i, i + s/2) of a section of s channels, 1 pairs (2i, 2i + 1).   inverse: the turn by the negative angle = the
+ *            transposed map = the backward pass.
+ * MVIT_EUNSUPPORTED: more than 2^31 workgroups. */
+enum { MVIT_ROTARY_AXES = 4, MVIT_ROTARY_PAIRS = 256 };
+enum { MVIT_POS_I32 = 1, MVIT_POS_I64 = 2, MVIT_POS_F32 = 3 };
+typedef struct {
+    const void* x;
+    void* y;
+    const void* add;
+    const void* pos;
+    int64_t xs[3], ys[3], as[3], ps[3];
+    int64_t L;
+    int32_t B, H;
+    int32_t pos_type;
+    int32_t grid[4];
+    double origin[4], step[4];
+} mvit_rotary_tensor;
+int mvit_rotary_tensor_bytes(void);
+int mvit_rotary(const mvit_rotary_tensor* tensors, int ntensors, int dim, int axes, const int* sections, const double* turns, int layout,
+                int inverse, int act_dtype, void* stream);
+
 #if defined(__GNUC__) || defined(__clang__)
 #pragma GCC visibility pop
 #endif
