@@ -89,6 +89,10 @@ _SIGS = {
     "mvit_adamw_step_dev": (c_i, [c_p, c_i, c_p, c_p, c_f, c_f, c_f, c_p]),
     "mvit_rotary_tensor_bytes": (c_i, []),
     "mvit_rotary": (c_i, [c_p, c_i, c_i, c_i, c_p, c_p, c_i, c_i, c_i, c_p]),
+    "mvit_ns_matrix_bytes": (c_i, []),
+    "mvit_newton_schulz_workspace_bytes": (c_l, [c_p, c_i, c_i]),
+    "mvit_newton_schulz": (c_i, [c_p, c_i, c_i, c_i, c_f, c_f, c_f, c_i, c_f, c_i, c_p, c_l, c_p]),
+    "mvit_muon_step": (c_i, [c_p, c_i, c_f, c_f, c_f, c_i, c_f, c_f, c_f, c_i, c_f, c_i, c_p, c_p, c_p, c_l, c_p]),
     "mvit_reduce_queue_begin": (c_i, []),
     "mvit_reduce_queue_flush": (c_i, [c_p]),
 }

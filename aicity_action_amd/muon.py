@@ -1,0 +1,169 @@
+"""Orthogonalised updates for weight matrices: Newton-Schulz products and the Muon step, on csrc/newton_schulz.hip.
+
+``orthogonalize`` pushes the singular values of matrices to about one; ``MuonMatrices`` renews the momenta of a set of weights and steps
+each weight by its orthogonalised momentum, all matrices in the same 17 launches whatever their sizes.  ``solver.construct_optimizer``
+builds a train step on it (``SOLVER.OPTIMIZING_METHOD muon``); the reference's own methods are those of slowfast/models/optimizer.py:140-206.
+Everything runs on the tensors' device and its current stream; there is no CPU fallback."""
+import math
+
+import numpy as np
+import torch
+
+from . import _hip
+
+QUINTIC = (3.4445, -4.7750, 2.0315)       # a, b, c of X <- a X + (b A + c A A) X: steep at zero, between 0.68 and 1.21 from 0.1 on after five steps
+_REC = np.dtype([("u", "u8"), ("w", "u8"), ("m", "u8"), ("out", "u8"), ("rs", "i8"), ("cs", "i8"), ("rows", "i4"), ("cols", "i4"),
+                 ("scale", "f4"), ("pad", "i4")])
+_ARITHMETIC = {"fp16": 0, "split": 1}
+
+
+def _check_iteration(steps, coefficients, eps, arithmetic):
+    if not 1 <= int(steps) <= 100:
+        raise ValueError("Newton-Schulz: 1 to 100 steps, got %r" % (steps,))
+    if len(coefficients) != 3 or not all(math.isfinite(c) for c in coefficients):
+        raise ValueError("Newton-Schulz: three finite coefficients, got %r" % (coefficients,))
+    if not (math.isfinite(eps) and eps > 0.0):
+        raise ValueError("Newton-Schulz: eps must be positive, got %r" % (eps,))
+    if arithmetic not in _ARITHMETIC:
+        raise ValueError("Newton-Schulz: arithmetic must be 'fp16' or 'split', got %r" % (arithmetic,))
+
+
+def _workspace(L, rec, split, device):
+    n = L.mvit_newton_schulz_workspace_bytes(rec.ctypes.data, len(rec), split)
+    _hip.check(min(int(n), 0), "newton_schulz (sizes)")
+    # from torch's allocator, per call: ordered with the stream, and a captured call owns its own
+    return torch.empty(int(n), dtype=torch.uint8, device=device), int(n)
+
+
+def orthogonalize(update, steps=5, coefficients=QUINTIC, eps=1e-7, dtype=torch.bfloat16, arithmetic=None):
+    """Newton-Schulz orthogonalisation of one matrix, a batch [..., rows, columns] or a list of either (sizes may differ; one set of
+    launches for all).  float32 / bfloat16 / float16, any strides.  Returns contiguous tensors of ``dtype``.
+
+    ``arithmetic``: "fp16" (default for 16-bit results; within about 2e-3) computes the products from fp16 operands, "split" (default for
+    float32; 1e-5) from pairs of them at three times the work.  A matrix of zeros stays zero; one with NaN or infinity gives NaN."""
+    many = isinstance(update, (list, tuple))
+    ts = list(update) if many else [update]
+    if arithmetic is None:
+        arithmetic = "split" if dtype == torch.float32 else "fp16"
+    _check_iteration(steps, coefficients, eps, arithmetic)
+    if dtype not in (torch.float32, torch.bfloat16, torch.float16):
+        raise TypeError("orthogonalize: dtype must be float32, bfloat16 or float16, got %s" % dtype)
+    if not ts:
+        return []
+    for t in ts:
+        if t.dim() < 2:
+            raise ValueError("orthogonalize: matrices [..., rows, columns], got %s" % (tuple(t.shape),))
+        if t.dtype not in (torch.float32, torch.bfloat16, torch.float16):
+            raise TypeError("orthogonalize: float32, bfloat16 or float16, got %s" % t.dtype)
+        if t.dtype != ts[0].dtype or t.device != ts[0].device:
+            raise ValueError("orthogonalize: all updates must have one dtype and one device")
+        if t.requires_grad and torch.is_grad_enabled():
+            raise RuntimeError("orthogonalize has no backward pass: call it under torch.no_grad() or on detached updates")
+    if not ts[0].is_cuda:
+        raise RuntimeError("orthogonalize needs its updates on a gfx950 device; there is no CPU fallback")
+    if ts[0].dtype != torch.float32 and dtype != torch.float32 and ts[0].dtype != dtype:
+        ts = [t.float() for t in ts]                # bfloat16 and float16 are different libraries
+    half = torch.float16 in (ts[0].dtype, dtype)
+    with torch.cuda.device(ts[0].device), torch.no_grad():
+        outs = [torch.empty(t.shape, dtype=dtype, device=t.device) for t in ts]
+        rows = []
+        for t, o in zip(ts, outs):
+            if t.numel() == 0:
+                continue
+            size, osize = t.element_size(), o.element_size()
+            r, c = t.shape[-2:]
+            for i, at in enumerate(np.ndindex(*t.shape[:-2])):
+                rows.append((t.data_ptr() + size * sum(a * s for a, s in zip(at, t.stride())), 0, 0, o.data_ptr() + osize * i * r * c,
+                             t.stride(-2), t.stride(-1), r, c, 0.0, 0))
+        if rows:
+            rec = np.array(rows, dtype=_REC)
+            L = _hip.lib("fp16" if half else "bf16")
+            split = _ARITHMETIC[arithmetic]
+            ws, n = _workspace(L, rec, split, ts[0].device)
+            code = lambda d: _hip.F32 if d == torch.float32 else _hip.BF16  # noqa: E731
+            _hip.check(L.mvit_newton_schulz(rec.ctypes.data, len(rec), code(ts[0].dtype), code(dtype), *[float(v) for v in coefficients],
+                                            int(steps), float(eps), split, _hip.ptr(ws), n, torch.cuda.current_stream().cuda_stream),
+                       "newton_schulz")
+    return outs if many else outs[0]
+
+
+class MuonMatrices(object):
+    """A set of weight matrices and their momenta, stepped together.
+
+    ``step``:  M <- mu M + (1 - mu) g;  U = (1 - mu) g + mu M (Nesterov) or M;  W <- W (1 - lr weight_decay) - lr rms sqrt(max(rows,
+    columns)) NS(U).  ``rms`` 0.2 gives the update the size that AdamW's typically has, so that one learning rate and weight decay serve
+    both.  Weights and momenta: contiguous float32 matrices, updated in place; gradients: float32, any strides."""
+
+    def __init__(self, params, momenta=None, momentum=0.95, nesterov=True, weight_decay=0.0, rms=0.2, steps=5, coefficients=QUINTIC,
+                 eps=1e-7, arithmetic="fp16"):
+        self.params = list(params)
+        if not self.params:
+            raise ValueError("MuonMatrices: no parameters")
+        _check_iteration(steps, coefficients, eps, arithmetic)
+        if not 0.0 <= momentum < 1.0:
+            raise ValueError("MuonMatrices: momentum must be in [0, 1), got %r" % (momentum,))
+        if not (weight_decay >= 0.0 and math.isfinite(weight_decay)) or not (rms > 0.0 and math.isfinite(rms)):
+            raise ValueError("MuonMatrices: weight_decay must not be negative and rms must be positive")
+        if momenta is not None and len(momenta) != len(self.params):
+            raise ValueError("MuonMatrices: %d momenta for %d parameters" % (len(momenta), len(self.params)))
+        for p in self.params:
+            self._check_matrix(p, "parameter")
+        self.momenta = list(momenta) if momenta is not None else [torch.zeros_like(p, requires_grad=False) for p in self.params]
+        for p, m in zip(self.params, self.momenta):
+            self._check_matrix(m, "momentum")
+            if m.shape != p.shape:
+                raise ValueError("MuonMatrices: a momentum of shape %s for a parameter of shape %s" % (tuple(m.shape), tuple(p.shape)))
+        spans = sorted((t.data_ptr(), t.data_ptr() + 4 * t.numel()) for t in self.params + self.momenta)
+        if any(a[1] > b[0] for a, b in zip(spans, spans[1:])):
+            raise ValueError("MuonMatrices: parameters and momenta must not share memory (the same tensor twice?)")
+        self.momentum, self.nesterov, self.weight_decay, self.rms = float(momentum), bool(nesterov), float(weight_decay), float(rms)
+        self.steps, self.coefficients, self.eps, self.arithmetic = int(steps), tuple(float(c) for c in coefficients), float(eps), arithmetic
+
+    def _check_matrix(self, t, what):
+        if t.dim() != 2 or t.numel() == 0:
+            raise ValueError("MuonMatrices: every %s must be a matrix, got shape %s" % (what, tuple(t.shape)))
+        if t.dtype != torch.float32 or not t.is_contiguous():
+            raise ValueError("MuonMatrices: every %s must be contiguous float32, got %s with strides %s" % (what, t.dtype, t.stride()))
+        if t.device != self.params[0].device:
+            raise ValueError("MuonMatrices: parameters and momenta must be on one device")
+
+    def step(self, grads=None, lr=None, norm_coef=None, hyper=None):
+        """One step with ``grads`` (default: each parameter's ``.grad``; a parameter whose gradient is None is left as it is).
+
+        ``norm_coef``: two floats on the device, mvit_grad_norm's [norm, factor]: gradients are multiplied by the factor, and a norm or
+        factor that is not finite leaves weights and momenta as they are.  ``hyper``: device floats whose first is the learning rate, read
+        by the kernels in place of ``lr`` (a captured step is replayed with new values)."""
+        if (lr is None) == (hyper is None):
+            raise ValueError("MuonMatrices.step: give the learning rate either as lr or in hyper")
+        if lr is not None and not math.isfinite(lr):
+            raise ValueError("MuonMatrices.step: lr must be finite, got %r" % (lr,))
+        grads = [p.grad for p in self.params] if grads is None else list(grads)
+        if len(grads) != len(self.params):
+            raise ValueError("MuonMatrices.step: %d gradients for %d parameters" % (len(grads), len(self.params)))
+        device, rows, touched = self.params[0].device, [], []
+        for t, n, what in ((norm_coef, 2, "norm_coef"), (hyper, 1, "hyper")):
+            if t is not None and (t.dtype != torch.float32 or t.numel() < n or not t.is_contiguous() or t.device != device):
+                raise ValueError("MuonMatrices.step: %s must be %d contiguous float32 values or more on %s" % (what, n, device))
+        for p, m, g in zip(self.params, self.momenta, grads):
+            if g is None:
+                continue
+            if g.shape != p.shape or g.dtype != torch.float32 or g.device != device:
+                raise ValueError("MuonMatrices.step: a %s gradient of shape %s on %s for a float32 parameter of shape %s on %s"
+                                 % (g.dtype, tuple(g.shape), g.device, tuple(p.shape), device))
+            r, c = p.shape
+            rows.append((g.data_ptr(), p.data_ptr(), m.data_ptr(), 0, g.stride(0), g.stride(1), r, c, self.rms * math.sqrt(max(r, c)), 0))
+            touched += [p, m]
+        if not rows:
+            return
+        if not self.params[0].is_cuda:
+            raise RuntimeError("MuonMatrices needs its parameters on a gfx950 device; there is no CPU fallback")
+        rec = np.array(rows, dtype=_REC)
+        L, split = _hip.lib(), _ARITHMETIC[self.arithmetic]
+        with torch.cuda.device(device):
+            ws, n = _workspace(L, rec, split, device)
+            _hip.check(L.mvit_muon_step(rec.ctypes.data, len(rec), float(lr or 0.0), self.weight_decay, self.momentum, int(self.nesterov),
+                                        *self.coefficients, self.steps, self.eps, split, _hip.ptr(norm_coef), _hip.ptr(hyper), _hip.ptr(ws), n,
+                                        torch.cuda.current_stream().cuda_stream), "muon_step")
+        # written behind torch's back: whatever is cached by version (16-bit weight copies) is refreshed on its next use
+        for t in touched:
+            torch.autograd.graph.increment_version(t)

@@ -386,6 +386,35 @@ int mvit_rotary_tensor_bytes(void);
 int mvit_rotary(const mvit_rotary_tensor* tensors, int ntensors, int dim, int axes, const int* sections, const double* turns, int layout,
                 int inverse, int act_dtype, void* stream);
 
+/* Newton-Schulz orthogonalisation of a set of matrices and the Muon step around it (csrc/newton_schulz.hip):
+ *   X = u / (|u|_F + eps);  steps times:  A = X X^T, X <- a X + (b A + c A A) X   (on the transposed matrix where rows > cols).
+ * mats: HOST array of count records; the matrices may have any sizes (MVIT_EUNSUPPORTED from 2^31 padded elements on) and run together,
+ * in sets of 72.  u: in_dtype-typed, element strides given.
+ *   mvit_newton_schulz: out [rows][cols] of out_dtype.
+ *   mvit_muon_step (fp32):  momentum <- mu momentum + (1 - mu) f u;  update = nesterov ? (1 - mu) f u + mu momentum : momentum;
+ *       w <- w (1 - lr weight_decay) - lr scale NS(update);   w, momentum [rows][cols] contiguous, updated in place.
+ *       norm_coef: NULL (f = 1) or mvit_grad_norm's out2 (f = out2[1]; a non-finite norm or factor leaves w and momentum as they are);
+ *       hyper: NULL or device memory whose first float is the learning rate (captured steps, as mvit_adamw_step_dev).
+ * split 0: products from fp16 operands (result within about 2e-3 of the exact one), 1: from pairs of them (1e-5; three times the work).
+ * workspace: mvit_newton_schulz_workspace_bytes(mats, count, split) bytes (negative: MVIT_E*), 128-byte aligned, used by this call alone. */
+typedef struct {
+    const void* u;
+    float* w;
+    float* momentum;
+    void* out;
+    int64_t row_stride, col_stride;
+    int32_t rows, cols;
+    float scale;
+    int32_t pad;
+} mvit_ns_matrix;
+int mvit_ns_matrix_bytes(void);
+int64_t mvit_newton_schulz_workspace_bytes(const mvit_ns_matrix* mats, int count, int split);
+int mvit_newton_schulz(const mvit_ns_matrix* mats, int count, int in_dtype, int out_dtype, float a, float b, float c, int steps, float eps,
+                       int split, void* workspace, int64_t workspace_bytes, void* stream);
+int mvit_muon_step(const mvit_ns_matrix* mats, int count, float lr, float weight_decay, float momentum, int nesterov, float a, float b,
+                   float c, int steps, float eps, int split, const float* norm_coef, const float* hyper, void* workspace,
+                   int64_t workspace_bytes, void* stream);
+
 #if defined(__GNUC__) || defined(__clang__)
 #pragma GCC visibility pop
 #endif

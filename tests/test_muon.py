@@ -1,0 +1,297 @@
+"""Newton-Schulz orthogonalisation and the Muon step (aicity_action_amd/muon.py) against the definition in 64 bits, and their refusals."""
+import math
+
+import pytest
+import torch
+
+from aicity_action_amd.muon import QUINTIC, MuonMatrices, orthogonalize
+
+gpu = pytest.mark.gpu
+DEV = "cuda:0"
+A, B, C = QUINTIC
+
+
+def definition(u, steps=5, eps=1e-7):
+    u = u.double()
+    x = u / (u.square().sum((-2, -1), keepdim=True).sqrt() + eps)
+    tall = x.shape[-2] > x.shape[-1]
+    x = x.mT.contiguous() if tall else x
+    for _ in range(steps):
+        s = x @ x.mT.contiguous()
+        x = A * x + (B * s + C * (s @ s)) @ x
+    return x.mT if tall else x
+
+
+def rounded(u, split, steps=5, eps=1e-7):
+    """The same with the roundings that the kernels are allowed: X as two fp16 values, A and B as one (split: two) times 2^12, products from
+    the high halves (split: three of the four), sums exact.  Its distance from the definition is the yardstick of the tests below."""
+    def two(x, k):
+        hi = (x * k).half().double()
+        return hi / k, ((x * k) - hi).half().double() / k
+
+    def mul(p, q):
+        return p[0] @ q[0] + (p[0] @ q[1] + p[1] @ q[0] if split else 0.0)
+    u = u.double()
+    x = (u / (u.square().sum((-2, -1), keepdim=True).sqrt() + eps)).float().double()
+    tall = x.shape[-2] > x.shape[-1]
+    x = x.mT.contiguous() if tall else x
+    s = 4096.0
+    x = two(x, s)
+    for _ in range(steps):
+        xt = tuple(v.mT.contiguous() for v in x)
+        g = two(mul(x, xt), s)
+        g = g if split else (g[0], 0.0 * g[0])
+        p = two(B * (g[0] + g[1]) + C * mul(g, g), s)
+        full = A * (x[0] + x[1]) + mul(p, x)
+        x = two(full, s)
+    return full.mT if tall else full
+
+
+def near(got, u, split, steps=5):
+    """Twice the yardstick (another order of roundings and sums), the fp32 sums of K products (2^-24 sqrt(K) of B X and the like, amplified
+    with the rest: under 2e-5), and one rounding to the result's type."""
+    want = definition(u, steps)
+    norm = want.norm().item()
+    tol = 2 * (rounded(u, split, steps) - want).norm().item() + (2e-5 + torch.finfo(got.dtype).eps / 2) * norm
+    err = (got.double() - want).norm().item()
+    assert err <= tol, (err / norm, tol / norm)
+
+
+def gradient(r, c, seed, fall=2.0, noise=0.1):
+    """Like a weight's gradient: a falling spectrum over noise."""
+    g = torch.Generator().manual_seed(seed)
+    k = min(r, c, 16)
+    s = torch.logspace(0, -fall, k) if k > 1 else torch.ones(1)
+    return ((torch.randn(r, k, generator=g) * s) @ torch.randn(k, c, generator=g) + noise * torch.randn(r, c, generator=g)).to(DEV)
+
+
+SHAPES = [(1, 1), (1, 5), (7, 1), (3, 2), (16, 16), (63, 65), (64, 64), (96, 288), (288, 96), (130, 70), (200, 333), (513, 129), (18, 768), (768, 18)]
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("shape", SHAPES)
+def test_orthogonalize(shape, dtype):
+    for seed, (fall, noise) in enumerate(((0.0, 1.0), (2.0, 0.1), (3.0, 0.001))):
+        u = gradient(*shape, seed, fall, noise) * 1e-4
+        near(orthogonalize(u, dtype=dtype), u, dtype == torch.float32)
+
+
+@gpu
+def test_other_arithmetic_input_types_and_steps():
+    u = gradient(100, 150, 3)
+    near(orthogonalize(u, dtype=torch.float32, arithmetic="fp16"), u, False)
+    near(orthogonalize(u, dtype=torch.bfloat16, arithmetic="split"), u, True)
+    for steps in (1, 2, 3, 7):
+        near(orthogonalize(u, steps=steps, dtype=torch.float32), u, True, steps)
+        near(orthogonalize(u.t(), steps=steps, dtype=torch.bfloat16), u.t(), False, steps)
+    for dt in (torch.bfloat16, torch.float16):
+        v = u.to(dt)
+        for out in (torch.bfloat16, torch.float16, torch.float32):
+            got = orthogonalize(v, dtype=out)
+            assert got.dtype == out
+            near(got, v, out == torch.float32)
+
+
+@gpu
+def test_strides_batches_and_lists():
+    big = gradient(300, 400, 5)
+    views = [big[3:90, 7:200], big[::3, ::2], big.t()[:50, 1:301], big[:, 5:6], big[8:9], big[:1, :1].expand(40, 60)]
+    for got, v in zip(orthogonalize(views, dtype=torch.float32), views):
+        assert got.shape == v.shape and got.is_contiguous()
+        near(got, v.clone(), True)
+    batch = torch.stack([gradient(70, 40, s) for s in range(6)]).view(2, 3, 70, 40)
+    got = orthogonalize(batch.transpose(0, 1), dtype=torch.bfloat16)
+    assert got.shape == (3, 2, 70, 40)
+    for i in range(3):
+        for j in range(2):
+            near(got[i, j], batch[j, i], False)
+            # a matrix comes out the same beside others and alone
+            assert torch.equal(got[i, j], orthogonalize(batch[j, i], dtype=torch.bfloat16))
+    many = [gradient(1 + s % 7, 2 + s % 5, s) for s in range(150)]       # more than one set of launches
+    for got, v in zip(orthogonalize(many, dtype=torch.float32), many):
+        near(got, v, True)
+    assert orthogonalize([]) == [] and orthogonalize(torch.empty(0, 3, 4, device=DEV)).shape == (0, 3, 4)
+    assert orthogonalize(torch.empty(3, 0, device=DEV)).shape == (3, 0)
+
+
+@gpu
+@pytest.mark.parametrize("shape", [(2048, 4096), (4160, 2112)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_large_matrices(shape, dtype):
+    u = gradient(*shape, 1)
+    near(orthogonalize(u, dtype=dtype), u, dtype == torch.float32)
+
+
+@gpu
+def test_degenerate_values():
+    u = gradient(50, 70, 2)
+    near(orthogonalize(u * 1e-5, dtype=torch.float32), u * 1e-5, True)
+    for scale in (1e-30, 1e30):                 # (against eps = 1e-7 an update of 1e-30 is nothing: it comes out as small as it is)
+        got = orthogonalize(u * scale, dtype=torch.float32)
+        assert torch.isfinite(got).all()
+        if scale > 1:
+            near(got, u * scale, True)
+        else:
+            assert got.abs().max() < 1e-15
+    zero, nan = torch.zeros(50, 70, device=DEV), u.clone()
+    nan[3, 4] = math.nan
+    outs = orthogonalize([u, zero, nan, u], dtype=torch.bfloat16)
+    assert torch.equal(outs[1], zero.bfloat16()) and torch.equal(outs[0], outs[3]) and torch.isnan(outs[2].float()).all()
+    near(outs[0], u, False)
+    same = torch.ones(40, 60, device=DEV)       # rank one
+    near(orthogonalize(same, dtype=torch.float32), same, True)
+
+
+def muon_definition(w, m, g, lr, mu, nesterov, wd, factor=1.0, rms=0.2):
+    w, m, g = w.double(), m.double(), g.double() * factor
+    m = mu * m + (1 - mu) * g
+    u = (1 - mu) * g + mu * m if nesterov else m
+    return u, w * (1 - lr * wd), lr * rms * math.sqrt(max(w.shape)), m
+
+
+def check_step(w1, m1, w, m, g, lr, mu, nesterov, wd, factor=1.0, split=False):
+    u, kept, step, m_want = muon_definition(w, m, g, lr, mu, nesterov, wd, factor)
+    assert ((m1 - m_want).abs() <= 3 * 2.0 ** -23 * (mu * m.double().abs() + (1 - mu) * (g.double() * factor).abs())).all()
+    o = definition(u)
+    tol = step * (2 * (rounded(u, split) - o).norm().item() + 2e-5 * o.norm().item()) + 2.0 ** -22 * kept.norm().item()
+    err = (w1.double() - (kept - step * o)).norm().item()
+    assert err <= tol, (err, tol)
+
+
+MATS = [(96, 288), (288, 96), (1, 300), (77, 1), (130, 70), (64, 64), (18, 768)]
+
+
+@gpu
+@pytest.mark.parametrize("nesterov", [True, False])
+@pytest.mark.parametrize("arithmetic", ["fp16", "split"])
+def test_muon_step(nesterov, arithmetic):
+    ws = [0.02 * gradient(r, c, 10 + i, 0.0, 1.0) for i, (r, c) in enumerate(MATS)]
+    ms = [1e-3 * gradient(r, c, 30 + i) for i, (r, c) in enumerate(MATS)]
+    gs = [gradient(r, c, 50 + i) for i, (r, c) in enumerate(MATS)]
+    gs[4] = gs[4].t().contiguous().t()                                       # a gradient in another order
+    gs[5] = torch.cat([gs[5], gs[5]], 1)[:, 1:65]                            # and one that is not aligned
+    w0, m0, g0 = [w.clone() for w in ws], [m.clone() for m in ms], [g.clone() for g in gs]
+    plan = MuonMatrices(ws, ms, momentum=0.9, nesterov=nesterov, weight_decay=0.05, arithmetic=arithmetic)
+    versions = [w._version for w in ws]
+    gs[2] = None
+    plan.step(gs, lr=0.01)
+    for i, g in enumerate(g0):
+        if gs[i] is None:
+            assert torch.equal(ws[i], w0[i]) and torch.equal(ms[i], m0[i]) and ws[i]._version == versions[i]
+            continue
+        assert torch.equal(gs[i], g) and ws[i]._version > versions[i]
+        check_step(ws[i], ms[i], w0[i], m0[i], g, 0.01, 0.9, nesterov, 0.05, split=arithmetic == "split")
+    # the same inputs give the same bits
+    again_w, again_m = [w.clone() for w in w0], [m.clone() for m in m0]
+    MuonMatrices(again_w, again_m, momentum=0.9, nesterov=nesterov, weight_decay=0.05, arithmetic=arithmetic).step(gs, lr=0.01)
+    assert all(torch.equal(a, b) for a, b in zip(again_w + again_m, ws + ms))
+
+
+@gpu
+def test_muon_factor_guard_and_grad_attribute():
+    w, g = torch.nn.Parameter(0.02 * gradient(40, 60, 1)), gradient(40, 60, 2)
+    plan, w0 = MuonMatrices([w], weight_decay=0.1), w.detach().clone()
+    w.grad = g
+    coef = torch.tensor([5.0, 0.25], device=DEV)
+    plan.step(lr=0.02, norm_coef=coef)
+    check_step(w.detach(), plan.momenta[0], w0, torch.zeros_like(w0), g, 0.02, 0.95, True, 0.1, factor=0.25)
+    w1, m1 = w.detach().clone(), plan.momenta[0].clone()
+    for bad in ((math.inf, 0.0), (math.nan, 1.0), (1.0, math.nan)):
+        plan.step(lr=0.02, norm_coef=torch.tensor(bad, device=DEV))
+        assert torch.equal(w.detach(), w1) and torch.equal(plan.momenta[0], m1)
+    w.grad = None
+    plan.step(lr=0.02)
+    assert torch.equal(w.detach(), w1)
+
+
+@gpu
+def test_two_captured_steps_replayed_in_turn():
+    """Two graphs of two plans (each capture owns its workspace), replayed alternately with eager work between, against eager steps."""
+    def build(seed):
+        ws = [0.02 * gradient(r, c, seed + i) for i, (r, c) in enumerate(MATS[:4])]
+        return ws, [torch.zeros_like(w) for w in ws], [torch.empty_like(w) for w in ws]
+    sides = [build(100), build(200)]
+    lrs = [torch.zeros(1, device=DEV) for _ in sides]
+    graphs, plans = [], []
+    for (ws, ms, gs), lr in zip(sides, lrs):
+        plan = MuonMatrices(ws, ms)
+        graph = torch.cuda.CUDAGraph()
+        torch.cuda.synchronize()
+        with torch.cuda.graph(graph):
+            plan.step(gs, hyper=lr)
+        graphs.append(graph)
+        plans.append(plan)
+    twins = [([w.clone() for w in ws], [m.clone() for m in ms]) for ws, ms, _ in sides]
+    twin_plans = [MuonMatrices(ws, ms) for ws, ms in twins]
+    for turn in range(4):
+        for k, (ws, ms, gs) in enumerate(sides):
+            for i, g in enumerate(gs):
+                g.copy_(gradient(*g.shape, 1000 * turn + 10 * k + i))
+            lrs[k].fill_(0.01 / (turn + 1))
+            graphs[k].replay()
+            twin_plans[k].step(gs, hyper=lrs[k])
+            torch.cuda.synchronize()
+            for got, want in zip(ws + ms, twins[k][0] + twins[k][1]):
+                assert torch.equal(got, want)
+
+
+@gpu
+def test_side_stream_matches():
+    u = [gradient(300, 200, s) for s in range(3)]
+    want = orthogonalize(u)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = orthogonalize(u)
+    torch.cuda.current_stream().wait_stream(side)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_refusals():
+    u = torch.zeros(4, 6)
+    for kw in (dict(steps=0), dict(steps=101), dict(coefficients=(1.0, 2.0)), dict(coefficients=(1.0, 2.0, math.nan)), dict(eps=0.0),
+               dict(eps=math.inf), dict(arithmetic="bf16")):
+        with pytest.raises(ValueError, match="Newton-Schulz"):
+            orthogonalize(u, **kw)
+        with pytest.raises(ValueError, match="Newton-Schulz"):
+            MuonMatrices([u], **kw)
+    with pytest.raises(ValueError, match="matrices"):
+        orthogonalize(u[0])
+    for bad in (u.double(), u.long()):
+        with pytest.raises(TypeError):
+            orthogonalize(bad)
+    with pytest.raises(TypeError):
+        orthogonalize(u, dtype=torch.float64)
+    with pytest.raises(ValueError, match="one dtype"):
+        orthogonalize([u, u.half()])
+    with pytest.raises(RuntimeError, match="no backward"):
+        orthogonalize(u.clone().requires_grad_(True))
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        orthogonalize(u)
+    for kw in (dict(momentum=1.0), dict(momentum=-0.1), dict(weight_decay=-1.0), dict(rms=0.0), dict(momenta=[]), dict(momenta=[torch.zeros(6, 4)])):
+        with pytest.raises(ValueError):
+            MuonMatrices([u], **kw)
+    for bad in ([], [u[0]], [u.half()], [u.t()], [torch.empty(0, 3)]):
+        with pytest.raises(ValueError):
+            MuonMatrices(bad)
+    for params, momenta in (([u, u], None), ([u], [u]), ([u, u[1:3]], None)):
+        with pytest.raises(ValueError, match="share memory"):
+            MuonMatrices(params, momenta)
+    plan = MuonMatrices([u])
+    with pytest.raises(ValueError, match="learning rate"):
+        plan.step([u])
+    with pytest.raises(ValueError, match="learning rate"):
+        plan.step([u], lr=0.1, hyper=torch.zeros(1))
+    for lr in (math.nan, math.inf):
+        with pytest.raises(ValueError, match="finite"):
+            plan.step([u], lr=lr)
+    for grads in ([], [u.half()], [u.t()]):
+        with pytest.raises(ValueError):
+            plan.step(grads, lr=0.1)
+    for kw in (dict(norm_coef=torch.zeros(1)), dict(norm_coef=torch.zeros(2).double())):
+        with pytest.raises(ValueError, match="norm_coef"):
+            plan.step([u], lr=0.1, **kw)
+    plan.step([None], lr=0.1)
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        plan.step([u], lr=0.1)
