@@ -14,6 +14,7 @@ import os
 import torch
 
 from . import _hip
+from .rotary import add_
 
 
 def _st():
@@ -321,7 +322,17 @@ class _BlockFn(torch.autograd.Function):
         o = torch.empty(Mq, Cout, dtype=adt, device=dev)
         lse = torch.empty(B, h, Lq, dtype=torch.float32, device=dev)
         addq = 1 if hx.m.use_query_residual_pool else 0
-        _hip.check(_hip.attention_fwd(L, q, k, v, o, lse, B, h, Lq, Lk, 96 ** -0.5, addq, act, _st()), "attention")
+        rot = hx.m.rotary
+        q_plain = q
+        if rot is not None:       # HIP.ROTARY: q and k turn by their places; the residual keeps the pooled query as it is
+            plan, *grids = rot[g.index]
+            q, k = plan.turn([q, k], grids, outs=None if addq else [q, k])
+        _hip.check(_hip.attention_fwd(L, q, k, v, o, lse, B, h, Lq, Lk, 96 ** -0.5, addq if rot is None else 0, act, _st()), "attention")
+        o_att = o                 # what the attention backward reads (the kernels' own residual is taken out there)
+        if rot is not None and addq:
+            o = o_att.clone()
+            add_(o.view(B, Lq, h, 96).transpose(1, 2), q_plain)
+        del q_plain
         r = x2
         r_full = None
         if _skip_fused(g, act, B):
@@ -359,7 +370,7 @@ class _BlockFn(torch.autograd.Function):
             hid = torch.empty_like(pre)
             _hip.check(L.mvit_gelu_fwd(_hip.ptr(pre), _hip.ptr(hid), pre.numel(), act, _st()), "gelu")
         out = hx.linear(hid, hx.w(blk.mlp.fc2.weight), blk.mlp.fc2.bias, torch.float32, residual=y, row_scale=dp2, rps=Lq)
-        saved = (x2, u, qkv, q, k, v, o, lse, r_full, y, vn, pre, hid, dp1, dp2)
+        saved = (x2, u, qkv, q, k, v, o, o_att, lse, r_full, y, vn, pre, hid, dp1, dp2)
         return out.view(B, Lq, Cout), saved, pool_saved, mlp_dsave
 
     @staticmethod
@@ -388,7 +399,7 @@ class _BlockFn(torch.autograd.Function):
             del xin
         else:
             saved, pool_saved = ctx.saved, ctx.pool_saved
-        x2, u, qkv, q, k, v, o, lse, r_full, y, vn, pre, hid, dp1, dp2 = saved
+        x2, u, qkv, q, k, v, o, o_att, lse, r_full, y, vn, pre, hid, dp1, dp2 = saved
         del saved
         ctx.saved = None
         ctx.pool_saved = None
@@ -449,9 +460,13 @@ class _BlockFn(torch.autograd.Function):
         dkv = torch.empty(2, B, h, Lk, 96, dtype=k.dtype, device=dev)
         dk, dv = dkv[0], dkv[1]
         ws = _ws(L.mvit_attention_bwd_workspace_bytes(B, h, Lq, Lk), dev)
-        _hip.check(_hip.attention_bwd(L, q, k, v, o, lse, d_o, dq, dk, dv, ws, B, h, Lq, Lk, 96 ** -0.5, ctx.addq, act, _st()),
-                   "attention_bwd")
-        del d_o
+        rot = hx.m.rotary
+        _hip.check(_hip.attention_bwd(L, q, k, v, o_att, lse, d_o, dq, dk, dv, ws, B, h, Lq, Lk, 96 ** -0.5, ctx.addq if rot is None else 0,
+                                      act, _st()), "attention_bwd")
+        if rot is not None:       # back from the turned to the pooled q and k, in place; the residual's gradient joins the query's
+            plan, *grids = rot[g.index]
+            plan.turn([dq, dk], grids, outs=[dq, dk], adds=[d_o.view(B, Lq, h, 96).transpose(1, 2) if ctx.addq else None, None], inverse=True)
+        del d_o, o_att
         d_qkv = torch.empty(M, 3 * Cout, dtype=adt, device=dev)
         pws_bytes = max(L.mvit_pool_bwd_workspace_bytes(B, h, T, H, W, g.stride_q[1] if g.stride_q else 1),
                         L.mvit_pool_bwd_workspace_bytes(B, h, T, H, W, g.stride_kv[1]))

@@ -123,10 +123,12 @@ def _defaults():
         # DDP_*: how build_model wraps DistributedDataParallel (gradients live in the all-reduce buckets, static graph; optional
         # bf16 gradient payload: 70.6 MB instead of 141 MB per step over xGMI).  STAT_QUEUE_DEPTH: iterations the training loop may
         # run ahead of the GPU before it waits for a step's scalars (meters.DeviceScalarQueue).  GRAPH_STEP: engine.train_epoch
-        # captures the whole train step in a hipGraph after two eager iterations and replays it (graph_step.py)
+        # captures the whole train step in a hipGraph after two eager iterations and replays it (graph_step.py).  ROTARY: queries and keys
+        # of every block turn by their (t, h, w) places before the attention (rotary.py).  MUON_*: SOLVER.OPTIMIZING_METHOD muon
         "HIP": {"PRECISION": "auto", "STREAMS": 3, "TRAIN_STREAMS": 1, "WGRAD_STREAM": True, "DDP_BUCKET_VIEW": True,
                 "DDP_STATIC_GRAPH": True, "DDP_BF16_GRADS": False, "STAT_QUEUE_DEPTH": 2, "GRAPH_STEP": False,
-                "REL_POS_BIAS": False},
+                "REL_POS_BIAS": False, "ROTARY": False, "ROTARY_BASE": 10000.0, "MUON_MOMENTUM": 0.95, "MUON_NESTEROV": True,
+                "MUON_STEPS": 5},
     }
 
 

@@ -20,6 +20,7 @@ import torch
 import torch.nn as nn
 
 from .. import _hip
+from ..rotary import AxialRotary, TokenGrid, add_
 from .build import MODEL_REGISTRY
 from .spec import derive_block_geoms
 
@@ -98,6 +99,8 @@ _TAIL_FUSE = os.environ.get("MVIT_TAIL_FUSE", "1") != "0"
 
 @MODEL_REGISTRY.register()
 class MViT(nn.Module):
+    rotary = None      # per block: (plan, places of the queries, places of the keys) where HIP.ROTARY is on
+
     def __init__(self, cfg):
         super().__init__()
         assert cfg.DATA.TRAIN_CROP_SIZE == cfg.DATA.TEST_CROP_SIZE   # video_model_builder.py:805
@@ -149,6 +152,13 @@ class MViT(nn.Module):
                 _unsupported(bool(st) and (st[0] != 1 or st[1] != st[2]), "pool stride %s" % (st,))
             _unsupported(bool(g.stride_q) and g.stride_q[1] not in (1, 2), "q stride %s" % (g.stride_q,))
         self.geoms = geoms
+        # HIP.ROTARY (not in the reference): rotary (t, h, w) places for the pooled queries and keys of every block, in units of the
+        # block's input tokens (a token pooled with stride s stands at every s-th of them).  Values and the pooled-query residual are not turned
+        hip = getattr(cfg, "HIP", None)
+        if bool(getattr(hip, "ROTARY", False)):
+            plan = AxialRotary(96, base=getattr(hip, "ROTARY_BASE", 10000.0))
+            self.rotary = [(plan, TokenGrid(g.thw_q, step=g.stride_q if g.kernel_q else None),
+                            TokenGrid(g.thw_kv, step=g.stride_kv)) for g in geoms]
 
         embed_dim = mv.EMBED_DIM
         self.patch_embed = _PatchEmbed(cfg.DATA.INPUT_CHANNEL_NUM[0], embed_dim, mv.PATCH_KERNEL, mv.PATCH_STRIDE,
@@ -565,22 +575,29 @@ class MViT(nn.Module):
         if "pool" in ex:
             q, kv = q.to(adt), kv.to(adt)
             k, v = kv[0], kv[1]
+        addq = 1 if self.use_query_residual_pool else 0
+        q_plain = q
+        if self.rotary is not None:      # q and k turn by their places; the residual keeps the pooled query as it is
+            plan, *grids = self.rotary[g.index]
+            q, k = plan.turn([q, k], grids, outs=None if addq else [q, k])
         # 4. fused attention (+ pooled-q residual), heads merged on store   attention.py:267-279
         if "attention" in ex:
             o = torch.empty(B * Lq, Cout, dtype=torch.float32, device=dev)
             _hip.check(_hip.attention_fwd(L, q.float(), k.float(), v.float(), o, None, B, h, Lq, Lk, 96 ** -0.5,
-                                          1 if self.use_query_residual_pool else 0, _hip.F32, st), "attention")
+                                          addq if self.rotary is None else 0, _hip.F32, st), "attention")
             o = o.to(adt)
         else:
             o = torch.empty(B * Lq, Cout, dtype=adt, device=dev)
-            _hip.check(_hip.attention_fwd(L, q, k, v, o, None, B, h, Lq, Lk, 96 ** -0.5, 1 if self.use_query_residual_pool else 0, act, st),
+            _hip.check(_hip.attention_fwd(L, q, k, v, o, None, B, h, Lq, Lk, 96 ** -0.5, addq if self.rotary is None else 0, act, st),
                        "attention")
+        if self.rotary is not None and addq:
+            add_(o.view(B, Lq, h, 96).transpose(1, 2), q_plain)
         if taps is not None:
             taps["block%d.q" % g.index] = q
             taps["block%d.k" % g.index] = k
             taps["block%d.v" % g.index] = v
             taps["block%d.attn_out" % g.index] = o.view(B, Lq, Cout)
-        del q, k, v
+        del q, k, v, q_plain
         # 5. skip path: channel expand on the un-normed x, then max-pool     attention.py:424-432
         r = x.view(M, Cin)
         from ..autograd import _skip_fused

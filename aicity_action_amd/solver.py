@@ -5,7 +5,8 @@ Mirrors the reference's ``construct_optimizer`` parameter grouping and AdamW hyp
 ``model.no_weight_decay()`` too), ``set_lr`` (:224-236), the cosine + linear warm-up policy
 (slowfast/utils/lr_policy.py:9-53) and ``clip_grad_norm_(params, SOLVER.CLIP_GRAD_L2NORM)``
 (tools/train_net.py:239-243).  The arithmetic is two kernels per step (global grad norm, fused AdamW) over a device
-table of chunk descriptors instead of ~350 small kernels.
+table of chunk descriptors instead of ~350 small kernels.  ``HipMuon`` (not in the reference) steps the blocks' weight matrices by
+their orthogonalised momenta (muon.py) and everything else by the same AdamW.
 """
 import math
 
@@ -13,6 +14,7 @@ import numpy as np
 import torch
 
 from . import _hip
+from .muon import MuonMatrices
 
 _CHUNK = 65536
 _DT = np.dtype([("p", "u8"), ("g", "u8"), ("m", "u8"), ("v", "u8"), ("n", "i4"), ("wd", "f4")])
@@ -61,7 +63,7 @@ class HipAdamW(object):
     """AdamW(betas (0.9, 0.999), eps 1e-8) with fused global-norm clipping, fp32 state."""
 
     def __init__(self, model, cfg):
-        if cfg.SOLVER.OPTIMIZING_METHOD not in ("adamw", "zero_adamw"):
+        if cfg.SOLVER.OPTIMIZING_METHOD not in ("adamw", "zero_adamw", "muon"):
             raise NotImplementedError("Does not support {} optimizer".format(cfg.SOLVER.OPTIMIZING_METHOD))
         self.cfg = cfg
         self.lr = cfg.SOLVER.BASE_LR
@@ -444,9 +446,82 @@ class HipZeroAdamW(HipAdamW):
             self._gathered = None                       # one-shot: the other ranks' moments are not kept
 
 
+class HipMuon(HipAdamW):
+    """``SOLVER.OPTIMIZING_METHOD muon``: the weight matrices of the blocks (qkv, proj, fc1, fc2, proj_max_pool) step by their
+    orthogonalised momenta (``muon.MuonMatrices``), every other parameter -- biases, norms, convolutions, embeddings, the head -- by AdamW.
+    One learning rate, weight decay and global-norm clip serve both (the matrices' update has the size AdamW's typically has).  Momentum,
+    Nesterov and the number of Newton-Schulz steps: ``HIP.MUON_*``; HIP.PRECISION fp32 computes the products from pairs of fp16 values.
+    Every rank of a DistributedDataParallel run takes the whole step on the gradients it holds (the kernels add in a fixed order, so the
+    ranks stay equal bit by bit).  Gradient clipping, the loss scaler, the guard against a non-finite norm and the captured step
+    (HIP.GRAPH_STEP) work as for AdamW."""
+
+    def __init__(self, model, cfg):
+        super().__init__(model, cfg)
+        hip = getattr(cfg, "HIP", None)
+        self._hyper = None
+        self._matrices = None
+        if self.groups[0]["params"]:
+            self._matrices = MuonMatrices(self.groups[0]["params"], momentum=getattr(hip, "MUON_MOMENTUM", 0.95),
+                                          nesterov=bool(getattr(hip, "MUON_NESTEROV", True)), steps=getattr(hip, "MUON_STEPS", 5),
+                                          weight_decay=cfg.SOLVER.WEIGHT_DECAY,
+                                          arithmetic="split" if getattr(hip, "PRECISION", "auto") == "fp32" else "fp16")
+
+    def _make_groups(self, model, cfg):
+        decay, no_decay = param_groups(model, cfg)
+        matrix = lambda n, p: p.ndim == 2 and n.startswith("blocks.")  # noqa: E731
+        parts = ([x for x in decay if matrix(*x)], [x for x in decay if not matrix(*x)], no_decay)
+        return [{"params": [p for _, p in part], "names": [n for n, _ in part], "weight_decay": wd}
+                for part, wd in zip(parts, (cfg.SOLVER.WEIGHT_DECAY, cfg.SOLVER.WEIGHT_DECAY, 0.0))]
+
+    def _ownership(self):
+        return {p for grp in self.groups[1:] for p in grp["params"]}      # AdamW's part of the chunk table
+
+    def step(self, max_norm=None, grad_scale=None, hyper=None):
+        self._hyper = hyper
+        try:
+            return super().step(max_norm, grad_scale, hyper)
+        finally:
+            self._hyper = None
+
+    def _after_update(self):
+        if self._matrices is not None:
+            self._matrices.step(lr=self.lr if self._hyper is None else None, norm_coef=self._out2, hyper=self._hyper)
+
+    def state_dict(self):
+        """AdamW's layout with the matrices as the first group: their entries hold ``momentum_buffer``."""
+        sd = super().state_dict()
+        if self._matrices is not None:
+            for i, m in enumerate(self._matrices.momenta):
+                sd["state"][i] = {"step": torch.tensor(float(self.step_count)), "momentum_buffer": m.detach().clone()}
+            grp = sd["param_groups"][0]
+            for key in ("betas", "eps", "amsgrad"):
+                del grp[key]
+            grp.update(momentum=self._matrices.momentum, nesterov=self._matrices.nesterov, ns_steps=self._matrices.steps)
+        return sd
+
+    def load_state_dict(self, sd):
+        if "param_groups" not in sd:
+            raise ValueError("loaded optimizer state is not one of SOLVER.OPTIMIZING_METHOD muon")
+        n = len(self.groups[0]["params"])
+        entries = [sd["state"].get(i) for i in range(n)]
+        for i, ent in enumerate(entries):
+            have = None if ent is None or "momentum_buffer" not in ent else tuple(ent["momentum_buffer"].shape)
+            if ent is not None and have != tuple(self.groups[0]["params"][i].shape):
+                raise ValueError("optimizer state %d (%s): momentum_buffer has shape %s, the parameter %s" % (
+                    i, self.groups[0]["names"][i], have, tuple(self.groups[0]["params"][i].shape)))
+        super().load_state_dict(sd)
+        for i, ent in enumerate(entries):
+            if ent is not None:
+                self._matrices.momenta[i].copy_(ent["momentum_buffer"])
+                self.step_count = int(float(ent["step"]))
+
+
 def construct_optimizer(model, cfg):
     """slowfast/models/optimizer.py:14-206 for the methods the MViT recipes use: ``adamw`` (the README recipe; parameter groups of
-    :56-75) and ``zero_adamw`` (:189-199); anything else raises NotImplementedError as the reference does for unknown names."""
+    :56-75) and ``zero_adamw`` (:189-199); ``muon`` is this framework's own; anything else raises NotImplementedError as the reference does
+    for unknown names."""
+    if cfg.SOLVER.OPTIMIZING_METHOD == "muon":
+        return HipMuon(model, cfg)
     if cfg.SOLVER.OPTIMIZING_METHOD == "zero_adamw":
         return HipZeroAdamW(model, cfg)
     return HipAdamW(model, cfg)

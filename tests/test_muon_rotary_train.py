@@ -1,0 +1,272 @@
+"""Rotary positions (HIP.ROTARY) and the Muon optimiser (SOLVER.OPTIMIZING_METHOD muon) in the model and its training loop."""
+import copy
+
+import pytest
+import torch
+
+import mvit_oracle as O
+from conftest import cfg_for_case, load_golden
+from test_muon import definition, muon_definition, rounded
+from test_rotary import oracle as turned
+
+from aicity_action_amd import engine
+from aicity_action_amd.models import build_model
+from aicity_action_amd.models.mvit import MViT
+from aicity_action_amd.rotary import TokenGrid
+from aicity_action_amd.solver import HipGradScaler, construct_optimizer, soft_target_cross_entropy
+from aicity_action_amd.utils.synth import load_synth_weights, synth_clip
+
+gpu = pytest.mark.gpu
+
+
+def config(name, precision, rotary=True, muon=True, gpus=1):
+    _, meta = load_golden(name)
+    cfg = cfg_for_case(meta, precision, train=True)
+    cfg.NUM_GPUS = gpus
+    cfg.MVIT.DROPPATH_RATE, cfg.MODEL.DROPOUT_RATE = 0.0, 0.0
+    cfg.HIP.ROTARY, cfg.HIP.ROTARY_BASE = rotary, 100.0
+    if muon:
+        cfg.SOLVER.OPTIMIZING_METHOD = "muon"
+    return cfg, meta
+
+
+def model_and_batch(name, precision, **kw):
+    cfg, meta = config(name, precision, **kw)
+    model = build_model(cfg)
+    load_synth_weights(model, meta["weight_seed"])
+    clip = synth_clip(meta["batch"], meta["num_frames"], meta["crop"], meta["clip_seed"])
+    labels = torch.softmax(torch.randn(meta["batch"], cfg.MODEL.NUM_CLASSES, generator=torch.Generator().manual_seed(0)), 1)
+    return cfg, meta, model, clip, labels
+
+
+def rotary_attention(xn, thw, sd, pre, spec, taps=None):
+    """The oracle's attention with turned queries and keys (differentiable, in the inputs' precision)."""
+    B, N, _ = xn.shape
+    h, C = spec.heads, spec.dim_out
+    qkv = torch.nn.functional.linear(xn, sd[pre + "qkv.weight"], sd.get(pre + "qkv.bias")).reshape(B, N, 3, h, C // h).permute(2, 0, 3, 1, 4)
+    q, k, v = qkv[0], qkv[1], qkv[2]
+    q_thw, k_thw, sq, sk = list(thw), list(thw), (1, 1, 1), (1, 1, 1)
+    if len(spec.pool_q) > 0:
+        q, q_thw = O._pool_conv_ln(q, thw, sd[pre + "pool_q.weight"], spec.stride_q, sd[pre + "norm_q.weight"], sd[pre + "norm_q.bias"])
+        sq = spec.stride_q
+    if len(spec.pool_kv) > 0:
+        k, k_thw = O._pool_conv_ln(k, thw, sd[pre + "pool_k.weight"], spec.stride_kv, sd[pre + "norm_k.weight"], sd[pre + "norm_k.bias"])
+        v, _ = O._pool_conv_ln(v, thw, sd[pre + "pool_v.weight"], spec.stride_kv, sd[pre + "norm_v.weight"], sd[pre + "norm_v.bias"])
+        sk = spec.stride_kv
+
+    def turn(x, sizes, step):
+        place = torch.stack([g.reshape(-1) for g in torch.meshgrid(*[torch.arange(n) * float(s) for n, s in zip(sizes, step)], indexing="ij")], -1)
+        f = torch.tensor([100.0 ** (-2.0 * i / 32) for i in range(16)])
+        ang = (place[:, :, None] * f).reshape(-1, 48)                       # [tokens, axis * 16 + pair]
+        c, s = torch.cos(ang), torch.sin(ang)
+        x = x.unflatten(-1, (3, 2, 16))
+        a, b = x[..., 0, :].flatten(-2), x[..., 1, :].flatten(-2)
+        y = torch.stack([(a * c - b * s).unflatten(-1, (3, 16)), (a * s + b * c).unflatten(-1, (3, 16))], -2)
+        return y.flatten(-3)
+    qr, kr = turn(q, q_thw, sq), turn(k, k_thw, sk)
+    # (the helper above against the operator's own oracle, so that the two tests hold each other)
+    assert (qr.detach().double() - turned(q, TokenGrid(q_thw, step=sq), (32, 32, 32), 100.0, "half")[0]).abs().max() <= 1e-5 * q.abs().max()
+    att = ((qr @ kr.transpose(-2, -1)) * (C // h) ** -0.5).softmax(dim=-1)
+    o = (att @ v).transpose(1, 2).reshape(B, q.shape[2], C)
+    if spec.q_residual:
+        o = o + q.transpose(1, 2).reshape(B, q.shape[2], C)
+    return torch.nn.functional.linear(o, sd[pre + "proj.weight"], sd[pre + "proj.bias"]), q_thw
+
+
+@gpu
+@pytest.mark.parametrize("name", ["tiny_even", "tiny_odd", "tiny_plain"])
+def test_rotary_model_matches_the_oracle(name, monkeypatch):
+    """Logits and every gradient of the fp32 path, at the bounds that the model without rotary positions is held to (1e-4 on logits and on
+    gradients relative to max(1, largest)); inference in fp32 likewise."""
+    cfg, meta, model, clip, labels = model_and_batch(name, "fp32")
+    monkeypatch.setattr(O, "attention", rotary_attention)
+    sd = {k: v.detach().cpu().clone().requires_grad_(True) for k, v in model.state_dict().items()}
+    _, want = O.forward(sd, clip, copy.deepcopy(cfg.MVIT.to_dict()), training=False, head_act=False)
+    model.train()
+    logits = model([clip.cuda()])
+    assert (logits.detach().cpu() - want.detach()).abs().max() <= 1e-4
+    O.soft_target_cross_entropy(want, labels).backward()
+    soft_target_cross_entropy(logits, labels.cuda()).backward()
+    for k, p in model.named_parameters():
+        ref = sd[k].grad
+        assert (p.grad.cpu() - ref).abs().max() <= 1e-4 * max(1.0, ref.abs().max().item()), k
+    model.eval()
+    with torch.no_grad():
+        probs = model([clip.cuda()])
+    assert (probs.cpu() - want.detach().softmax(1)).abs().max() <= 1e-4
+    plain = config(name, "fp32", rotary=False)[0]                           # and the option does something
+    other = build_model(plain).eval()
+    other.load_state_dict(model.state_dict())
+    with torch.no_grad():
+        assert not torch.equal(other([clip.cuda()]), probs)
+
+
+@gpu
+@pytest.mark.parametrize("precision", ["bf16", "fp16"])
+def test_rotary_model_in_16_bits(precision):
+    """Inference within the 16-bit bounds of the model without rotary positions (1e-2 for bfloat16, a quarter of it for half), sub-batches
+    on streams included, and a training step whose gradients point where the fp32 path's do."""
+    cfg, meta, model, clip, labels = model_and_batch("tiny_even", precision)
+    exact = build_model(config("tiny_even", "fp32")[0]).eval()
+    exact.load_state_dict(model.state_dict())
+    clips = torch.cat([clip, clip.flip(0)] * 2).cuda()
+    model.eval()
+    with torch.no_grad():
+        assert (model([clips]) - exact([clips])).abs().max() <= (1e-2 if precision == "bf16" else 2.5e-3)
+    scale = 1.0 if precision == "bf16" else 1024.0
+    for m in (model, exact):
+        m.train()
+        (soft_target_cross_entropy(m([clip.cuda()]), labels.cuda()) * scale).backward()
+    a, b = (torch.cat([p.grad.flatten() for p in m.parameters()]).double() for m in (model, exact))
+    assert torch.dot(a, b) / (a.norm() * b.norm()) >= 0.995
+
+
+@gpu
+def test_rotary_with_activation_checkpointing_gives_the_same_gradients():
+    grads = []
+    for ckpt in (False, True):
+        cfg, meta = config("tiny_even", "bf16")
+        cfg.MODEL.ACT_CHECKPOINT = ckpt
+        model = build_model(cfg).train()
+        load_synth_weights(model, meta["weight_seed"])
+        clip = synth_clip(meta["batch"], meta["num_frames"], meta["crop"], meta["clip_seed"]).cuda()
+        model([clip]).square().sum().backward()
+        grads.append([p.grad.clone() for p in model.parameters()])
+    assert all(torch.equal(a, b) for a, b in zip(*grads))
+
+
+def one_backward(model, clip, labels):
+    for p in model.parameters():
+        p.grad = None
+    soft_target_cross_entropy(model([clip.cuda()]), labels.cuda()).backward()
+
+
+@gpu
+@pytest.mark.parametrize("precision,scaled", [("fp32", False), ("bf16", False), ("fp16", True)])
+def test_muon_train_step(precision, scaled):
+    """Matrices against the definition in 64 bits on the clipped gradients, the rest bit for bit as HipAdamW takes it."""
+    cfg, meta, model, clip, labels = model_and_batch("tiny_even", precision)
+    opt = construct_optimizer(model.train(), cfg)
+    twin_cfg = copy.deepcopy(cfg)
+    twin_cfg.SOLVER.OPTIMIZING_METHOD = "adamw"
+    twin = build_model(twin_cfg).train()
+    twin.load_state_dict(model.state_dict())
+    adamw = construct_optimizer(twin, twin_cfg)
+    names = set(opt.groups[0]["names"])
+    assert names == {n for n, p in model.named_parameters() if n.startswith("blocks.") and p.ndim == 2}
+    assert [sum(p.numel() for g in opt.groups for p in g["params"])] == [sum(p.numel() for p in model.parameters())]
+    lr, mu, split = 1e-3, 0.95, precision == "fp32"
+    momenta = {n: torch.zeros_like(p) for n, p in model.named_parameters()}
+    for step in range(2):
+        scaler = HipGradScaler(init_scale=256.0, enabled=scaled)
+        for m in (model, twin):
+            for p in m.parameters():
+                p.grad = None
+        scaler.scale(soft_target_cross_entropy(model([clip.cuda()]), labels.cuda())).backward()
+        for p, t in zip(model.parameters(), twin.parameters()):
+            t.grad = p.grad.clone()
+            with torch.no_grad():
+                t.copy_(p)
+        before = {n: p.detach().clone() for n, p in model.named_parameters()}
+        for o in (opt, adamw):
+            o.set_lr(lr)
+        out = scaler.step(opt)
+        assert torch.equal(out, HipGradScaler(init_scale=256.0, enabled=scaled).step(adamw))
+        factor = out[1].item()
+        for (n, p), t, m in zip(model.named_parameters(), twin.parameters(), momenta):
+            if n not in names:
+                assert torch.equal(p, t), n
+                continue
+            u, kept, size, m_new = muon_definition(before[n], momenta[n], p.grad, lr, mu, True, cfg.SOLVER.WEIGHT_DECAY, factor)
+            o = definition(u)
+            tol = size * (2 * (rounded(u, split) - o).norm() + 2e-5 * o.norm()) + 2.0 ** -22 * kept.norm()
+            assert (p.detach().double() - (kept - size * o)).norm() <= tol, n
+            momenta[n] = m_new.float()
+
+
+@gpu
+def test_muon_checkpoint_resume_and_non_finite_steps(tmp_path):
+    cfg, meta, model, clip, labels = model_and_batch("tiny_odd", "bf16")
+    opt = construct_optimizer(model.train(), cfg)
+    for _ in range(2):
+        one_backward(model, clip, labels)
+        opt.step()
+    cfg.OUTPUT_DIR = str(tmp_path)
+    engine.save_checkpoint(cfg.OUTPUT_DIR, model, opt, 0, cfg)
+    again = build_model(cfg).train()
+    opt2 = construct_optimizer(again, cfg)
+    cfg.TRAIN.AUTO_RESUME = True
+    assert engine.load_train_checkpoint(cfg, again, opt2) == 1
+    assert opt2.step_count == 2 and all(torch.equal(a, b) for a, b in zip(opt._matrices.momenta, opt2._matrices.momenta))
+    for m, o in ((model, opt), (again, opt2)):
+        one_backward(m, clip, labels)
+        o.step()
+    assert all(torch.equal(a, b) for a, b in zip(model.parameters(), again.parameters()))
+    before = [t.clone() for t in list(model.parameters()) + opt._matrices.momenta]
+    one_backward(model, clip, labels)
+    next(model.parameters()).grad.view(-1)[0] = float("nan")
+    opt.step()
+    assert all(torch.equal(a, b) for a, b in zip(before, list(model.parameters()) + opt._matrices.momenta))
+
+
+@gpu
+def test_graphed_muon_rotary_step_reproduces_the_eager_step():
+    """The whole step captured in a graph and replayed (graph_step.GraphedTrainStep) against the eager loop, bit for bit."""
+    from aicity_action_amd.graph_step import GraphedTrainStep
+    runs = []
+    for graphed in (False, True):
+        cfg, meta, model, clip, labels = model_and_batch("tiny_even", "bf16")
+        model.train()
+        opt = construct_optimizer(model, cfg)
+        gs = GraphedTrainStep(model, opt, cfg, lambda c, p, l: soft_target_cross_entropy(p, l), engine.topks_correct, 2)
+        stats = []
+        for i in range(6):
+            x = synth_clip(meta["batch"], meta["num_frames"], meta["crop"], 50 + i).cuda()
+            if graphed:
+                stats.append(gs.run(x, labels.cuda(), 1e-3 / (i + 1)))
+            else:
+                opt.set_lr(1e-3 / (i + 1))
+                stats.append(gs._step(x, labels.cuda()))
+            torch.cuda.synchronize()
+        assert not graphed or gs.replays == 4
+        runs.append(stats + [p.detach().clone() for p in model.parameters()] + opt._matrices.momenta)
+    assert all(torch.equal(a, b) for a, b in zip(*runs))
+
+
+def test_rotary_option_and_muon_groups_on_the_host():
+    """What the model and the optimiser set up, without a device."""
+    model = MViT(config("tiny_even", "fp32", gpus=0)[0])
+    assert len(model.rotary) == len(model.geoms) and model.rotary[0][1].tokens == model.geoms[0].lq
+    for (plan, q, k), g in zip(model.rotary, model.geoms):
+        assert plan.sections == (32, 32, 32) and (q.sizes, k.sizes) == (tuple(g.thw_q), tuple(g.thw_kv)) and k.tokens == g.lk
+        assert q.step == tuple(float(s) for s in (g.stride_q or (1, 1, 1))) and k.step == tuple(float(s) for s in g.stride_kv)
+    copied = copy.deepcopy(model)
+    assert list(copied.rotary[0][0]._turns) == list(model.rotary[0][0]._turns) and len(copied.state_dict()) == len(model.state_dict())
+    assert MViT(config("tiny_even", "fp32", rotary=False, gpus=0)[0]).rotary is None
+    cfg, _ = config("tiny_even", "fp32", gpus=0)
+    cfg.HIP.MUON_MOMENTUM, cfg.HIP.MUON_STEPS, cfg.HIP.MUON_NESTEROV = 0.9, 3, False
+    opt = construct_optimizer(model, cfg)
+    assert [len(g["params"]) > 0 for g in opt.groups] == [True] * 3
+    assert (opt._matrices.momentum, opt._matrices.steps, opt._matrices.nesterov, opt._matrices.arithmetic) == (0.9, 3, False, "split")
+    sd = opt.state_dict()
+    n = len(opt.groups[0]["params"])
+    assert all(set(sd["state"][i]) == {"step", "momentum_buffer"} for i in range(n)) and "exp_avg" in sd["state"][n]
+    for i in range(n):
+        sd["state"][i]["momentum_buffer"] += 1.0
+        sd["state"][i]["step"] += 7
+    opt.load_state_dict(sd)
+    assert opt.step_count == 0 or opt.step_count == 7
+    assert all((m == 1.0).all() for m in opt._matrices.momenta)
+    adamw_cfg = copy.deepcopy(cfg)
+    adamw_cfg.SOLVER.OPTIMIZING_METHOD = "adamw"
+    other = construct_optimizer(MViT(adamw_cfg), adamw_cfg)
+    with pytest.raises(ValueError, match="shape|groups"):
+        opt.load_state_dict(other.state_dict())
+    with pytest.raises(ValueError, match="groups"):
+        other.load_state_dict(sd)
+    sd["state"][0]["momentum_buffer"] = sd["state"][0]["momentum_buffer"][:1]
+    with pytest.raises(ValueError, match="momentum_buffer"):
+        opt.load_state_dict(sd)
+    cfg.SOLVER.OPTIMIZING_METHOD = "lion"
+    with pytest.raises(NotImplementedError):
+        construct_optimizer(model, cfg)
