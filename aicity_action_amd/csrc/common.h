@@ -67,6 +67,12 @@ __device__ __forceinline__ uint32_t pack_bf16x2(float lo, float hi) {
     return __builtin_bit_cast(uint32_t, v);
 }
 
+// A product that is rounded by itself: the compiler may not contract it into the sum that uses it.
+__device__ __forceinline__ float rounded_f32(float v) {
+    asm("" : "+v"(v));
+    return v;
+}
+
 template <typename T> struct ActIO;
 template <> struct ActIO<float> {
     static __device__ __forceinline__ float load(const float* p) { return *p; }

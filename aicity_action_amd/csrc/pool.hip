@@ -101,12 +101,12 @@ __global__ __launch_bounds__(256) void pool_conv_ln_kernel(const TA* __restrict_
         for (int e = 0; e < 24; ++e) sum += acc[e];
         sum += __shfl_xor(sum, 1, 64);
         sum += __shfl_xor(sum, 2, 64);
-        const float mean = sum * (1.0f / 96.0f);
+        const float mean = rounded_f32(sum * (1.0f / 96.0f));
         float sq = 0.f;
 #pragma unroll
         for (int e = 0; e < 24; ++e) {
             acc[e] -= mean;
-            sq += acc[e] * acc[e];
+            sq += rounded_f32(acc[e] * acc[e]);
         }
         sq += __shfl_xor(sq, 1, 64);
         sq += __shfl_xor(sq, 2, 64);
@@ -306,12 +306,12 @@ __global__ __launch_bounds__(S == 1 ? 384 : 192, 3) void pool_tiled_kernel(
             for (int e = 0; e < 24; ++e) sum += v[e];
             sum += __shfl_xor(sum, 1, 64);
             sum += __shfl_xor(sum, 2, 64);
-            const float mean = sum * (1.0f / 96.0f);
+            const float mean = rounded_f32(sum * (1.0f / 96.0f));
             float sq = 0.f;
 #pragma unroll
             for (int e = 0; e < 24; ++e) {
                 v[e] -= mean;
-                sq += v[e] * v[e];
+                sq += rounded_f32(v[e] * v[e]);
             }
             sq += __shfl_xor(sq, 1, 64);
             sq += __shfl_xor(sq, 2, 64);

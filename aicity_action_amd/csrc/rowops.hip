@@ -37,12 +37,12 @@ __global__ __launch_bounds__(256) void ln_fwd_kernel(const float* __restrict__ x
         float s = 0.f;
 #pragma unroll
         for (int i = 0; i < 3; ++i) s += (v[i].x + v[i].y) + (v[i].z + v[i].w);
-        const float mean = group_sum<LPR>(s) * (1.0f / C);
+        const float mean = rounded_f32(group_sum<LPR>(s) * (1.0f / C));
         float q = 0.f;
 #pragma unroll
         for (int i = 0; i < 3; ++i) {
             v[i].x -= mean; v[i].y -= mean; v[i].z -= mean; v[i].w -= mean;
-            q += (v[i].x * v[i].x + v[i].y * v[i].y) + (v[i].z * v[i].z + v[i].w * v[i].w);
+            q += (rounded_f32(v[i].x * v[i].x) + rounded_f32(v[i].y * v[i].y)) + (rounded_f32(v[i].z * v[i].z) + rounded_f32(v[i].w * v[i].w));
         }
         const float rstd = 1.0f / sqrtf(group_sum<LPR>(q) * (1.0f / C) + eps);
         if (ok) {
@@ -121,12 +121,12 @@ __global__ __launch_bounds__(256) void head_ln_partial_kernel(const float* __res
         float s = 0.f;
 #pragma unroll
         for (int i = 0; i < 3; ++i) s += (v[i].x + v[i].y) + (v[i].z + v[i].w);
-        const float mean = group_sum<LPR>(s) * (1.0f / C);
+        const float mean = rounded_f32(group_sum<LPR>(s) * (1.0f / C));
         float q = 0.f;
 #pragma unroll
         for (int i = 0; i < 3; ++i) {
             v[i].x -= mean; v[i].y -= mean; v[i].z -= mean; v[i].w -= mean;
-            q += (v[i].x * v[i].x + v[i].y * v[i].y) + (v[i].z * v[i].z + v[i].w * v[i].w);
+            q += (rounded_f32(v[i].x * v[i].x) + rounded_f32(v[i].y * v[i].y)) + (rounded_f32(v[i].z * v[i].z) + rounded_f32(v[i].w * v[i].w));
         }
         const float rstd = 1.0f / sqrtf(group_sum<LPR>(q) * (1.0f / C) + eps);
         if (ok) {
