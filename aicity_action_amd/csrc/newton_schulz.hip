@@ -16,12 +16,14 @@
 // both halves (high high + high low + low high, three times the matrix work): 1e-6, for results wanted in single precision.
 #include "common.h"
 #include <string.h>
+#include <algorithm>
 
 typedef _Float16 h16;
 typedef __attribute__((ext_vector_type(8))) _Float16 h16x8;
 typedef __attribute__((ext_vector_type(4))) _Float16 h16x4;
 typedef __attribute__((address_space(1))) const void ns_gptr_t;
 typedef __attribute__((address_space(3))) void ns_lptr_t;
+typedef __attribute__((address_space(3))) bf16x4 ns_lds_b4;
 
 #define NS_MAX 72            // matrices per set of launches (kernel arguments hold their table)
 #define NS_PARTS 256         // partial sums of squares per matrix
@@ -49,7 +51,6 @@ struct NsLoadArgs {
     float mu;
     int nesterov;
     float eps;
-    int lo_t;                // the last iteration comes next: it reads a tall matrix' low half in X^T's order
 };
 struct NsGemmArgs {
     uint32_t first[NS_MAX];
@@ -62,28 +63,26 @@ struct NsGemmArgs {
     uint32_t blocks;
     h16* ws;
     float a, b, c;
-    int cur;                 // which of the two X^T buffers holds the current one
-    int lo_t;                // as above, for the X that this launch writes
+    int cur;                 // which of the two buffers holds the current X
     const float* norm_coef;
     const float* hyper;      // {lr, ...} in device memory or NULL
     float lr, wd;
 };
 
 __device__ __forceinline__ int ns_pad(int v) { return (v + 63) & ~63; }
-// A matrix' region: X high | X low | X^T[0] | X^T[1] | X^T[0] low | A | B, and for SPLIT X^T[1] low | A low | B low
+// A matrix' region: X[0] high | X[1] high | X[0] low | A | B, and for SPLIT X[1] low | A low | B low.  X is an operand of the product that
+// renews it, so it alternates between two buffers; its low half, which only the tile's own workgroup reads, stays in place without SPLIT.
 struct NsRegion {
     h16* base;
     int64_t mn, mm;
     __device__ __forceinline__ NsRegion(h16* ws, uint32_t off, int m, int n)
         : base(ws + (int64_t)off * 64), mn((int64_t)ns_pad(m) * ns_pad(n)), mm((int64_t)ns_pad(m) * ns_pad(m)) {}
-    __device__ __forceinline__ h16* x() const { return base; }
-    __device__ __forceinline__ h16* xlo() const { return base + mn; }
-    __device__ __forceinline__ h16* xt(int i) const { return base + (i ? 3 : 2) * mn; }
-    __device__ __forceinline__ h16* a() const { return base + 5 * mn; }
-    __device__ __forceinline__ h16* b() const { return base + 5 * mn + mm; }
-    __device__ __forceinline__ h16* xtlo(int i) const { return i ? base + 5 * mn + 2 * mm : base + 4 * mn; }
-    __device__ __forceinline__ h16* alo() const { return base + 6 * mn + 2 * mm; }
-    __device__ __forceinline__ h16* blo() const { return base + 6 * mn + 3 * mm; }
+    __device__ __forceinline__ h16* x(int i) const { return base + i * mn; }
+    __device__ __forceinline__ h16* xlo(int i) const { return i ? base + 3 * mn + 2 * mm : base + 2 * mn; }
+    __device__ __forceinline__ h16* a() const { return base + 3 * mn; }
+    __device__ __forceinline__ h16* b() const { return base + 3 * mn + mm; }
+    __device__ __forceinline__ h16* alo() const { return base + 4 * mn + 2 * mm; }
+    __device__ __forceinline__ h16* blo() const { return base + 4 * mn + 3 * mm; }
 };
 // Pins a value to fp32 before it is cut into a high and a low half.  Left to itself the compiler folds the product behind it and the
 // conversion of one use into v_fma_mixlo_f16, which rounds once where the conversion of the other use rounds twice: about one value in
@@ -171,16 +170,16 @@ __global__ __launch_bounds__(256) void ns_square_kernel(const NsLoadArgs a) {
     if (threadIdx.x == 0) a.parts[(int64_t)id * NS_PARTS + part] = (red[0] + red[1]) + (red[2] + red[3]);
 }
 
-// ---- 2. X_0 in both orders ----------------------------------------------------------------------------------------------------------
-// One 64 x 64 tile of X per workgroup, through LDS, padding written as zeros.  The update is formed again from the gradient and the new
-// momentum: the same bytes as writing it down and reading it back.
-template <typename T, bool SPLIT>
+// ---- 2. X_0 --------------------------------------------------------------------------------------------------------------------------
+// One 64 x 64 tile of X per workgroup, through LDS (a tall update is transposed there), padding written as zeros.  The update is formed
+// again from the gradient and the new momentum: the same bytes as writing it down and reading it back.
+template <typename T>
 __global__ __launch_bounds__(256) void ns_start_kernel(const NsLoadArgs a) {
     const int id = ns_find([&](int i) { return a.mat[i].first; }, a.n, blockIdx.x);
     const NsMat& t = a.mat[id];
     const bool tall = t.rows > t.cols;
     const int m = tall ? t.cols : t.rows, n = tall ? t.rows : t.cols;
-    const int mp = ns_pad(m), np = ns_pad(n);
+    const int np = ns_pad(n);
     const uint32_t tile = blockIdx.x - t.first;
     const int per_row = np / 64;
     const int ti = tile / per_row, tj = tile - ti * per_row;       // tile row (of m), tile column (of n)
@@ -217,103 +216,104 @@ __global__ __launch_bounds__(256) void ns_start_kernel(const NsLoadArgs a) {
     __syncthreads();
     const float f = s_inv * NS_S;
     const NsRegion g(a.ws, t.off, m, n);
-    // eight consecutive values per thread: X rows (64 of n each), then X^T rows (64 of m each)
+    // eight consecutive values of a row of X per thread
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
         const int e = k * 256 + tid, row = e >> 3, ch = (e & 7) * 8;
-        h16x8 hi, lo, hit, lot;
+        h16x8 hi, lo;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            float vx = (tall ? sh[ch + j][row] : sh[row][ch + j]) * f;          // X[ti*64 + row][tj*64 + ch + j]
-            float vt = (tall ? sh[row][ch + j] : sh[ch + j][row]) * f;          // X^T[tj*64 + row][ti*64 + ch + j]
-            ns_pin(vx);
-            ns_pin(vt);
-            hi[j] = (h16)vx; lo[j] = (h16)(vx - (float)hi[j]);
-            hit[j] = (h16)vt; lot[j] = (h16)(vt - (float)hit[j]);
+            float v = (tall ? sh[ch + j][row] : sh[row][ch + j]) * f;           // X[ti*64 + row][tj*64 + ch + j]
+            ns_pin(v);
+            hi[j] = (h16)v;
+            lo[j] = (h16)(v - (float)hi[j]);
         }
-        const int64_t ix = (int64_t)(ti * 64 + row) * np + tj * 64 + ch, it = (int64_t)(tj * 64 + row) * mp + ti * 64 + ch;
-        *reinterpret_cast<h16x8*>(g.x() + ix) = hi;
-        *reinterpret_cast<h16x8*>(g.xt(0) + it) = hit;
-        if (SPLIT) {
-            *reinterpret_cast<h16x8*>(g.xlo() + ix) = lo;
-            *reinterpret_cast<h16x8*>(g.xtlo(0) + it) = lot;
-        } else if (a.lo_t && tall) *reinterpret_cast<h16x8*>(g.xtlo(0) + it) = lot;
-        else *reinterpret_cast<h16x8*>(g.xlo() + ix) = lo;
+        const int64_t ix = (int64_t)(ti * 64 + row) * np + tj * 64 + ch;
+        *reinterpret_cast<h16x8*>(g.x(0) + ix) = hi;
+        *reinterpret_cast<h16x8*>(g.xlo(0) + ix) = lo;
     }
 }
 
 // ---- 3. the products -----------------------------------------------------------------------------------------------------------------
-// D[M][N] = sum_k P[M][k] Q[N][k] with both operands contiguous in k: A = X X^T (P = Q = X), A A (P = Q = A, symmetric), B X (P = X^T,
-// Q = B) and, in the last iteration of a tall matrix, P = B, Q = X^T.  X is kept in both orders for this; A and B are symmetric: only
-// tiles on and above the diagonal are computed, each written twice.
-// One workgroup = one T x T tile, four waves in 2 x 2, K steps of 64 from two LDS stages: a step's fragments are read into registers, the
-// next step's tile is requested (LDS-DMA), then the matrix instructions run while it flies.  LDS rows are 128 bytes; 16-byte chunk c of row
-// r lies at c ^ ((r >> 1) & 7), so the 16 rows that a read serves together fall on 16 different slots of the 256-byte bank period.
-// The tile leaves through LDS in whole rows, in the order [N][M] ("direct": an accumulator register quad is four values of one such row)
-// and, where both orders are kept, [M][N].
+// D[M][N] = sum_k P(k, M) Q[N][k]:  A = X X^T (P = Q = X) and A A (P = Q = A) with both operands contiguous in k, only tiles on and above
+// the diagonal computed and each written twice;  X^T B^T = (B X)^T with P = X as it lies, k down its rows, read through the transposing LDS
+// read, so that X is kept in one order.
+// One workgroup = one T x T tile.  A group of four waves (2 x 2) takes K steps of 64 from two LDS stages of its own: a step's fragments
+// are read into registers, the next step's tile is requested (LDS-DMA), then the matrix instructions run while it flies.  With G groups the
+// steps are dealt in turn and the groups' sums added in order at the end: for launches of few tiles, whose time is the latency of a step
+// times their number.
+// LDS: k-contiguous tiles have rows of 128 bytes, 16-byte chunk c of row r at c ^ ((r >> 1) & 7): the 16 rows that a read serves together
+// fall on 16 different slots of the 256-byte bank period.  X tiles as they lie have rows of 2 T bytes (a k each), 64-byte unit u of row r at
+// u ^ (r & 3) (T = 128) or u ^ ((r >> 1) & 1) (T = 64): the four rows of a transposing read fall on different banks.
+// The tile leaves through LDS in whole rows.  An accumulator register quad is four values along M, so [N][M] is the straight order:
+// X itself, A, B, and the result of a wide matrix; the mirrored tiles of A and B and the result of a tall matrix are turned on the way.
 enum { NS_GRAM = 0, NS_POLY = 1, NS_STEP = 2, NS_LAST16 = 3, NS_LAST32 = 4, NS_MUON = 5 };
 
-template <int T, int PHASE, bool SPLIT>
-__global__ __launch_bounds__(256, 2) void ns_gemm_kernel(const NsGemmArgs a) {
+template <int T, int G, int PHASE>
+constexpr int ns_lds_bytes() {
+    const int stages = G * 2 * 2 * T * 128, sums = (G - 1) * 4096 * (T / 64) * (T / 64) * 4;
+    const int out = PHASE >= NS_LAST16 ? T * (T * 4 + 16) : 2 * T * (T * 2 + 16);
+    return stages > out ? (stages > sums ? stages : sums) : (out > sums ? out : sums);
+}
+
+template <int T, int G, int PHASE, bool SPLIT>
+__global__ __launch_bounds__(256 * G, G == 1 ? 2 : 4) void ns_gemm_kernel(const NsGemmArgs a) {
     constexpr int F = T / 64;                      // 32 x 32 accumulators per wave and direction
     constexpr int STAGE = 2 * T * 128;             // bytes of P tile + Q tile
-    constexpr int OROW = T * 2 + 16;               // bytes of an output row in LDS
     constexpr bool SYM = PHASE == NS_GRAM || PHASE == NS_POLY;
     constexpr bool LAST = PHASE >= NS_LAST16;
     extern __shared__ __attribute__((aligned(16))) char smem[];
     const uint32_t blk = blockIdx.x;
     const int id = ns_find([&](int i) { return a.first[i]; }, a.count, blk);
     const int m = a.m[id], n = a.n[id], mp = ns_pad(m), np = ns_pad(n);
-    const bool tall = a.tall[id];
     const NsRegion g(a.ws, a.off[id], m, n);
     const uint32_t tile = blk - a.first[id];
 
-    // operands and tile
-    const h16 *p, *q, *plo = nullptr, *qlo = nullptr;
-    int ldk, rows_p, rows_q, tm, tn;
+    int tm, tn;
     if (SYM) {
         int J = (int)((sqrtf(8.0f * (float)tile + 1.0f) - 1.0f) * 0.5f);
         while ((uint32_t)(J + 1) * (J + 2) / 2 <= tile) ++J;
         while ((uint32_t)J * (J + 1) / 2 > tile) --J;
         tn = J;
         tm = (int)(tile - (uint32_t)J * (J + 1) / 2);
-        rows_p = rows_q = mp;
-        if (PHASE == NS_GRAM) { p = q = g.x(); plo = qlo = g.xlo(); ldk = np; }
-        else { p = q = g.a(); plo = qlo = g.alo(); ldk = mp; }
     } else {
-        ldk = mp;
-        const bool swap = LAST && tall;
-        p = swap ? g.b() : g.xt(a.cur);
-        q = swap ? g.xt(a.cur) : g.b();
-        if (SPLIT) { plo = swap ? g.blo() : g.xtlo(a.cur); qlo = swap ? g.xtlo(a.cur) : g.blo(); }
-        rows_p = swap ? mp : np;
-        rows_q = swap ? np : mp;
-        const int tiles_m = (rows_p + T - 1) / T;
-        tn = tile / tiles_m;
-        tm = tile - tn * tiles_m;
+        const int tiles_n = (mp + T - 1) / T;      // neighbouring workgroups share the tile of X
+        tm = tile / tiles_n;
+        tn = tile - tm * tiles_n;
     }
     const int m0 = tm * T, n0 = tn * T;
-    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
-    const int r = lane & 31, h = lane >> 5;
+    const int lim_m = SYM ? mp : np, lim_n = mp;   // extents of the output
+    const int tid = threadIdx.x, grp = __builtin_amdgcn_readfirstlane(tid >> 8), wave = __builtin_amdgcn_readfirstlane((tid >> 6) & 3);
+    const int lane = tid & 63, r = lane & 31, h = lane >> 5;
     const int wm = (wave & 1) * (T / 2), wn = (wave >> 1) * (T / 2);
+    char* const lds = smem + grp * 2 * STAGE;
 
-    // LDS-DMA: a wave instruction brings 8 rows of 128 bytes; wave w moves T/16 of the T/4 pieces (the first half is P)
+    // LDS-DMA: a wave instruction brings 1 KiB; waves 0 and 1 move P, waves 2 and 3 Q, T/16 pieces each.  Rows or columns past the padded
+    // matrix are read again from its last ones; what comes of them is never stored
     constexpr int PW = T / 16;
     const bool is_q = wave >= 2;
-    int src_off[PW];                               // element offset of this lane's 16 bytes from the operand's tile column
+    const bool by_k = !SYM && !is_q;               // the tile of X as it lies
+    const int ldk = PHASE == NS_GRAM || !SYM ? np : mp;      // row length of P
+    const int ld_src = is_q && !SYM ? mp : ldk;
+    int src_off[PW];                               // element offset of this lane's 16 bytes from the operand's tile
 #pragma unroll
     for (int i = 0; i < PW; ++i) {
-        const int row = ((wave & 1) * PW + i) * 8 + (lane >> 3);
-        const int slot = lane & 7, ch = slot ^ ((row >> 1) & 7);
-        const int lim = is_q ? rows_q : rows_p;
-        int grow = (is_q ? n0 : m0) + row;
-        grow = grow < lim ? grow : lim - 1;        // rows past the padded matrix: read again, never stored
-        src_off[i] = grow * ldk + ch * 8;
+        const int piece = (wave & 1) * PW + i;
+        if (by_k) {
+            const int row = piece * (512 / T) + lane / (T / 8), slot = lane % (T / 8);
+            const int ch = T == 128 ? slot ^ ((row & 3) << 2) : slot ^ (((row >> 1) & 1) << 2);
+            const int col = min(m0 + ch * 8, np - 8);
+            src_off[i] = row * ld_src + col;
+        } else {
+            const int row = piece * 8 + (lane >> 3), ch = (lane & 7) ^ ((row >> 1) & 7);
+            src_off[i] = min((is_q ? n0 : m0) + row, mp - 1) * ld_src + ch * 8;
+        }
     }
-    const int nk = ldk / NS_BK;
+    const int64_t k_step = by_k ? (int64_t)NS_BK * ld_src : NS_BK;
+    const int nk = (PHASE == NS_GRAM ? np : mp) / NS_BK;
     const int steps = SPLIT ? 3 * nk : nk;
-    const h16* const src_hi = is_q ? q : p;
-    const h16* const src_lo = is_q ? qlo : plo;
+    const h16* const src_hi = PHASE == NS_GRAM ? g.x(a.cur) : PHASE == NS_POLY ? g.a() : is_q ? g.b() : g.x(a.cur);
+    const h16* const src_lo = PHASE == NS_GRAM ? g.xlo(a.cur) : PHASE == NS_POLY ? g.alo() : is_q ? g.blo() : g.xlo(a.cur);
     auto dma = [=](int kt, int stage) {
         const h16* base = src_hi;
         if (SPLIT) {        // high high, then high low, then low high
@@ -321,36 +321,71 @@ __global__ __launch_bounds__(256, 2) void ns_gemm_kernel(const NsGemmArgs a) {
             kt -= seg * nk;
             if (seg == (is_q ? 1 : 2)) base = src_lo;
         }
-        base += kt * NS_BK;
-        char* dst = smem + stage * STAGE + (is_q ? T * 128 : 0) + (wave & 1) * PW * 1024;
+        base += kt * k_step;
+        char* dst = lds + stage * STAGE + (is_q ? T * 128 : 0) + (wave & 1) * PW * 1024;
 #pragma unroll
         for (int i = 0; i < PW; ++i)
             __builtin_amdgcn_global_load_lds((ns_gptr_t*)(base + src_off[i]), (ns_lptr_t*)(dst + 1024 * i), 16, 0, 0);
     };
 
+    if (grp < steps) dma(grp, 0);
+
+    // X <- a X + B X: the sum begins at a X (without SPLIT: with it the many roundings at the size of a X would be what it is there to avoid)
+    const h16* const res = PHASE == NS_POLY ? g.a() : g.x(a.cur);
+    const h16* const reslo = PHASE == NS_POLY ? g.alo() : g.xlo(SPLIT ? a.cur : 0);
+    constexpr bool START = !SYM && !SPLIT;
+    auto residual = [&](int i, int j, int e4) {
+        const int M = m0 + wm + 32 * i + 8 * e4 + 4 * h, N = n0 + wn + 32 * j + r;
+        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (M < lim_m && N < lim_n) {
+            const int64_t at = (int64_t)N * lim_m + M;
+            const h16x4 hi = *reinterpret_cast<const h16x4*>(res + at);
+            x = make_float4((float)hi[0], (float)hi[1], (float)hi[2], (float)hi[3]);
+            if (PHASE != NS_POLY || SPLIT) {
+                const h16x4 lo = *reinterpret_cast<const h16x4*>(reslo + at);
+                x.x += (float)lo[0]; x.y += (float)lo[1]; x.z += (float)lo[2]; x.w += (float)lo[3];
+            }
+        }
+        return x;
+    };
     f32x16 acc[F][F];
 #pragma unroll
     for (int i = 0; i < F; ++i)
 #pragma unroll
         for (int j = 0; j < F; ++j)
 #pragma unroll
-            for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
+            for (int e4 = 0; e4 < 4; ++e4) {
+                float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (START && grp == 0) x = residual(i, j, e4);
+                const float f = a.a * NS_S;
+                acc[i][j][4 * e4] = f * x.x; acc[i][j][4 * e4 + 1] = f * x.y; acc[i][j][4 * e4 + 2] = f * x.z; acc[i][j][4 * e4 + 3] = f * x.w;
+            }
 
-    dma(0, 0);
-    for (int kt = 0; kt < steps; ++kt) {
+    const int q4 = (lane & 15) >> 2;               // transposing read: this lane names four columns of row 8 h + q4 (+ 4)
+    const int tr_row = 8 * h + q4, tr_col = (16 * ((lane >> 4) & 1) + 4 * (lane & 3)) * 2;
+    for (int kt = grp, it = 0; it * G < steps; kt += G, ++it) {
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __syncthreads();                            // the step's tile has landed; everyone has read the stage refilled below
-        const char* sp = smem + (kt & 1) * STAGE;
+        if (G > 1 && kt >= steps) continue;
+        const char* sp = lds + (it & 1) * STAGE;
+        const char* sq = sp + T * 128;
         h16x8 fp[F][4], fq[F][4];
 #pragma unroll
         for (int ks = 0; ks < 4; ++ks)
 #pragma unroll
             for (int i = 0; i < F; ++i) {
                 const int rp = wm + 32 * i + r, rq = wn + 32 * i + r;
-                fp[i][ks] = *reinterpret_cast<const h16x8*>(sp + rp * 128 + (((2 * ks + h) ^ ((rp >> 1) & 7)) * 16));
-                fq[i][ks] = *reinterpret_cast<const h16x8*>(sp + T * 128 + rq * 128 + (((2 * ks + h) ^ ((rq >> 1) & 7)) * 16));
+                if (SYM) fp[i][ks] = *reinterpret_cast<const h16x8*>(sp + rp * 128 + (((2 * ks + h) ^ ((rp >> 1) & 7)) * 16));
+                else {
+                    const int unit = (wm >> 5) + i, uu = T == 128 ? unit ^ q4 : unit ^ (q4 >> 1);
+                    const char* at = sp + (16 * ks + tr_row) * (2 * T) + uu * 64 + tr_col;
+                    const h16x4 lo = __builtin_bit_cast(h16x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((ns_lds_b4*)at));
+                    const h16x4 hi = __builtin_bit_cast(h16x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((ns_lds_b4*)(at + 4 * 2 * T)));
+                    fp[i][ks] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+                }
+                fq[i][ks] = *reinterpret_cast<const h16x8*>(sq + rq * 128 + (((2 * ks + h) ^ ((rq >> 1) & 7)) * 16));
             }
-        if (kt + 1 < steps) dma(kt + 1, (kt + 1) & 1);
+        if (kt + G < steps) dma(kt + G, (it + 1) & 1);
 #pragma unroll
         for (int ks = 0; ks < 4; ++ks)
 #pragma unroll
@@ -360,114 +395,151 @@ __global__ __launch_bounds__(256, 2) void ns_gemm_kernel(const NsGemmArgs a) {
                     acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fp[i][ks], fq[j][ks], acc[i][j], 0, 0, 0);
     }
 
-    // ---- epilogue: the new values in the accumulators -------------------------------------------------------------------------------
-    const int lim_m = SYM ? mp : rows_p, lim_n = SYM ? mp : rows_q;      // extent of the output, both directions
-    const h16* res = PHASE == NS_POLY ? g.a() : (LAST && tall) ? g.xt(a.cur) : g.x();
-    const h16* reslo = PHASE == NS_POLY ? g.alo() : (LAST && tall) ? g.xtlo(SPLIT ? a.cur : 0) : g.xlo();
-    const int64_t ldr = SYM ? mp : rows_p;                                // a row of the output [N][M]
-    const float f_acc = PHASE == NS_POLY ? a.c / NS_S : LAST ? 1.0f / (NS_S * NS_S) : 1.0f / NS_S;
-    const float f_res = PHASE == NS_POLY ? a.b : LAST ? a.a / NS_S : a.a;
+    if (G > 1) {        // the groups' sums, in order
+        __syncthreads();
+        float* sums = reinterpret_cast<float*>(smem);
+        if (grp > 0)
 #pragma unroll
-    for (int i = 0; i < F; ++i)
+            for (int i = 0; i < F; ++i)
 #pragma unroll
-        for (int j = 0; j < F; ++j)
+                for (int j = 0; j < F; ++j)
 #pragma unroll
-            for (int e4 = 0; e4 < 4; ++e4) {
-                const int M = m0 + wm + 32 * i + 8 * e4 + 4 * h, N = n0 + wn + 32 * j + r;
-                float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-                if (PHASE != NS_GRAM && M < lim_m && N < lim_n) {
-                    const h16x4 hi = *reinterpret_cast<const h16x4*>(res + N * ldr + M);
-                    x = make_float4((float)hi[0], (float)hi[1], (float)hi[2], (float)hi[3]);
-                    if (PHASE != NS_POLY || SPLIT) {
-                        const h16x4 lo = *reinterpret_cast<const h16x4*>(reslo + N * ldr + M);
-                        x.x += (float)lo[0]; x.y += (float)lo[1]; x.z += (float)lo[2]; x.w += (float)lo[3];
-                    }
-                }
-                float* v = reinterpret_cast<float*>(&acc[i][j]) + 4 * e4;
-                v[0] = f_res * x.x + f_acc * v[0]; v[1] = f_res * x.y + f_acc * v[1];
-                v[2] = f_res * x.z + f_acc * v[2]; v[3] = f_res * x.w + f_acc * v[3];
-            }
+                    for (int e = 0; e < 16; ++e) sums[(((grp - 1) * 4 + wave) * F * F + i * F + j) * 1024 + e * 64 + lane] = acc[i][j][e];
+        __syncthreads();
+        if (grp == 0)
+#pragma unroll
+            for (int o = 0; o < G - 1; ++o)
+#pragma unroll
+                for (int i = 0; i < F; ++i)
+#pragma unroll
+                    for (int j = 0; j < F; ++j)
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) acc[i][j][e] += sums[((o * 4 + wave) * F * F + i * F + j) * 1024 + e * 64 + lane];
+    }
 
-    if (LAST) {       // rows of the result: N = the result's row, M its column
-        const int R = tall ? n : m, C = tall ? m : n;
-        const bool bad = PHASE == NS_MUON && ns_bad(a.norm_coef);
-        const float lr = a.hyper ? a.hyper[0] : a.lr;
-        const float keep = 1.0f - lr * a.wd, step = lr * a.scale[id];
-        if (bad) return;
+    // ---- the new values, times 2^12 but for the last iteration's ---------------------------------------------------------------------------
+    const float f_acc = PHASE == NS_POLY ? a.c / NS_S : LAST ? 1.0f / (NS_S * NS_S) : 1.0f / NS_S;
+    const float f_res = PHASE == NS_GRAM || START ? 0.f : PHASE == NS_POLY ? a.b : LAST ? a.a / NS_S : a.a;
+    if (grp == 0)
 #pragma unroll
         for (int i = 0; i < F; ++i)
 #pragma unroll
-            for (int j = 0; j < F; ++j)
+            for (int j = 0; j < F; ++j) {
 #pragma unroll
                 for (int e4 = 0; e4 < 4; ++e4) {
-                    const int M = m0 + wm + 32 * i + 8 * e4 + 4 * h, N = n0 + wn + 32 * j + r;
-                    if (N >= R) continue;
+                    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+                    if (PHASE != NS_GRAM && !START) x = residual(i, j, e4);
+                    const float xs[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        if (M + e >= C) continue;
-                        const int64_t at = (int64_t)N * C + M + e;
-                        const float v = acc[i][j][4 * e4 + e];
-                        if (PHASE == NS_LAST16) static_cast<bf16_t*>(a.out[id])[at] = f32_to_bf16(v);
-                        else if (PHASE == NS_LAST32) static_cast<float*>(a.out[id])[at] = v;
-                        else {
-                            float* w = static_cast<float*>(a.out[id]) + at;
-                            *w = *w * keep - step * v;
-                        }
-                    }
+                    for (int e = 0; e < 4; ++e) acc[i][j][4 * e4 + e] = f_res * xs[e] + f_acc * acc[i][j][4 * e4 + e];
                 }
+                ns_pin(acc[i][j]);
+            }
+
+    if (LAST) {       // the result's rows through LDS in single precision
+        constexpr int ROWB = T * 4 + 16;
+        const bool tall = a.tall[id];
+        const int R = tall ? n : m, C = tall ? m : n, row0 = tall ? m0 : n0, col0 = tall ? n0 : m0;
+        if (PHASE == NS_MUON && ns_bad(a.norm_coef)) return;
+        __syncthreads();
+        if (grp == 0)
+#pragma unroll
+            for (int i = 0; i < F; ++i)
+#pragma unroll
+                for (int j = 0; j < F; ++j)
+#pragma unroll
+                    for (int e4 = 0; e4 < 4; ++e4) {
+                        const int M = wm + 32 * i + 8 * e4 + 4 * h, N = wn + 32 * j + r;
+                        if (tall)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) *reinterpret_cast<float*>(smem + (M + e) * ROWB + N * 4) = acc[i][j][4 * e4 + e];
+                        else
+                            *reinterpret_cast<float4*>(smem + N * ROWB + M * 4) =
+                                make_float4(acc[i][j][4 * e4], acc[i][j][4 * e4 + 1], acc[i][j][4 * e4 + 2], acc[i][j][4 * e4 + 3]);
+                    }
+        __syncthreads();
+        const float lr = a.hyper ? a.hyper[0] : a.lr;
+        const float keep = 1.0f - lr * a.wd, step = lr * a.scale[id];
+        const bool quads = (C & 3) == 0 && (reinterpret_cast<uintptr_t>(a.out[id]) & (PHASE == NS_LAST16 ? 7 : 15)) == 0;
+        if (quads) {
+#pragma unroll 4
+            for (int k = tid; k < T * T / 4; k += 256 * G) {
+                const int row = k / (T / 4), c4 = (k - row * (T / 4)) * 4;
+                if (row0 + row >= R || col0 + c4 >= C) continue;
+                const float4 v = *reinterpret_cast<const float4*>(smem + row * ROWB + c4 * 4);
+                const int64_t at = (int64_t)(row0 + row) * C + col0 + c4;
+                if (PHASE == NS_LAST16) store4(static_cast<bf16_t*>(a.out[id]) + at, v);
+                else if (PHASE == NS_LAST32) store4(static_cast<float*>(a.out[id]) + at, v);
+                else {
+                    float4* w = reinterpret_cast<float4*>(static_cast<float*>(a.out[id]) + at);
+                    float4 x = *w;
+                    x.x = x.x * keep - step * v.x; x.y = x.y * keep - step * v.y;
+                    x.z = x.z * keep - step * v.z; x.w = x.w * keep - step * v.w;
+                    *w = x;
+                }
+            }
+        } else {
+#pragma unroll 4
+            for (int k = tid; k < T * T; k += 256 * G) {
+                const int row = k / T, c = k - row * T;
+                if (row0 + row >= R || col0 + c >= C) continue;
+                const float v = *reinterpret_cast<const float*>(smem + row * ROWB + c * 4);
+                const int64_t at = (int64_t)(row0 + row) * C + col0 + c;
+                if (PHASE == NS_LAST16) static_cast<bf16_t*>(a.out[id])[at] = f32_to_bf16(v);
+                else if (PHASE == NS_LAST32) static_cast<float*>(a.out[id])[at] = v;
+                else {
+                    float* w = static_cast<float*>(a.out[id]) + at;
+                    *w = *w * keep - step * v;
+                }
+            }
+        }
         return;
     }
 
-    // ---- the tile through LDS: [N][M] and [M][N], high halves, then low halves ------------------------------------------------------------
+    // ---- the tile through LDS: X's high and low half in one pass; A and B and their mirror image, high halves, then (SPLIT) low halves ---------
+    constexpr int ROWB = T * 2 + 16;
+    const bool mirror = SYM && tm != tn;
+    char* const o1 = smem;
+    char* const o2 = smem + T * ROWB;
 #pragma unroll
-    for (int i = 0; i < F; ++i)
-#pragma unroll
-        for (int j = 0; j < F; ++j) ns_pin(acc[i][j]);
-    h16* dst_d = PHASE == NS_GRAM ? g.a() : PHASE == NS_POLY ? g.b() : g.x();                 // [N][M]
-    h16* dst_t = PHASE == NS_GRAM ? g.a() : PHASE == NS_POLY ? g.b() : g.xt(a.cur ^ 1);     // [M][N]
-    const bool write_t = !SYM || tm != tn;
-    const int ld_t = SYM ? mp : rows_q;
-    const bool lo_in_t = PHASE == NS_STEP && !SPLIT && a.lo_t && tall;
-    char* od = smem;
-    char* ot = smem + T * OROW;
-#pragma unroll
-    for (int pass = 0; pass < 2; ++pass) {
-        if (pass == 1) {
-            if (SYM && !SPLIT) break;
-            dst_d = PHASE == NS_GRAM ? g.alo() : PHASE == NS_POLY ? g.blo() : g.xlo();
-            dst_t = PHASE == NS_GRAM ? g.alo() : PHASE == NS_POLY ? g.blo() : g.xtlo(SPLIT ? a.cur ^ 1 : 0);
-        }
-        const bool do_d = pass == 0 || !lo_in_t;
-        const bool do_t = write_t && (pass == 0 || SPLIT || lo_in_t);
+    for (int pass = 0; pass < (SYM && SPLIT ? 2 : 1); ++pass) {
+        h16* const d1 = PHASE == NS_STEP ? g.x(a.cur ^ 1) : PHASE == NS_GRAM ? (pass ? g.alo() : g.a()) : (pass ? g.blo() : g.b());
+        h16* const d2 = PHASE == NS_STEP ? g.xlo(SPLIT ? a.cur ^ 1 : 0) : d1;
         __syncthreads();
+        if (grp == 0)
 #pragma unroll
-        for (int i = 0; i < F; ++i)
+            for (int i = 0; i < F; ++i)
 #pragma unroll
-            for (int j = 0; j < F; ++j)
+                for (int j = 0; j < F; ++j)
 #pragma unroll
-                for (int e4 = 0; e4 < 4; ++e4) {
-                    const int M = wm + 32 * i + 8 * e4 + 4 * h, N = wn + 32 * j + r;
-                    h16x4 v;
+                    for (int e4 = 0; e4 < 4; ++e4) {
+                        const int M = wm + 32 * i + 8 * e4 + 4 * h, N = wn + 32 * j + r;
+                        h16x4 hi, lo;
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const float x = acc[i][j][4 * e4 + e];
-                        const h16 hi = (h16)x;
-                        v[e] = pass == 0 ? hi : (h16)(x - (float)hi);
+                        for (int e = 0; e < 4; ++e) {
+                            const float x = acc[i][j][4 * e4 + e];
+                            hi[e] = (h16)x;
+                            lo[e] = (h16)(x - (float)hi[e]);
+                        }
+                        const h16x4 v = pass ? lo : hi;
+                        *reinterpret_cast<h16x4*>(o1 + N * ROWB + M * 2) = v;
+                        if (PHASE == NS_STEP) *reinterpret_cast<h16x4*>(o2 + N * ROWB + M * 2) = lo;
+                        else if (mirror)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) *reinterpret_cast<h16*>(o2 + (M + e) * ROWB + N * 2) = v[e];
                     }
-                    if (do_d) *reinterpret_cast<h16x4*>(od + N * OROW + M * 2) = v;
-                    if (do_t)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) *reinterpret_cast<h16*>(ot + (M + e) * OROW + N * 2) = v[e];
-                }
         __syncthreads();
         constexpr int CH = T / 8;                 // 16-byte chunks of a row
 #pragma unroll 4
-        for (int k = tid; k < T * CH; k += 256) {
+        for (int k = tid; k < T * CH; k += 256 * G) {
             const int row = k / CH, c8 = (k - row * CH) * 8;
-            if (do_d && n0 + row < lim_n && m0 + c8 < lim_m)
-                *reinterpret_cast<h16x8*>(dst_d + (int64_t)(n0 + row) * ldr + m0 + c8) = *reinterpret_cast<const h16x8*>(od + row * OROW + c8 * 2);
-            if (do_t && m0 + row < lim_m && n0 + c8 < lim_n)
-                *reinterpret_cast<h16x8*>(dst_t + (int64_t)(m0 + row) * ld_t + n0 + c8) = *reinterpret_cast<const h16x8*>(ot + row * OROW + c8 * 2);
+            const bool straight = n0 + row < lim_n && m0 + c8 < lim_m;
+            const int64_t at = (int64_t)(n0 + row) * lim_m + m0 + c8;
+            if (straight) *reinterpret_cast<h16x8*>(d1 + at) = *reinterpret_cast<const h16x8*>(o1 + row * ROWB + c8 * 2);
+            if (PHASE == NS_STEP) {
+                if (straight) *reinterpret_cast<h16x8*>(d2 + at) = *reinterpret_cast<const h16x8*>(o2 + row * ROWB + c8 * 2);
+            } else if (mirror && m0 + row < lim_m && n0 + c8 < lim_n)
+                *reinterpret_cast<h16x8*>(d2 + (int64_t)(m0 + row) * lim_m + n0 + c8) = *reinterpret_cast<const h16x8*>(o2 + row * ROWB + c8 * 2);
         }
     }
 }
@@ -477,7 +549,7 @@ static inline int64_t pad64(int64_t v) { return (v + 63) & ~(int64_t)63; }
 
 static int64_t ns_region_units(int rows, int cols, int split) {       // units of 64 fp16
     const int64_t mp = pad64(rows < cols ? rows : cols), np = pad64(rows < cols ? cols : rows);
-    return (split ? 6 * mp * np + 4 * mp * mp : 5 * mp * np + 2 * mp * mp) / 64;
+    return (split ? 4 * mp * np + 4 * mp * mp : 3 * mp * np + 2 * mp * mp) / 64;
 }
 
 static int ns_check(const mvit_ns_matrix* mats, int count) {
@@ -507,40 +579,60 @@ extern "C" int64_t mvit_newton_schulz_workspace_bytes(const mvit_ns_matrix* mats
     return most * 128 + (int64_t)NS_MAX * NS_PARTS * 8;
 }
 
-template <int T, int PHASE, bool SPLIT>
-static int ns_launch(NsGemmArgs& g, hipStream_t st) {
-    constexpr int LDS = 2 * 2 * T * 128 > 2 * T * (T * 2 + 16) ? 2 * 2 * T * 128 : 2 * T * (T * 2 + 16);
+// tiles of a launch at a tile side
+static int64_t ns_tiles(const NsGemmArgs& g, int side, bool sym, uint32_t* first) {
+    int64_t at = 0;
+    for (int i = 0; i < g.count; ++i) {
+        const int64_t mt = (pad64(g.m[i]) + side - 1) / side, nt = (pad64(g.n[i]) + side - 1) / side;
+        if (first) first[i] = (uint32_t)at;
+        at += sym ? mt * (mt + 1) / 2 : mt * nt;
+    }
+    return at;
+}
+
+template <int T, int G, int PHASE, bool SPLIT>
+static int ns_launch_as(NsGemmArgs& g, hipStream_t st) {
+    constexpr int LDS = ns_lds_bytes<T, G, PHASE>();
     static DevFlags done;
-    auto* kern = &ns_gemm_kernel<T, PHASE, SPLIT>;
     DevFlag flag = dev_flag(done);
     if (LDS > 65536 && !flag) {
-        if (hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, LDS) != hipSuccess)
+        if (hipFuncSetAttribute(reinterpret_cast<const void*>(&ns_gemm_kernel<T, G, PHASE, SPLIT>), hipFuncAttributeMaxDynamicSharedMemorySize,
+                                LDS) != hipSuccess)
             return MVIT_ELAUNCH;
         flag = true;
     }
-    uint64_t at = 0;
-    for (int i = 0; i < g.count; ++i) {
-        const int64_t mt = (pad64(g.m[i]) + T - 1) / T, nt = (pad64(g.n[i]) + T - 1) / T;
-        g.first[i] = (uint32_t)at;
-        at += PHASE == NS_GRAM || PHASE == NS_POLY ? mt * (mt + 1) / 2 : mt * nt;
-    }
-    if (at > 0x7fffffffu) return MVIT_EUNSUPPORTED;
-    g.blocks = (uint32_t)at;
-    hipLaunchKernelGGL((ns_gemm_kernel<T, PHASE, SPLIT>), dim3(g.blocks), dim3(256), LDS, st, g);
+    const int64_t tiles = ns_tiles(g, T, PHASE == NS_GRAM || PHASE == NS_POLY, g.first);
+    if (tiles > 0x7fffffff) return MVIT_EUNSUPPORTED;
+    g.blocks = (uint32_t)tiles;
+    hipLaunchKernelGGL((ns_gemm_kernel<T, G, PHASE, SPLIT>), dim3(g.blocks), dim3(256 * G), LDS, st, g);
     return hipGetLastError() == hipSuccess ? MVIT_OK : MVIT_ELAUNCH;
 }
 
-template <int T, bool SPLIT>
+// Tiles of 128 once there are two for each of the 256 CUs, else tiles of 64; four groups of waves per tile where even those leave CUs idle
+// and the longest sum has steps for them.
+template <int PHASE, bool SPLIT>
+static int ns_launch(NsGemmArgs& g, hipStream_t st) {
+    constexpr bool SYM = PHASE == NS_GRAM || PHASE == NS_POLY;
+    if (ns_tiles(g, 128, SYM, nullptr) >= 512) return ns_launch_as<128, 1, PHASE, SPLIT>(g, st);
+    int steps = 0;
+    for (int i = 0; i < g.count; ++i) {
+        const int k = (int)(pad64(PHASE == NS_GRAM ? g.n[i] : g.m[i]) / NS_BK) * (SPLIT ? 3 : 1);
+        steps = k > steps ? k : steps;
+    }
+    if (steps >= 8 && ns_tiles(g, 64, SYM, nullptr) <= 256) return ns_launch_as<64, 4, PHASE, SPLIT>(g, st);
+    return ns_launch_as<64, 1, PHASE, SPLIT>(g, st);
+}
+
+template <bool SPLIT>
 static int ns_iterate(NsGemmArgs& g, int steps, int last, hipStream_t st) {
     int rc;
     for (int it = 0; it < steps; ++it) {
         g.cur = it & 1;
-        g.lo_t = it + 2 == steps;                 // the X written now is read by the last iteration
-        if ((rc = ns_launch<T, NS_GRAM, SPLIT>(g, st)) != MVIT_OK) return rc;
-        if ((rc = ns_launch<T, NS_POLY, SPLIT>(g, st)) != MVIT_OK) return rc;
-        if (it + 1 < steps) rc = ns_launch<T, NS_STEP, SPLIT>(g, st);
-        else rc = last == NS_LAST16 ? ns_launch<T, NS_LAST16, SPLIT>(g, st)
-                : last == NS_LAST32 ? ns_launch<T, NS_LAST32, SPLIT>(g, st) : ns_launch<T, NS_MUON, SPLIT>(g, st);
+        if ((rc = ns_launch<NS_GRAM, SPLIT>(g, st)) != MVIT_OK) return rc;
+        if ((rc = ns_launch<NS_POLY, SPLIT>(g, st)) != MVIT_OK) return rc;
+        if (it + 1 < steps) rc = ns_launch<NS_STEP, SPLIT>(g, st);
+        else rc = last == NS_LAST16 ? ns_launch<NS_LAST16, SPLIT>(g, st)
+                : last == NS_LAST32 ? ns_launch<NS_LAST32, SPLIT>(g, st) : ns_launch<NS_MUON, SPLIT>(g, st);
         if (rc != MVIT_OK) return rc;
     }
     return MVIT_OK;
@@ -571,11 +663,14 @@ static int ns_run(const mvit_ns_matrix* mats, int count, const NsCall& k, void* 
         l.ws = g.ws = reinterpret_cast<h16*>(static_cast<char*>(workspace) + (int64_t)NS_MAX * NS_PARTS * 8);
         l.norm_coef = g.norm_coef = k.norm_coef;
         l.mu = k.mu; l.nesterov = k.nesterov; l.eps = k.eps;
-        l.lo_t = k.steps == 1;
         g.a = k.a; g.b = k.b; g.c = k.c; g.hyper = k.hyper; g.lr = k.lr; g.wd = k.wd;
+        // the matrices with the longest sums first, so that no launch ends on them
+        int order[NS_MAX];
+        for (int i = 0; i < l.n; ++i) order[i] = s + i;
+        std::stable_sort(order, order + l.n, [&](int x, int y) { return (int64_t)mats[x].rows + mats[x].cols > (int64_t)mats[y].rows + mats[y].cols; });
         int64_t off = 0, blocks = 0;
         for (int i = 0; i < l.n; ++i) {
-            const mvit_ns_matrix& t = mats[s + i];
+            const mvit_ns_matrix& t = mats[order[i]];
             const int64_t tiles = ((t.rows + 63) / 64) * (int64_t)((t.cols + 63) / 64);
             l.mat[i] = {t.u, muon ? t.momentum : nullptr, t.row_stride, t.col_stride, t.rows, t.cols, (uint32_t)off, (uint32_t)blocks};
             g.off[i] = (uint32_t)off;
@@ -598,20 +693,10 @@ static int ns_run(const mvit_ns_matrix* mats, int count, const NsCall& k, void* 
         }
         if (blocks > 0x7fffffff) return MVIT_EUNSUPPORTED;
         l.blocks = (uint32_t)blocks;
-        if (k.in_dtype == MVIT_F32) {
-            if (k.split) hipLaunchKernelGGL((ns_start_kernel<float, true>), dim3(l.blocks), dim3(256), 0, st, l);
-            else hipLaunchKernelGGL((ns_start_kernel<float, false>), dim3(l.blocks), dim3(256), 0, st, l);
-        } else {
-            if (k.split) hipLaunchKernelGGL((ns_start_kernel<bf16_t, true>), dim3(l.blocks), dim3(256), 0, st, l);
-            else hipLaunchKernelGGL((ns_start_kernel<bf16_t, false>), dim3(l.blocks), dim3(256), 0, st, l);
-        }
+        if (k.in_dtype == MVIT_F32) hipLaunchKernelGGL(ns_start_kernel<float>, dim3(l.blocks), dim3(256), 0, st, l);
+        else hipLaunchKernelGGL(ns_start_kernel<bf16_t>, dim3(l.blocks), dim3(256), 0, st, l);
         MVIT_LAUNCH_CHECK();
-        // tiles of 128 once there are enough of them to fill 256 CUs twice, else tiles of 64
-        int64_t big = 0;
-        for (int i = 0; i < l.n; ++i) big += (pad64(g.m[i]) + 127) / 128 * ((pad64(g.n[i]) + 127) / 128);
-        int rc;
-        if (big >= 512) rc = k.split ? ns_iterate<128, true>(g, k.steps, k.last, st) : ns_iterate<128, false>(g, k.steps, k.last, st);
-        else rc = k.split ? ns_iterate<64, true>(g, k.steps, k.last, st) : ns_iterate<64, false>(g, k.steps, k.last, st);
+        const int rc = k.split ? ns_iterate<true>(g, k.steps, k.last, st) : ns_iterate<false>(g, k.steps, k.last, st);
         if (rc != MVIT_OK) return rc;
     }
     return MVIT_OK;

@@ -8,15 +8,17 @@
 // Bound by HBM: 2 * itemsize bytes and six operations per channel.  The angle is not read from a table: the place times the frequency (in
 // turns) is one product in 64 bits -- a place of a million turns the fastest pair 160,000 times, which 32 bits would round to a hundredth
 // of a turn -- whose fraction goes to sincospif in 32 bits (angle off by at most 2^-24 of half a turn).  That costs about 40 VALU cycles
-// per pair and wave, half of what the memory time of the pair's row leaves free, and is shared by all heads that a thread walks.
+// per pair and wave -- as long as the memory takes for a pair of one row -- and is shared by the rows that a thread walks: the heads of a
+// batch entry, or of all of them where their places are the same.
 #include "common.h"
 
 struct RotaryArgs {
     mvit_rotary_tensor t[2];
     uint32_t first_block_1;        // blocks of t[1] begin here
-    uint32_t blocks_per_group[2];  // blocks that cover L tokens x tasks of one (batch, head group)
-    uint32_t groups[2];            // head groups per batch
-    int heads_per_thread[2];
+    uint32_t blocks_per_group[2];  // blocks that cover L tokens x tasks of one group of rows
+    uint32_t groups[2];            // groups of rows per span
+    int rows_per_thread[2];        // rows = (batch, head) pairs
+    int span[2];                   // rows that share their places: heads of one batch entry, or all
     int dim, pairs, axes;          // channels, rotated pairs of a head
     int tasks;                     // threads per token: pair chunks, then chunks of the channels that pass through
     int sec[MVIT_ROTARY_AXES];     // channels of each section
@@ -53,7 +55,44 @@ __device__ __forceinline__ void rot_store(T* p, const float (&f)[V]) {
     *reinterpret_cast<typename RotVec<T, V>::type*>(p) = v;
 }
 
-// A thread owns V pairs of one token (2 V channels: two vectors of V) in up to heads_per_thread heads.  INTER: the pairs are (2i, 2i + 1),
+// The two vectors of a thread.  Interleaved pairs are 2 V channels side by side, aligned to V of them: one access (a dword pair needs no
+// more than dword alignment).
+template <typename T, int V> struct RotPair { typedef T type __attribute__((ext_vector_type(2 * V), aligned(V * sizeof(T)))); };
+template <typename T, int V, bool INTER>
+__device__ __forceinline__ void rot_load_pair(const T* p, int ca, int cb, float (&u)[V], float (&w)[V]) {
+    if (INTER) {
+        const typename RotPair<T, V>::type v = *reinterpret_cast<const typename RotPair<T, V>::type*>(p + ca);
+#pragma unroll
+        for (int j = 0; j < 2 * V; ++j) {
+            float f;
+            if constexpr (sizeof(T) == 2) f = bf16_to_f32(v[j]);
+            else f = v[j];
+            if (j < V) u[j % V] = f;
+            else w[j % V] = f;
+        }
+    } else {
+        rot_load<T, V>(p + ca, u);
+        rot_load<T, V>(p + cb, w);
+    }
+}
+template <typename T, int V, bool INTER>
+__device__ __forceinline__ void rot_store_pair(T* p, int ca, int cb, const float (&u)[V], const float (&w)[V]) {
+    if (INTER) {
+        typename RotPair<T, V>::type v;
+#pragma unroll
+        for (int j = 0; j < 2 * V; ++j) {
+            const float f = j < V ? u[j % V] : w[j % V];
+            if constexpr (sizeof(T) == 2) v[j] = f32_to_bf16(f);
+            else v[j] = f;
+        }
+        *reinterpret_cast<typename RotPair<T, V>::type*>(p + ca) = v;
+    } else {
+        rot_store<T, V>(p + ca, u);
+        rot_store<T, V>(p + cb, w);
+    }
+}
+
+// A thread owns V pairs of one token (2 V channels: two vectors of V) in up to rows_per_thread rows.  INTER: the pairs are (2i, 2i + 1),
 // else (i, i + s / 2) within a section of s.  V divides what the host checked: every vector is aligned and none crosses a section's half
 // (interleaved: pairs of two sections may share a thread, each pair looks up its own axis).
 template <typename T, int V, bool INTER>
@@ -65,32 +104,34 @@ __global__ __launch_bounds__(256) void rotary_kernel(const RotaryArgs a) {
     const uint32_t item = in_row * 256u + threadIdx.x;
     const uint32_t l = item / (uint32_t)a.tasks, task = item - l * (uint32_t)a.tasks;
     if ((int64_t)l >= t.L) return;
-    const uint32_t b = row / a.groups[which], grp = row - b * a.groups[which];
-    const int h0 = (int)grp * a.heads_per_thread[which];
-    const int h1 = min(h0 + a.heads_per_thread[which], t.H);
+    const uint32_t sp = row / a.groups[which], grp = row - sp * a.groups[which];
+    const int r0 = (int)sp * a.span[which] + (int)grp * a.rows_per_thread[which];
+    const int r1 = min(r0 + a.rows_per_thread[which], ((int)sp + 1) * a.span[which]);
+    const uint32_t b = (uint32_t)r0 / (uint32_t)t.H;     // (one batch entry per span, or places shared by all)
 
-    const T* x = static_cast<const T*>(t.x) + (int64_t)b * t.xs[0] + (int64_t)l * t.xs[2];
-    T* y = static_cast<T*>(t.y) + (int64_t)b * t.ys[0] + (int64_t)l * t.ys[2];
-    const T* add = t.add ? static_cast<const T*>(t.add) + (int64_t)b * t.as[0] + (int64_t)l * t.as[2] : nullptr;
+    const T* const x0 = static_cast<const T*>(t.x) + (int64_t)l * t.xs[2];
+    T* const y0 = static_cast<T*>(t.y) + (int64_t)l * t.ys[2];
+    const T* const add0 = t.add ? static_cast<const T*>(t.add) + (int64_t)l * t.as[2] : nullptr;
     const int p0 = (int)task * V;           // first pair of this thread
     const int chunks = a.pairs / V;
 
     if ((int)task >= chunks) {              // channels that pass through
         const int c0 = 2 * a.pairs + ((int)task - chunks) * 2 * V;
-        for (int h = h0; h < h1; ++h) {
+        for (int row = r0; row < r1; ++row) {
+            const int64_t bi = row / t.H, h = row - (int)bi * t.H;
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
                 const int c = c0 + half * V;
                 if (c >= a.dim) break;
                 float f[V];
-                rot_load<T, V>(x + (int64_t)h * t.xs[1] + c, f);
-                if (add) {
+                rot_load<T, V>(x0 + bi * t.xs[0] + h * t.xs[1] + c, f);
+                if (add0) {
                     float g[V];
-                    rot_load<T, V>(add + (int64_t)h * t.as[1] + c, g);
+                    rot_load<T, V>(add0 + bi * t.as[0] + h * t.as[1] + c, g);
 #pragma unroll
                     for (int j = 0; j < V; ++j) f[j] += g[j];
                 }
-                rot_store<T, V>(y + (int64_t)h * t.ys[1] + c, f);
+                rot_store<T, V>(y0 + bi * t.ys[0] + h * t.ys[1] + c, f);
             }
         }
         return;
@@ -139,11 +180,12 @@ __global__ __launch_bounds__(256) void rotary_kernel(const RotaryArgs a) {
             else { ca = first + (p0 - first / 2); cb = ca + a.sec[axis] / 2; }
         }
     }
-    for (int h = h0; h < h1; ++h) {
+    for (int row = r0; row < r1; ++row) {
+        const int64_t bi = row / t.H, h = row - (int)bi * t.H;
+        const T* xh = x0 + bi * t.xs[0] + h * t.xs[1];
+        T* yh = y0 + bi * t.ys[0] + h * t.ys[1];
         float u[V], w[V];
-        const T* xh = x + (int64_t)h * t.xs[1];
-        rot_load<T, V>(xh + ca, u);
-        rot_load<T, V>(xh + cb, w);
+        rot_load_pair<T, V, INTER>(xh, ca, cb, u, w);
         float yu[V], yw[V];
 #pragma unroll
         for (int j = 0; j < V; ++j) {
@@ -158,15 +200,12 @@ __global__ __launch_bounds__(256) void rotary_kernel(const RotaryArgs a) {
                 yw[j] = u[j] * sn[j] + w[j] * cs[j];
             }
         }
-        if (add) {
-            rot_load<T, V>(add + (int64_t)h * t.as[1] + ca, u);
-            rot_load<T, V>(add + (int64_t)h * t.as[1] + cb, w);
+        if (add0) {
+            rot_load_pair<T, V, INTER>(add0 + bi * t.as[0] + h * t.as[1], ca, cb, u, w);
 #pragma unroll
             for (int j = 0; j < V; ++j) { yu[j] += u[j]; yw[j] += w[j]; }
         }
-        T* yh = y + (int64_t)h * t.ys[1];
-        rot_store<T, V>(yh + ca, yu);
-        rot_store<T, V>(yh + cb, yw);
+        rot_store_pair<T, V, INTER>(yh, ca, cb, yu, yw);
     }
 }
 
@@ -207,7 +246,7 @@ extern "C" int mvit_rotary(const mvit_rotary_tensor* tensors, int ntensors, int 
     uint64_t total_blocks = 0;
     for (int i = 0; i < 2; ++i) {
         a.first_block_1 = (uint32_t)total_blocks;
-        a.blocks_per_group[i] = 1; a.groups[i] = 1; a.heads_per_thread[i] = 1;
+        a.blocks_per_group[i] = 1; a.groups[i] = 1; a.rows_per_thread[i] = 1; a.span[i] = 1;
         if (i >= ntensors) { a.t[i] = a.t[0]; a.first_block_1 = 0xffffffffu; continue; }
         const mvit_rotary_tensor& t = a.t[i] = tensors[i];
         if (t.B < 0 || t.H < 0 || t.L < 0) return MVIT_EINVAL;
@@ -234,21 +273,23 @@ extern "C" int mvit_rotary(const mvit_rotary_tensor* tensors, int ntensors, int 
         }
     }
     a.tasks = a.pairs / (int)fit + (dim - channels + 2 * (int)fit - 1) / (2 * (int)fit);
-    // Heads per thread: one head each until there are two rounds of full workgroups on the 256 CUs, then more, so that a turn serves
-    // several heads (up to 8)
+    // Rows per thread: as many (up to 8) as leave 2048 workgroups = 32 waves on each of the 256 CUs, so that a turn serves several rows
     for (int i = 0; i < ntensors; ++i) {
         const mvit_rotary_tensor& t = a.t[i];
         if (i == 1) a.first_block_1 = (uint32_t)total_blocks;
         if (t.B == 0 || t.H == 0 || t.L == 0) continue;
         const uint64_t items = (uint64_t)t.L * a.tasks;
-        if (items > 0xffffff00u) return MVIT_EUNSUPPORTED;
+        if (items > 0xffffff00u || (int64_t)t.B * t.H > 0x7fffffff) return MVIT_EUNSUPPORTED;
         const uint64_t per = (items + 255) / 256;
-        int hpt = 1;
-        while (hpt < 8 && hpt < t.H && per * t.B * ((t.H + 2 * hpt - 1) / (2 * hpt)) >= 4096) hpt *= 2;
-        a.heads_per_thread[i] = hpt;
-        a.groups[i] = (uint32_t)((t.H + hpt - 1) / hpt);
+        const bool shared = !t.pos || t.ps[0] == 0;
+        const int span = shared ? t.B * t.H : t.H, spans = shared ? 1 : t.B;
+        int rpt = 1;
+        while (rpt < 8 && rpt < span && per * spans * (uint64_t)((span + 2 * rpt - 1) / (2 * rpt)) >= 2048) rpt *= 2;
+        a.rows_per_thread[i] = rpt;
+        a.span[i] = span;
+        a.groups[i] = (uint32_t)((span + rpt - 1) / rpt);
         a.blocks_per_group[i] = (uint32_t)per;
-        total_blocks += per * a.groups[i] * (uint64_t)t.B;
+        total_blocks += per * a.groups[i] * (uint64_t)spans;
         if (total_blocks > 0x7fffffffu) return MVIT_EUNSUPPORTED;
     }
     if (!total_blocks) return MVIT_OK;

@@ -13,6 +13,7 @@ CPU fallback.
 """
 import ctypes
 import math
+import struct
 
 import torch
 
@@ -21,14 +22,8 @@ from . import _hip
 _MAX_AXES, _MAX_PAIRS = 4, 256
 _POS = {torch.int32: 1, torch.int64: 2, torch.float32: 3}
 _LAYOUTS = {"half": 0, "interleaved": 1}
-_i3 = ctypes.c_int64 * 3
-
-
-class _Tensor(ctypes.Structure):
-    """mvit_rotary_tensor of include/mvit_hip.h."""
-    _fields_ = [("x", ctypes.c_void_p), ("y", ctypes.c_void_p), ("add", ctypes.c_void_p), ("pos", ctypes.c_void_p),
-                ("xs", _i3), ("ys", _i3), ("as_", _i3), ("ps", _i3), ("L", ctypes.c_int64), ("B", ctypes.c_int32), ("H", ctypes.c_int32),
-                ("pos_type", ctypes.c_int32), ("grid", ctypes.c_int32 * 4), ("origin", ctypes.c_double * 4), ("step", ctypes.c_double * 4)]
+_RECORD = struct.Struct("@4P12qq3i4i8d")        # mvit_rotary_tensor of include/mvit_hip.h
+_NO_GRID = (0,) * 4 + (0.0,) * 8
 
 
 class TokenGrid(object):
@@ -46,6 +41,8 @@ class TokenGrid(object):
         if not all(math.isfinite(v) for v in self.step + self.origin):
             raise ValueError("TokenGrid: step and origin must be finite")
         self.tokens = math.prod(self.sizes)
+        fill = lambda v, x: v + (x,) * (4 - len(v))  # noqa: E731
+        self.record = fill(self.sizes, 0) + fill(self.origin, 0.0) + fill(self.step, 0.0)      # as in mvit_rotary_tensor
 
     def __repr__(self):
         return "TokenGrid(%s, step=%s, origin=%s)" % (self.sizes, self.step, self.origin)
@@ -154,26 +151,27 @@ def add_(out, add):
 
 
 def _launch(xs, outs, adds, ps, dim, axes, sections, turns, layout, inverse):
-    x = xs[0]
-    rec = (_Tensor * len(xs))()
+    x, rec = xs[0], b""
     for i, (t, y, p) in enumerate(zip(xs, outs, ps)):
-        r = rec[i]
-        r.x, r.y = t.data_ptr(), y.data_ptr()
-        r.xs[:], r.ys[:] = t.stride()[:3], y.stride()[:3]
-        if adds is not None and adds[i] is not None:
-            r.add = adds[i].data_ptr()
-            r.as_[:] = adds[i].stride()[:3]
-        r.B, r.H, r.L = t.shape[0], t.shape[1], t.shape[2]
+        add = adds[i] if adds is not None else None
+        place, kind, steps, grid = 0, 0, (0, 0, 0), _NO_GRID
         if isinstance(p, TokenGrid):
-            n = len(p.sizes)
-            r.grid[:n], r.origin[:n], r.step[:n] = p.sizes, p.origin, p.step
+            grid = p.record
         elif p is not None:
-            r.pos, r.pos_type = p.data_ptr(), _POS[p.dtype]
-            r.ps[:] = (p.stride(0) if p.dim() == 3 and p.shape[0] > 1 else 0,) + tuple(p.stride()[-2:])
-    L = _hip.lib("fp16" if x.dtype == torch.float16 else "bf16")
-    with torch.cuda.device(x.device):
-        _hip.check(L.mvit_rotary(rec, len(xs), dim, axes, sections, turns, layout, 1 if inverse else 0,
-                                 _hip.F32 if x.dtype == torch.float32 else _hip.BF16, torch.cuda.current_stream().cuda_stream), "rotary")
+            place, kind, steps = p.data_ptr(), _POS[p.dtype], p.stride()
+            steps = (0,) + steps if len(steps) == 2 else steps if p.shape[0] > 1 else (0,) + steps[1:]
+        B, H, L, _ = t.shape
+        rec += _RECORD.pack(t.data_ptr(), y.data_ptr(), add.data_ptr() if add is not None else 0, place, *t.stride()[:3], *y.stride()[:3],
+                            *(add.stride()[:3] if add is not None else (0, 0, 0)), *steps, L, B, H, kind, *grid)
+    lib = _hip.lib("fp16" if x.dtype == torch.float16 else "bf16")
+    act = _hip.F32 if x.dtype == torch.float32 else _hip.BF16
+    args = (rec, len(xs), dim, axes, sections, turns, layout, 1 if inverse else 0, act)
+    if x.device.index == torch.cuda.current_device():
+        rc = lib.mvit_rotary(*args, torch.cuda.current_stream().cuda_stream)
+    else:
+        with torch.cuda.device(x.device):
+            rc = lib.mvit_rotary(*args, torch.cuda.current_stream().cuda_stream)
+    _hip.check(rc, "rotary")
 
 
 def _leaf_on_one_stream(t):
