@@ -7,9 +7,9 @@
 //
 // Bound by HBM: 2 * itemsize bytes and six operations per channel.  The angle is not read from a table: the place times the frequency (in
 // turns) is one product in 64 bits -- a place of a million turns the fastest pair 160,000 times, which 32 bits would round to a hundredth
-// of a turn -- whose fraction goes to sincospif in 32 bits (angle off by at most 2^-24 of half a turn).  That costs about 40 VALU cycles
-// per pair and wave -- as long as the memory takes for a pair of one row -- and is shared by the rows that a thread walks: the heads of a
-// batch entry, or of all of them where their places are the same.
+// of a turn -- whose fraction goes on in 32 bits (off by at most 2^-26 of a turn).  Sine and cosine of an eighth of a turn either way are
+// their Taylor polynomials (next terms: 1.8e-9 and 1e-10), the quarter turn is put back by a swap and two signs.  All of it is shared by
+// the rows that a thread walks: the heads of a batch entry, or of all of them where their places are the same.
 #include "common.h"
 
 struct RotaryArgs {
@@ -92,6 +92,18 @@ __device__ __forceinline__ void rot_store_pair(T* p, int ca, int cb, const float
     }
 }
 
+// sine and cosine of r turns, |r| <= 1/2
+__device__ __forceinline__ void rot_sincos(float r, float& sn, float& cs) {
+    const float q = __builtin_rintf(4.0f * r);
+    const float t = 6.283185307179586f * fmaf(-0.25f, q, r), t2 = t * t;
+    const float s = t * fmaf(t2, fmaf(t2, fmaf(t2, fmaf(t2, 1.0f / 362880, -1.0f / 5040), 1.0f / 120), -1.0f / 6), 1.0f);
+    const float c = fmaf(t2, fmaf(t2, fmaf(t2, fmaf(t2, fmaf(t2, -1.0f / 3628800, 1.0f / 40320), -1.0f / 720), 1.0f / 24), -0.5f), 1.0f);
+    const int n = (int)q;
+    const uint32_t ss = __float_as_uint(n & 1 ? c : s), cc = __float_as_uint(n & 1 ? s : c);
+    sn = __uint_as_float(ss ^ ((uint32_t)(n & 2) << 30));
+    cs = __uint_as_float(cc ^ ((uint32_t)((n + 1) & 2) << 30));
+}
+
 // A thread owns V pairs of one token (2 V channels: two vectors of V) in up to rows_per_thread rows.  INTER: the pairs are (2i, 2i + 1),
 // else (i, i + s / 2) within a section of s.  V divides what the host checked: every vector is aligned and none crosses a section's half
 // (interleaved: pairs of two sections may share a thread, each pair looks up its own axis).
@@ -108,6 +120,7 @@ __global__ __launch_bounds__(256) void rotary_kernel(const RotaryArgs a) {
     const int r0 = (int)sp * a.span[which] + (int)grp * a.rows_per_thread[which];
     const int r1 = min(r0 + a.rows_per_thread[which], ((int)sp + 1) * a.span[which]);
     const uint32_t b = (uint32_t)r0 / (uint32_t)t.H;     // (one batch entry per span, or places shared by all)
+    const int h0 = r0 - (int)b * t.H;
 
     const T* const x0 = static_cast<const T*>(t.x) + (int64_t)l * t.xs[2];
     T* const y0 = static_cast<T*>(t.y) + (int64_t)l * t.ys[2];
@@ -117,8 +130,8 @@ __global__ __launch_bounds__(256) void rotary_kernel(const RotaryArgs a) {
 
     if ((int)task >= chunks) {              // channels that pass through
         const int c0 = 2 * a.pairs + ((int)task - chunks) * 2 * V;
+        int64_t bi = b, h = h0;
         for (int row = r0; row < r1; ++row) {
-            const int64_t bi = row / t.H, h = row - (int)bi * t.H;
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
                 const int c = c0 + half * V;
@@ -133,6 +146,7 @@ __global__ __launch_bounds__(256) void rotary_kernel(const RotaryArgs a) {
                 }
                 rot_store<T, V>(y0 + bi * t.ys[0] + h * t.ys[1] + c, f);
             }
+            if (++h == t.H) { h = 0; ++bi; }
         }
         return;
     }
@@ -160,28 +174,30 @@ __global__ __launch_bounds__(256) void rotary_kernel(const RotaryArgs a) {
         }
     }
     float cs[V], sn[V];
-    int ca = 0, cb = 0;                     // channels of the thread's two vectors
+    int ca = 2 * p0, cb = 2 * p0 + V;       // channels of the thread's two vectors
     int axis = 0, first = 0;                // axis of the pair, first channel of its section
+    double at = place[0];
 #pragma unroll
     for (int j = 0; j < V; ++j) {
         const int p = p0 + j;
+        if (INTER || j == 0) {              // (half: no vector crosses a section)
 #pragma unroll
-        for (int n = 0; n < MVIT_ROTARY_AXES - 1; ++n)
-            if (axis == n && 2 * p >= first + a.sec[n] && n + 1 < a.axes) { first += a.sec[n]; axis = n + 1; }
-        double at = place[0];
+            for (int n = 1; n < MVIT_ROTARY_AXES; ++n)
+                if (axis == n - 1 && n < a.axes && 2 * p >= first + a.sec[n - 1]) { first += a.sec[n - 1]; axis = n; at = place[n]; }
+            if (!INTER) {
+                int sec = a.sec[0];
 #pragma unroll
-        for (int n = 1; n < MVIT_ROTARY_AXES; ++n) at = axis == n ? place[n] : at;
-        const double turn = at * a.turns[p];
-        const float r = (float)(turn - __builtin_rint(turn));
-        sincospif(2.0f * r, &sn[j], &cs[j]);
-        sn[j] *= a.sign;
-        if (j == 0) {
-            if (INTER) { ca = 2 * p0; cb = 2 * p0 + V; }
-            else { ca = first + (p0 - first / 2); cb = ca + a.sec[axis] / 2; }
+                for (int n = 1; n < MVIT_ROTARY_AXES; ++n) sec = axis == n ? a.sec[n] : sec;
+                ca = first + (p0 - first / 2);
+                cb = ca + sec / 2;
+            }
         }
+        const double turn = at * a.turns[p];
+        rot_sincos((float)(turn - __builtin_rint(turn)), sn[j], cs[j]);
+        sn[j] *= a.sign;
     }
+    int64_t bi = b, h = h0;
     for (int row = r0; row < r1; ++row) {
-        const int64_t bi = row / t.H, h = row - (int)bi * t.H;
         const T* xh = x0 + bi * t.xs[0] + h * t.xs[1];
         T* yh = y0 + bi * t.ys[0] + h * t.ys[1];
         float u[V], w[V];
@@ -206,6 +222,7 @@ __global__ __launch_bounds__(256) void rotary_kernel(const RotaryArgs a) {
             for (int j = 0; j < V; ++j) { yu[j] += u[j]; yw[j] += w[j]; }
         }
         rot_store_pair<T, V, INTER>(yh, ca, cb, yu, yw);
+        if (++h == t.H) { h = 0; ++bi; }
     }
 }
 
@@ -273,7 +290,8 @@ extern "C" int mvit_rotary(const mvit_rotary_tensor* tensors, int ntensors, int 
         }
     }
     a.tasks = a.pairs / (int)fit + (dim - channels + 2 * (int)fit - 1) / (2 * (int)fit);
-    // Rows per thread: as many (up to 8) as leave 2048 workgroups = 32 waves on each of the 256 CUs, so that a turn serves several rows
+    // Rows per thread: as many (up to 8) as leave 1024 workgroups, four for each of the 256 CUs, so that a turn serves several
+    // rows (four heads on 8 x 28 x 28, B = 8: 19.0 us with 2048, 18.5 with 1024, 18.8 with 512; six heads of 4099 packed tokens 32.6, 29.6, 29.4)
     for (int i = 0; i < ntensors; ++i) {
         const mvit_rotary_tensor& t = a.t[i];
         if (i == 1) a.first_block_1 = (uint32_t)total_blocks;
@@ -284,7 +302,7 @@ extern "C" int mvit_rotary(const mvit_rotary_tensor* tensors, int ntensors, int 
         const bool shared = !t.pos || t.ps[0] == 0;
         const int span = shared ? t.B * t.H : t.H, spans = shared ? 1 : t.B;
         int rpt = 1;
-        while (rpt < 8 && rpt < span && per * spans * (uint64_t)((span + 2 * rpt - 1) / (2 * rpt)) >= 2048) rpt *= 2;
+        while (rpt < 8 && rpt < span && per * spans * (uint64_t)((span + 2 * rpt - 1) / (2 * rpt)) >= 1024) rpt *= 2;
         a.rows_per_thread[i] = rpt;
         a.span[i] = span;
         a.groups[i] = (uint32_t)((span + rpt - 1) / rpt);
