@@ -249,6 +249,15 @@ __global__ __launch_bounds__(256) void ns_start_kernel(const NsLoadArgs a) {
 // X itself, A, B, and the result of a wide matrix; the mirrored tiles of A and B and the result of a tall matrix are turned on the way.
 enum { NS_GRAM = 0, NS_POLY = 1, NS_STEP = 2, NS_LAST16 = 3, NS_LAST32 = 4, NS_MUON = 5 };
 
+// Workgroups go to the eight XCDs in turn, each with an L2 of its own: runs of NS_RUN tiles, which share operand tiles, go to one XCD.
+#ifndef NS_RUN
+#define NS_RUN 32
+#endif
+__device__ __forceinline__ uint32_t ns_tile_of(uint32_t wg) {
+    const uint32_t xcd = wg & 7, slot = wg >> 3;
+    return (slot / NS_RUN * 8 + xcd) * NS_RUN + slot % NS_RUN;
+}
+
 template <int T, int G, int PHASE>
 constexpr int ns_lds_bytes() {
     const int stages = G * 2 * 2 * T * 128, sums = (G - 1) * 4096 * (T / 64) * (T / 64) * 4;
@@ -263,7 +272,8 @@ __global__ __launch_bounds__(256 * G, G == 1 ? 2 : 4) void ns_gemm_kernel(const 
     constexpr bool SYM = PHASE == NS_GRAM || PHASE == NS_POLY;
     constexpr bool LAST = PHASE >= NS_LAST16;
     extern __shared__ __attribute__((aligned(16))) char smem[];
-    const uint32_t blk = blockIdx.x;
+    const uint32_t blk = ns_tile_of(blockIdx.x);
+    if (blk >= a.blocks) return;
     const int id = ns_find([&](int i) { return a.first[i]; }, a.count, blk);
     const int m = a.m[id], n = a.n[id], mp = ns_pad(m), np = ns_pad(n);
     const NsRegion g(a.ws, a.off[id], m, n);
@@ -277,9 +287,12 @@ __global__ __launch_bounds__(256 * G, G == 1 ? 2 : 4) void ns_gemm_kernel(const 
         tn = J;
         tm = (int)(tile - (uint32_t)J * (J + 1) / 2);
     } else {
-        const int tiles_n = (mp + T - 1) / T;      // neighbouring workgroups share the tile of X
-        tm = tile / tiles_n;
-        tn = tile - tm * tiles_n;
+        // bands of eight tiles of B, through all of X: a run of tiles shares few of either
+        const uint32_t tiles_n = (mp + T - 1) / T, tiles_m = (np + T - 1) / T;
+        const uint32_t band = tile / (8 * tiles_m), in_band = tile - band * 8 * tiles_m;
+        const uint32_t width = min(8u, tiles_n - band * 8);
+        tm = in_band / width;
+        tn = band * 8 + (in_band - (uint32_t)tm * width);
     }
     const int m0 = tm * T, n0 = tn * T;
     const int lim_m = SYM ? mp : np, lim_n = mp;   // extents of the output
@@ -330,23 +343,26 @@ __global__ __launch_bounds__(256 * G, G == 1 ? 2 : 4) void ns_gemm_kernel(const 
 
     if (grp < steps) dma(grp, 0);
 
-    // X <- a X + B X: the sum begins at a X (without SPLIT: with it the many roundings at the size of a X would be what it is there to avoid)
+    // What is added to the product -- a X or b A -- comes through LDS too, in whole rows: the tile's high half flies under the last step's
+    // matrix instructions, its low half follows.  16-byte chunk c of row r lies at c ^ (r & 15) (T = 128) or c ^ ((r >> 1) & 7) (T = 64)
+    constexpr bool RES = PHASE != NS_GRAM, RES_LO = RES && (PHASE != NS_POLY || SPLIT);
     const h16* const res = PHASE == NS_POLY ? g.a() : g.x(a.cur);
     const h16* const reslo = PHASE == NS_POLY ? g.alo() : g.xlo(SPLIT ? a.cur : 0);
-    constexpr bool START = !SYM && !SPLIT;
-    auto residual = [&](int i, int j, int e4) {
-        const int M = m0 + wm + 32 * i + 8 * e4 + 4 * h, N = n0 + wn + 32 * j + r;
-        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (M < lim_m && N < lim_n) {
-            const int64_t at = (int64_t)N * lim_m + M;
-            const h16x4 hi = *reinterpret_cast<const h16x4*>(res + at);
-            x = make_float4((float)hi[0], (float)hi[1], (float)hi[2], (float)hi[3]);
-            if (PHASE != NS_POLY || SPLIT) {
-                const h16x4 lo = *reinterpret_cast<const h16x4*>(reslo + at);
-                x.x += (float)lo[0]; x.y += (float)lo[1]; x.z += (float)lo[2]; x.w += (float)lo[3];
-            }
+    auto res_dma = [=](const h16* src, int stage) {
+        constexpr int PIECES = T * T / 2048;       // of a wave
+#pragma unroll
+        for (int i = 0; i < PIECES; ++i) {
+            const int piece = wave * PIECES + i;
+            const int row = piece * (512 / T) + lane / (T / 8), slot = lane % (T / 8);
+            const int ch = T == 128 ? slot ^ (row & 15) : slot ^ ((row >> 1) & 7);
+            const int64_t at = (int64_t)min(n0 + row, lim_n - 1) * lim_m + min(m0 + ch * 8, lim_m - 8);
+            __builtin_amdgcn_global_load_lds((ns_gptr_t*)(src + at), (ns_lptr_t*)(lds + stage * STAGE + 1024 * piece), 16, 0, 0);
         }
-        return x;
+    };
+    auto res_read = [=](int stage, int i, int j, int e4) {
+        const int M = wm + 32 * i + 8 * e4 + 4 * h, N = wn + 32 * j + r;
+        const int ch = T == 128 ? (M >> 3) ^ (N & 15) : (M >> 3) ^ ((N >> 1) & 7);
+        return *reinterpret_cast<const h16x4*>(lds + stage * STAGE + N * (2 * T) + ch * 16 + (M & 4) * 2);
     };
     f32x16 acc[F][F];
 #pragma unroll
@@ -354,12 +370,7 @@ __global__ __launch_bounds__(256 * G, G == 1 ? 2 : 4) void ns_gemm_kernel(const 
 #pragma unroll
         for (int j = 0; j < F; ++j)
 #pragma unroll
-            for (int e4 = 0; e4 < 4; ++e4) {
-                float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-                if (START && grp == 0) x = residual(i, j, e4);
-                const float f = a.a * NS_S;
-                acc[i][j][4 * e4] = f * x.x; acc[i][j][4 * e4 + 1] = f * x.y; acc[i][j][4 * e4 + 2] = f * x.z; acc[i][j][4 * e4 + 3] = f * x.w;
-            }
+            for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
 
     const int q4 = (lane & 15) >> 2;               // transposing read: this lane names four columns of row 8 h + q4 (+ 4)
     const int tr_row = 8 * h + q4, tr_col = (16 * ((lane >> 4) & 1) + 4 * (lane & 3)) * 2;
@@ -386,6 +397,7 @@ __global__ __launch_bounds__(256 * G, G == 1 ? 2 : 4) void ns_gemm_kernel(const 
                 fq[i][ks] = *reinterpret_cast<const h16x8*>(sq + rq * 128 + (((2 * ks + h) ^ ((rq >> 1) & 7)) * 16));
             }
         if (kt + G < steps) dma(kt + G, (it + 1) & 1);
+        else if (RES && grp == 0) res_dma(res, (it + 1) & 1);
 #pragma unroll
         for (int ks = 0; ks < 4; ++ks)
 #pragma unroll
@@ -395,43 +407,45 @@ __global__ __launch_bounds__(256 * G, G == 1 ? 2 : 4) void ns_gemm_kernel(const 
                     acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fp[i][ks], fq[j][ks], acc[i][j], 0, 0, 0);
     }
 
-    if (G > 1) {        // the groups' sums, in order
+    const int last = ((steps + G - 1) / G - 1) & 1;          // the stage of the last step
+    float* const sums = reinterpret_cast<float*>(smem + 2 * STAGE);
+    if (RES || G > 1) {
         __syncthreads();
-        float* sums = reinterpret_cast<float*>(smem);
-        if (grp > 0)
+        if (RES_LO && grp == 0) res_dma(reslo, last);
+        if (G > 1 && grp > 0)
 #pragma unroll
             for (int i = 0; i < F; ++i)
 #pragma unroll
                 for (int j = 0; j < F; ++j)
 #pragma unroll
                     for (int e = 0; e < 16; ++e) sums[(((grp - 1) * 4 + wave) * F * F + i * F + j) * 1024 + e * 64 + lane] = acc[i][j][e];
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __syncthreads();
-        if (grp == 0)
-#pragma unroll
-            for (int o = 0; o < G - 1; ++o)
-#pragma unroll
-                for (int i = 0; i < F; ++i)
-#pragma unroll
-                    for (int j = 0; j < F; ++j)
-#pragma unroll
-                        for (int e = 0; e < 16; ++e) acc[i][j][e] += sums[((o * 4 + wave) * F * F + i * F + j) * 1024 + e * 64 + lane];
     }
-
     // ---- the new values, times 2^12 but for the last iteration's ---------------------------------------------------------------------------
     const float f_acc = PHASE == NS_POLY ? a.c / NS_S : LAST ? 1.0f / (NS_S * NS_S) : 1.0f / NS_S;
-    const float f_res = PHASE == NS_GRAM || START ? 0.f : PHASE == NS_POLY ? a.b : LAST ? a.a / NS_S : a.a;
+    const float f_res = PHASE == NS_POLY ? a.b : LAST ? a.a / NS_S : a.a;
     if (grp == 0)
 #pragma unroll
         for (int i = 0; i < F; ++i)
 #pragma unroll
             for (int j = 0; j < F; ++j) {
+                if (G > 1)          // the groups' sums, in order
+#pragma unroll
+                    for (int o = 0; o < G - 1; ++o)
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) acc[i][j][e] += sums[((o * 4 + wave) * F * F + i * F + j) * 1024 + e * 64 + lane];
 #pragma unroll
                 for (int e4 = 0; e4 < 4; ++e4) {
-                    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-                    if (PHASE != NS_GRAM && !START) x = residual(i, j, e4);
-                    const float xs[4] = {x.x, x.y, x.z, x.w};
+                    h16x4 hi, lo;
+                    if (RES) hi = res_read(last ^ 1, i, j, e4);
+                    if (RES_LO) lo = res_read(last, i, j, e4);
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) acc[i][j][4 * e4 + e] = f_res * xs[e] + f_acc * acc[i][j][4 * e4 + e];
+                    for (int e = 0; e < 4; ++e) {
+                        float& v = reinterpret_cast<float*>(&acc[i][j])[4 * e4 + e];
+                        v *= f_acc;
+                        if (RES) v += f_res * (RES_LO ? (float)hi[e] + (float)lo[e] : (float)hi[e]);
+                    }
                 }
                 ns_pin(acc[i][j]);
             }
@@ -602,9 +616,10 @@ static int ns_launch_as(NsGemmArgs& g, hipStream_t st) {
         flag = true;
     }
     const int64_t tiles = ns_tiles(g, T, PHASE == NS_GRAM || PHASE == NS_POLY, g.first);
-    if (tiles > 0x7fffffff) return MVIT_EUNSUPPORTED;
+    if (tiles > 0x7fffff00) return MVIT_EUNSUPPORTED;
     g.blocks = (uint32_t)tiles;
-    hipLaunchKernelGGL((ns_gemm_kernel<T, G, PHASE, SPLIT>), dim3(g.blocks), dim3(256 * G), LDS, st, g);
+    const uint32_t runs = (g.blocks + 8 * NS_RUN - 1) / (8 * NS_RUN);
+    hipLaunchKernelGGL((ns_gemm_kernel<T, G, PHASE, SPLIT>), dim3(runs * 8 * NS_RUN), dim3(256 * G), LDS, st, g);
     return hipGetLastError() == hipSuccess ? MVIT_OK : MVIT_ELAUNCH;
 }
 
@@ -613,7 +628,10 @@ static int ns_launch_as(NsGemmArgs& g, hipStream_t st) {
 template <int PHASE, bool SPLIT>
 static int ns_launch(NsGemmArgs& g, hipStream_t st) {
     constexpr bool SYM = PHASE == NS_GRAM || PHASE == NS_POLY;
-    if (ns_tiles(g, 128, SYM, nullptr) >= 512) return ns_launch_as<128, 1, PHASE, SPLIT>(g, st);
+    #ifndef NS_BIG
+#define NS_BIG 512
+#endif
+    if (ns_tiles(g, 128, SYM, nullptr) >= NS_BIG) return ns_launch_as<128, 1, PHASE, SPLIT>(g, st);
     int steps = 0;
     for (int i = 0; i < g.count; ++i) {
         const int k = (int)(pad64(PHASE == NS_GRAM ? g.n[i] : g.m[i]) / NS_BK) * (SPLIT ? 3 : 1);
