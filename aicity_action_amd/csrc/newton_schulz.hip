@@ -60,7 +60,7 @@ struct NsGemmArgs {
     float scale[NS_MAX];     // last iteration: factor of the update (Muon)
     uint8_t tall[NS_MAX];
     int count;
-    uint32_t blocks;
+    uint32_t blocks, run;    // tiles, and how many in a row go to one XCD
     h16* ws;
     float a, b, c;
     int cur;                 // which of the two buffers holds the current X
@@ -249,30 +249,28 @@ __global__ __launch_bounds__(256) void ns_start_kernel(const NsLoadArgs a) {
 // X itself, A, B, and the result of a wide matrix; the mirrored tiles of A and B and the result of a tall matrix are turned on the way.
 enum { NS_GRAM = 0, NS_POLY = 1, NS_STEP = 2, NS_LAST16 = 3, NS_LAST32 = 4, NS_MUON = 5 };
 
-// Workgroups go to the eight XCDs in turn, each with an L2 of its own: runs of NS_RUN tiles, which share operand tiles, go to one XCD.
-#ifndef NS_RUN
-#define NS_RUN 32
-#endif
-__device__ __forceinline__ uint32_t ns_tile_of(uint32_t wg) {
-    const uint32_t xcd = wg & 7, slot = wg >> 3;
-    return (slot / NS_RUN * 8 + xcd) * NS_RUN + slot % NS_RUN;
-}
-
-template <int T, int G, int PHASE>
-constexpr int ns_lds_bytes() {
-    const int stages = G * 2 * 2 * T * 128, sums = (G - 1) * 4096 * (T / 64) * (T / 64) * 4;
-    const int out = PHASE >= NS_LAST16 ? T * (T * 4 + 16) : 2 * T * (T * 2 + 16);
-    return stages > out ? (stages > sums ? stages : sums) : (out > sums ? out : sums);
+// Workgroups go to the eight XCDs in turn, each with an L2 of its own: a run of tiles, which share operand tiles, goes to one XCD.
+__device__ __forceinline__ uint32_t ns_tile_of(uint32_t wg, uint32_t run) {
+    const uint32_t xcd = wg & 7, slot = wg >> 3, r = slot / run;
+    return (r * 8 + xcd) * run + (slot - r * run);
 }
 
 template <int T, int G, int PHASE, bool SPLIT>
-__global__ __launch_bounds__(256 * G, G == 1 ? 2 : 4) void ns_gemm_kernel(const NsGemmArgs a) {
+constexpr int ns_lds_bytes() {
+    const int stages = G * 2 * (SPLIT ? 4 : 2) * T * 128;           // (the groups' sums lie within: behind the first group's stages)
+    const int out = PHASE >= NS_LAST16 ? T * (T * 4 + 16) : 2 * T * (T * 2 + 16);
+    return stages > out ? stages : out;
+}
+
+template <int T, int G, int PHASE, bool SPLIT>
+__global__ __launch_bounds__(256 * G, G == 1 ? (SPLIT && T == 128 ? 1 : 2) : G) void ns_gemm_kernel(const NsGemmArgs a) {
     constexpr int F = T / 64;                      // 32 x 32 accumulators per wave and direction
-    constexpr int STAGE = 2 * T * 128;             // bytes of P tile + Q tile
+    constexpr int PL = SPLIT ? 2 : 1;              // planes of an operand: high halves, low halves
+    constexpr int STAGE = 2 * PL * T * 128;        // bytes of the P tiles + Q tiles of a step
     constexpr bool SYM = PHASE == NS_GRAM || PHASE == NS_POLY;
     constexpr bool LAST = PHASE >= NS_LAST16;
     extern __shared__ __attribute__((aligned(16))) char smem[];
-    const uint32_t blk = ns_tile_of(blockIdx.x);
+    const uint32_t blk = ns_tile_of(blockIdx.x, a.run);
     if (blk >= a.blocks) return;
     const int id = ns_find([&](int i) { return a.first[i]; }, a.count, blk);
     const int m = a.m[id], n = a.n[id], mp = ns_pad(m), np = ns_pad(n);
@@ -324,21 +322,18 @@ __global__ __launch_bounds__(256 * G, G == 1 ? 2 : 4) void ns_gemm_kernel(const 
     }
     const int64_t k_step = by_k ? (int64_t)NS_BK * ld_src : NS_BK;
     const int nk = (PHASE == NS_GRAM ? np : mp) / NS_BK;
-    const int steps = SPLIT ? 3 * nk : nk;
+    const int steps = nk;
     const h16* const src_hi = PHASE == NS_GRAM ? g.x(a.cur) : PHASE == NS_POLY ? g.a() : is_q ? g.b() : g.x(a.cur);
     const h16* const src_lo = PHASE == NS_GRAM ? g.xlo(a.cur) : PHASE == NS_POLY ? g.alo() : is_q ? g.blo() : g.xlo(a.cur);
     auto dma = [=](int kt, int stage) {
-        const h16* base = src_hi;
-        if (SPLIT) {        // high high, then high low, then low high
-            const int seg = kt >= 2 * nk ? 2 : kt >= nk ? 1 : 0;
-            kt -= seg * nk;
-            if (seg == (is_q ? 1 : 2)) base = src_lo;
-        }
-        base += kt * k_step;
-        char* dst = lds + stage * STAGE + (is_q ? T * 128 : 0) + (wave & 1) * PW * 1024;
+        char* dst = lds + stage * STAGE + (is_q ? PL * T * 128 : 0) + (wave & 1) * PW * 1024;
 #pragma unroll
-        for (int i = 0; i < PW; ++i)
-            __builtin_amdgcn_global_load_lds((ns_gptr_t*)(base + src_off[i]), (ns_lptr_t*)(dst + 1024 * i), 16, 0, 0);
+        for (int pl = 0; pl < PL; ++pl) {
+            const h16* base = (pl ? src_lo : src_hi) + kt * k_step;
+#pragma unroll
+            for (int i = 0; i < PW; ++i)
+                __builtin_amdgcn_global_load_lds((ns_gptr_t*)(base + src_off[i]), (ns_lptr_t*)(dst + pl * T * 128 + 1024 * i), 16, 0, 0);
+        }
     };
 
     if (grp < steps) dma(grp, 0);
@@ -378,24 +373,27 @@ __global__ __launch_bounds__(256 * G, G == 1 ? 2 : 4) void ns_gemm_kernel(const 
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __syncthreads();                            // the step's tile has landed; everyone has read the stage refilled below
         if (G > 1 && kt >= steps) continue;
-        const char* sp = lds + (it & 1) * STAGE;
-        const char* sq = sp + T * 128;
-        h16x8 fp[F][4], fq[F][4];
+        h16x8 fp[PL][F][4], fq[PL][F][4];
 #pragma unroll
-        for (int ks = 0; ks < 4; ++ks)
+        for (int pl = 0; pl < PL; ++pl) {
+            const char* sp = lds + (it & 1) * STAGE + pl * T * 128;
+            const char* sq = sp + PL * T * 128;
 #pragma unroll
-            for (int i = 0; i < F; ++i) {
-                const int rp = wm + 32 * i + r, rq = wn + 32 * i + r;
-                if (SYM) fp[i][ks] = *reinterpret_cast<const h16x8*>(sp + rp * 128 + (((2 * ks + h) ^ ((rp >> 1) & 7)) * 16));
-                else {
-                    const int unit = (wm >> 5) + i, uu = T == 128 ? unit ^ q4 : unit ^ (q4 >> 1);
-                    const char* at = sp + (16 * ks + tr_row) * (2 * T) + uu * 64 + tr_col;
-                    const h16x4 lo = __builtin_bit_cast(h16x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((ns_lds_b4*)at));
-                    const h16x4 hi = __builtin_bit_cast(h16x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((ns_lds_b4*)(at + 4 * 2 * T)));
-                    fp[i][ks] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+            for (int ks = 0; ks < 4; ++ks)
+#pragma unroll
+                for (int i = 0; i < F; ++i) {
+                    const int rp = wm + 32 * i + r, rq = wn + 32 * i + r;
+                    if (SYM) fp[pl][i][ks] = *reinterpret_cast<const h16x8*>(sp + rp * 128 + (((2 * ks + h) ^ ((rp >> 1) & 7)) * 16));
+                    else {
+                        const int unit = (wm >> 5) + i, uu = T == 128 ? unit ^ q4 : unit ^ (q4 >> 1);
+                        const char* at = sp + (16 * ks + tr_row) * (2 * T) + uu * 64 + tr_col;
+                        const h16x4 lo = __builtin_bit_cast(h16x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((ns_lds_b4*)at));
+                        const h16x4 hi = __builtin_bit_cast(h16x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((ns_lds_b4*)(at + 4 * 2 * T)));
+                        fp[pl][i][ks] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+                    }
+                    fq[pl][i][ks] = *reinterpret_cast<const h16x8*>(sq + rq * 128 + (((2 * ks + h) ^ ((rq >> 1) & 7)) * 16));
                 }
-                fq[i][ks] = *reinterpret_cast<const h16x8*>(sq + rq * 128 + (((2 * ks + h) ^ ((rq >> 1) & 7)) * 16));
-            }
+        }
         if (kt + G < steps) dma(kt + G, (it + 1) & 1);
         else if (RES && grp == 0) res_dma(res, (it + 1) & 1);
 #pragma unroll
@@ -403,8 +401,13 @@ __global__ __launch_bounds__(256 * G, G == 1 ? 2 : 4) void ns_gemm_kernel(const 
 #pragma unroll
             for (int i = 0; i < F; ++i)
 #pragma unroll
-                for (int j = 0; j < F; ++j)
-                    acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fp[i][ks], fq[j][ks], acc[i][j], 0, 0, 0);
+                for (int j = 0; j < F; ++j) {
+                    if (SPLIT) {        // low high and high low first: they are small
+                        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fp[PL - 1][i][ks], fq[0][j][ks], acc[i][j], 0, 0, 0);
+                        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fp[0][i][ks], fq[PL - 1][j][ks], acc[i][j], 0, 0, 0);
+                    }
+                    acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fp[0][i][ks], fq[0][j][ks], acc[i][j], 0, 0, 0);
+                }
     }
 
     const int last = ((steps + G - 1) / G - 1) & 1;          // the stage of the last step
@@ -606,7 +609,7 @@ static int64_t ns_tiles(const NsGemmArgs& g, int side, bool sym, uint32_t* first
 
 template <int T, int G, int PHASE, bool SPLIT>
 static int ns_launch_as(NsGemmArgs& g, hipStream_t st) {
-    constexpr int LDS = ns_lds_bytes<T, G, PHASE>();
+    constexpr int LDS = ns_lds_bytes<T, G, PHASE, SPLIT>();
     static DevFlags done;
     DevFlag flag = dev_flag(done);
     if (LDS > 65536 && !flag) {
@@ -618,26 +621,25 @@ static int ns_launch_as(NsGemmArgs& g, hipStream_t st) {
     const int64_t tiles = ns_tiles(g, T, PHASE == NS_GRAM || PHASE == NS_POLY, g.first);
     if (tiles > 0x7fffff00) return MVIT_EUNSUPPORTED;
     g.blocks = (uint32_t)tiles;
-    const uint32_t runs = (g.blocks + 8 * NS_RUN - 1) / (8 * NS_RUN);
-    hipLaunchKernelGGL((ns_gemm_kernel<T, G, PHASE, SPLIT>), dim3(runs * 8 * NS_RUN), dim3(256 * G), LDS, st, g);
+    // runs of about 32 tiles (16 and 64 measured the same), as many for every XCD
+    const uint32_t rounds = (g.blocks + 255) / 256;
+    g.run = (g.blocks + 8 * rounds - 1) / (8 * rounds);
+    hipLaunchKernelGGL((ns_gemm_kernel<T, G, PHASE, SPLIT>), dim3(rounds * 8 * g.run), dim3(256 * G), LDS, st, g);
     return hipGetLastError() == hipSuccess ? MVIT_OK : MVIT_ELAUNCH;
 }
 
-// Tiles of 128 once there are two for each of the 256 CUs, else tiles of 64; four groups of waves per tile where even those leave CUs idle
-// and the longest sum has steps for them.
+// Tiles of 128 once there are two for each of the 256 CUs, else tiles of 64; four groups of waves per tile (SPLIT, whose
+// stages are twice as large: two) where even those leave CUs idle and the longest sum has steps for them.
 template <int PHASE, bool SPLIT>
 static int ns_launch(NsGemmArgs& g, hipStream_t st) {
     constexpr bool SYM = PHASE == NS_GRAM || PHASE == NS_POLY;
-    #ifndef NS_BIG
-#define NS_BIG 512
-#endif
-    if (ns_tiles(g, 128, SYM, nullptr) >= NS_BIG) return ns_launch_as<128, 1, PHASE, SPLIT>(g, st);
+    if (ns_tiles(g, 128, SYM, nullptr) >= 512) return ns_launch_as<128, 1, PHASE, SPLIT>(g, st);
     int steps = 0;
     for (int i = 0; i < g.count; ++i) {
-        const int k = (int)(pad64(PHASE == NS_GRAM ? g.n[i] : g.m[i]) / NS_BK) * (SPLIT ? 3 : 1);
+        const int k = (int)(pad64(PHASE == NS_GRAM ? g.n[i] : g.m[i]) / NS_BK);
         steps = k > steps ? k : steps;
     }
-    if (steps >= 8 && ns_tiles(g, 64, SYM, nullptr) <= 256) return ns_launch_as<64, 4, PHASE, SPLIT>(g, st);
+    if (steps >= 8 && ns_tiles(g, 64, SYM, nullptr) <= 256) return ns_launch_as<64, SPLIT ? 2 : 4, PHASE, SPLIT>(g, st);
     return ns_launch_as<64, 1, PHASE, SPLIT>(g, st);
 }
 
