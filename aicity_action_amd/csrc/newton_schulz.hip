@@ -17,6 +17,7 @@
 #include "common.h"
 #include <string.h>
 #include <algorithm>
+#include <type_traits>
 
 typedef _Float16 h16;
 typedef __attribute__((ext_vector_type(8))) _Float16 h16x8;
@@ -561,6 +562,302 @@ __global__ __launch_bounds__(256 * G, G == 1 ? (SPLIT && T == 128 ? 1 : 2) : G) 
     }
 }
 
+// ---- 4. small matrices: everything in one workgroup -------------------------------------------------------------------------------------
+// A matrix of at most 48 (SPLIT: 32) tiles of 32 x 32 that fits into the 160 KB of LDS with A and B takes all iterations in one workgroup of
+// sixteen waves, and a call of such matrices is one launch instead of seventeen of 4 to 7 us each (96 x 288).  X stays in the accumulators
+// in single precision.  A lane holds a column of the array the matrix comes from, an accumulator quad four of its rows, so that global
+// accesses are whole lines; LDS holds the fp16 copy (SPLIT: both halves) as Y[column][row], which is X where the matrix is tall and X^T
+// where it is wide, and the products read it along its rows or, with the transposing read, down them as that asks.  Rows in LDS are 16
+// bytes longer than their values, so that the 16 rows a read serves together fall on different banks.
+#define NS_SMALL_MAX 56
+#define NS_SMALL_WAVES 16
+#define NS_SMALL_LDS 163840
+struct NsSmallMat {
+    const void* u;
+    float* mom;
+    void* out;
+    int64_t rs, cs;
+    int32_t rows, cols;
+    float scale;
+    int32_t pad;
+};
+struct NsSmallArgs {
+    NsSmallMat mat[NS_SMALL_MAX];
+    const float* norm_coef;
+    const float* hyper;
+    float mu, eps, a, b, c, lr, wd;
+    int nesterov, steps;
+};
+__host__ __device__ static inline int ns_pad32(int v) { return (v + 31) & ~31; }
+static inline int64_t ns_small_bytes(int rows, int cols, bool split) {
+    const int64_t mp = ns_pad32(rows < cols ? rows : cols), np = ns_pad32(rows < cols ? cols : rows);
+    if (mp > 128 || mp * np > (split ? 32 : 48) * 1024) return -1;
+    const int64_t y = rows > cols ? mp * (np * 2 + 16) : np * (mp * 2 + 16);
+    const int64_t bytes = (split ? 2 : 1) * (y + 2 * mp * (mp * 2 + 16)) + 256;
+    return bytes <= NS_SMALL_LDS ? bytes : -1;
+}
+
+// An array of R x C elements with element strides rs and cs as a buffer resource: reads past its end give zero, writes past it are dropped,
+// so a tile's sixteen accesses need one address and no comparison of rows.  (The whole offset goes into the address register, which the
+// hardware compares with the size; offsets of the padded extents fit 31 bits.)
+template <typename T>
+struct NsArray {
+    __amdgpu_buffer_rsrc_t rsrc;
+    int rs, cs;
+    __device__ __forceinline__ NsArray(const void* p, int R, int C, int rs_, int cs_)
+        : rsrc(__builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, ((R - 1) * rs_ + (C - 1) * cs_ + 1) * (int)sizeof(T), 0x27000)),
+          rs(rs_ * (int)sizeof(T)), cs(cs_ * (int)sizeof(T)) {}
+    __device__ __forceinline__ int at(int row, int col) const { return row * rs + col * cs; }
+    __device__ __forceinline__ float load(int at, int row) const {
+        if constexpr (sizeof(T) == 4) return __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(rsrc, at + row * rs, 0, 0));
+        else return bf16_to_f32(__builtin_amdgcn_raw_buffer_load_b16(rsrc, at + row * rs, 0, 0));
+    }
+    __device__ __forceinline__ void store(float v, int at, int row) const {
+        if constexpr (sizeof(T) == 4) __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(v), rsrc, at + row * rs, 0, 0);
+        else __builtin_amdgcn_raw_buffer_store_b16(f32_to_bf16(v), rsrc, at + row * rs, 0, 0);
+    }
+};
+
+template <int PHASE, typename T, int TPW, bool SPLIT, bool TALL>
+__device__ __forceinline__ void ns_small_body(const NsSmallArgs& a, const NsSmallMat& t, char* smem) {
+    constexpr int PL = SPLIT ? 2 : 1;
+    typedef std::conditional_t<PHASE == NS_LAST16, bf16_t, float> out_t;
+    const int R = t.rows, C = t.cols;
+    const int rp = ns_pad32(R), cp = ns_pad32(C), mp = TALL ? cp : rp, np = TALL ? rp : cp;
+    const int nb = mp / 32, row_tiles = rp / 32, tiles = row_tiles * (cp / 32);
+    const int ldy = rp * 2 + 16, lda = mp * 2 + 16;             // bytes of a row of Y, and of A and B
+    const int ypl = cp * ldy, apl = mp * lda;                   // bytes of a plane
+    char* const sy = smem + 256;
+    char* const sa = sy + PL * ypl;
+    char* const sb = sa + PL * apl;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane0 = threadIdx.x & 63;
+    const float coef = a.norm_coef ? a.norm_coef[1] : 1.0f;
+    const bool bad = ns_bad(a.norm_coef);
+    // the wave's k-th tile: rows from 32 rt, columns from 32 ct of the array; element 4 e4 + e of lane (r, h): row 8 e4 + 4 h + e, column r
+    auto tile_of = [=](int k, int& rt, int& ct) {
+        const int tile = wave + NS_SMALL_WAVES * k;
+        ct = tile / row_tiles;
+        rt = tile - ct * row_tiles;
+        return tile < tiles;
+    };
+    const int r0 = lane0 & 31, h0 = lane0 >> 5;
+    auto read_all = [=](const auto& arr, f32x16 (&v)[TPW]) {
+#pragma unroll
+        for (int k = 0; k < TPW; ++k) {
+            int rt, ct;
+            if (tile_of(k, rt, ct)) {
+                const int at = arr.at(32 * rt + 4 * h0, 32 * ct + r0);
+#pragma unroll
+                for (int e = 0; e < 16; ++e) v[k][e] = arr.load(at, 8 * (e >> 2) + (e & 3));
+            }
+        }
+    };
+    auto write_all = [=](const auto& arr, const f32x16 (&v)[TPW]) {
+#pragma unroll
+        for (int k = 0; k < TPW; ++k) {
+            int rt, ct;
+            if (tile_of(k, rt, ct) && 32 * ct + r0 < C) {
+                const int at = arr.at(32 * rt + 4 * h0, 32 * ct + r0);
+#pragma unroll
+                for (int e = 0; e < 16; ++e) arr.store(v[k][e], at, 8 * (e >> 2) + (e & 3));
+            }
+        }
+    };
+    f32x16 x[TPW];
+#pragma unroll
+    for (int k = 0; k < TPW; ++k)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) x[k][e] = 0.f;
+    read_all(NsArray<T>(t.u, R, C, (int)t.rs, (int)t.cs), x);
+    if (PHASE == NS_MUON) {
+        const NsArray<float> arr(t.mom, R, C, C, 1);
+        f32x16 mo[TPW];
+#pragma unroll
+        for (int k = 0; k < TPW; ++k)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) mo[k][e] = 0.f;
+        read_all(arr, mo);
+#pragma unroll
+        for (int k = 0; k < TPW; ++k)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                const float g = x[k][e], v = a.mu * mo[k][e] + (1.0f - a.mu) * (g * coef);
+                x[k][e] = a.nesterov ? (1.0f - a.mu) * (g * coef) + a.mu * v : v;
+                mo[k][e] = v;
+            }
+        if (!bad) write_all(arr, mo);
+    }
+    double sq = 0.0;
+#pragma unroll
+    for (int k = 0; k < TPW; ++k) {
+        int rt, ct;
+        const bool ok = tile_of(k, rt, ct) && 32 * ct + r0 < C;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+            const float v = ok && 32 * rt + 8 * (e >> 2) + 4 * h0 + (e & 3) < R ? x[k][e] : 0.f;
+            x[k][e] = v;
+            sq += (double)v * (double)v;
+        }
+    }
+    {
+        double* red = reinterpret_cast<double*>(smem);
+#pragma unroll
+        for (int off = 32; off >= 1; off >>= 1) sq += __shfl_xor(sq, off, 64);
+        if (lane0 == 0) red[wave] = sq;
+        __syncthreads();
+        double s = 0.0;
+#pragma unroll
+        for (int k = 0; k < NS_SMALL_WAVES; ++k) s += red[k];
+        const float f = (float)(1.0 / (sqrt(s) + (double)a.eps)) * NS_S;
+#pragma unroll
+        for (int k = 0; k < TPW; ++k)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) x[k][e] *= f;
+    }
+
+    const std::true_type down{};
+    const std::false_type along{};
+    for (int it = 0; it < a.steps; ++it) {
+        int lane = lane0;           // made anew every iteration: addresses are cheaper recomputed than kept in registers through all of them
+        ns_pin(lane);
+        const int r = lane & 31, h = lane >> 5, q4 = (lane & 15) >> 2, c16 = 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+        // four values along M of a tile into row N
+        auto put = [=](char* dst, int ld, int plane, const float (&v)[4], int N, int M) {
+            h16x4 hi, lo;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                float p = v[e];
+                ns_pin(p);
+                hi[e] = (h16)p;
+                lo[e] = (h16)(p - (float)hi[e]);
+            }
+            *reinterpret_cast<h16x4*>(dst + N * ld + M * 2) = hi;
+            if (SPLIT) *reinterpret_cast<h16x4*>(dst + plane + N * ld + M * 2) = lo;
+        };
+        // one 32 x 32 tile of sum_k P(k, M) Q(k, N): an operand's k runs along its rows, or down them (transposing read)
+        auto start = [=](auto tr, const char* p, int ld, int at) {
+            return decltype(tr)::value ? p + (8 * h + q4) * ld + (at + c16) * 2 : p + (at + r) * ld + 16 * h;
+        };
+        auto fetch = [=](auto tr, const char* p, int ld) {
+            if (decltype(tr)::value) {
+                const h16x4 lo = __builtin_bit_cast(h16x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((ns_lds_b4*)p));
+                const h16x4 hi = __builtin_bit_cast(h16x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((ns_lds_b4*)(p + 4 * ld)));
+                return (h16x8)__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+            }
+            return *reinterpret_cast<const h16x8*>(p);
+        };
+        auto product = [=](auto trp, auto trq, const char* P, int ldp, int ppl, const char* Q, int ldq, int qpl, int M0, int N0, int K) {
+            f32x16 acc;
+#pragma unroll
+            for (int e = 0; e < 16; ++e) acc[e] = 0.f;
+            const char* p0 = start(trp, P, ldp, M0);
+            const char* q0 = start(trq, Q, ldq, N0);
+            const int pk = decltype(trp)::value ? 16 * ldp : 32, qk = decltype(trq)::value ? 16 * ldq : 32;      // bytes of 16 steps of k
+            for (int k = 0; k < K; k += 32) {           // K is a multiple of 32
+                h16x8 fp[2][PL], fq[2][PL];
+#pragma unroll
+                for (int s = 0; s < 2; ++s) {
+#pragma unroll
+                    for (int pl = 0; pl < PL; ++pl) {
+                        fp[s][pl] = fetch(trp, p0 + pl * ppl, ldp);
+                        fq[s][pl] = fetch(trq, q0 + pl * qpl, ldq);
+                    }
+                    p0 += pk;
+                    q0 += qk;
+                }
+#pragma unroll
+                for (int s = 0; s < 2; ++s) {
+                    if (SPLIT) {
+                        acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(fp[s][PL - 1], fq[s][0], acc, 0, 0, 0);
+                        acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(fp[s][0], fq[s][PL - 1], acc, 0, 0, 0);
+                    }
+                    acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(fp[s][0], fq[s][0], acc, 0, 0, 0);
+                }
+            }
+            return acc;
+        };
+#pragma unroll
+        for (int k = 0; k < TPW; ++k) {
+            int rt, ct;
+            if (tile_of(k, rt, ct))
+#pragma unroll
+                for (int e4 = 0; e4 < 4; ++e4)
+                    put(sy, ldy, ypl, {x[k][4 * e4], x[k][4 * e4 + 1], x[k][4 * e4 + 2], x[k][4 * e4 + 3]}, 32 * ct + r, 32 * rt + 8 * e4 + 4 * h);
+        }
+        __syncthreads();
+        const int ti = wave / nb, tj = wave - ti * nb;          // the wave's tile of A and B
+        if (wave < nb * nb) {
+            const f32x16 acc = TALL ? product(along, along, sy, ldy, ypl, sy, ldy, ypl, 32 * ti, 32 * tj, np)
+                                    : product(down, down, sy, ldy, ypl, sy, ldy, ypl, 32 * ti, 32 * tj, np);
+#pragma unroll
+            for (int e4 = 0; e4 < 4; ++e4) {
+                const float f = 1.0f / NS_S;
+                put(sa, lda, apl, {f * acc[4 * e4], f * acc[4 * e4 + 1], f * acc[4 * e4 + 2], f * acc[4 * e4 + 3]}, 32 * tj + r, 32 * ti + 8 * e4 + 4 * h);
+            }
+        }
+        __syncthreads();
+        if (wave < nb * nb) {
+            const f32x16 acc = product(along, along, sa, lda, apl, sa, lda, apl, 32 * ti, 32 * tj, mp);
+#pragma unroll
+            for (int e4 = 0; e4 < 4; ++e4) {
+                const int N = 32 * tj + r, M = 32 * ti + 8 * e4 + 4 * h;
+                const h16x4 hi = *reinterpret_cast<const h16x4*>(sa + N * lda + M * 2);
+                float v[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[e] = (float)hi[e];
+                if (SPLIT) {
+                    const h16x4 lo = *reinterpret_cast<const h16x4*>(sa + apl + N * lda + M * 2);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) v[e] += (float)lo[e];
+                }
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[e] = a.b * v[e] + a.c / NS_S * acc[4 * e4 + e];
+                put(sb, lda, apl, v, N, M);
+            }
+        }
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < TPW; ++k) {
+            int rt, ct;
+            if (tile_of(k, rt, ct)) {
+                const f32x16 acc = TALL ? product(down, along, sy, ldy, ypl, sb, lda, apl, 32 * rt, 32 * ct, mp)
+                                        : product(along, along, sb, lda, apl, sy, ldy, ypl, 32 * rt, 32 * ct, mp);
+#pragma unroll
+                for (int e = 0; e < 16; ++e) x[k][e] = a.a * x[k][e] + acc[e] * (1.0f / NS_S);
+            }
+        }
+        __syncthreads();
+    }
+
+    if (PHASE == NS_MUON) {
+        if (bad) return;
+        const float lr = a.hyper ? a.hyper[0] : a.lr;
+        const float keep = 1.0f - lr * a.wd, step = lr * t.scale;
+        const NsArray<float> arr(t.out, R, C, C, 1);
+        f32x16 w[TPW];
+        read_all(arr, w);
+#pragma unroll
+        for (int k = 0; k < TPW; ++k)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) x[k][e] = w[k][e] * keep - step * (x[k][e] * (1.0f / NS_S));
+        write_all(arr, x);
+    } else {
+#pragma unroll
+        for (int k = 0; k < TPW; ++k)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) x[k][e] *= 1.0f / NS_S;
+        write_all(NsArray<out_t>(t.out, R, C, C, 1), x);
+    }
+}
+
+template <int PHASE, typename T, int TPW, bool SPLIT>
+__global__ __launch_bounds__(64 * NS_SMALL_WAVES) void ns_small_kernel(const NsSmallArgs a) {
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    const NsSmallMat t = a.mat[blockIdx.x];
+    if (t.rows > t.cols) ns_small_body<PHASE, T, TPW, SPLIT, true>(a, t, smem);
+    else ns_small_body<PHASE, T, TPW, SPLIT, false>(a, t, smem);
+}
+
 // ---- host side ------------------------------------------------------------------------------------------------------------------------
 static inline int64_t pad64(int64_t v) { return (v + 63) & ~(int64_t)63; }
 
@@ -580,12 +877,32 @@ static int ns_check(const mvit_ns_matrix* mats, int count) {
     return MVIT_OK;
 }
 
+// What a set is computed with: matrices of at most 32 rows or columns always from pairs -- the rounding of their few entries of A and B does
+// not average out (3 x 2: 0.4 %), and their products are short.  small: every matrix fits one workgroup.
+static void ns_plan(const mvit_ns_matrix* mats, int count, int asked, bool& split, bool& small) {
+    split = asked != 0;
+    small = true;
+    bool tiny = true;
+    for (int i = 0; i < count; ++i) tiny = tiny && (mats[i].rows <= 32 || mats[i].cols <= 32);
+    if (tiny) split = true;
+    for (int i = 0; i < count; ++i) {
+        const mvit_ns_matrix& t = mats[i];
+        const int64_t rs = t.row_stride, cs = t.col_stride, most = (int64_t)1 << 28;
+        small = small && ns_small_bytes(t.rows, t.cols, split) > 0 && rs >= 0 && cs >= 0 && rs < most && cs < most &&
+                (ns_pad32(t.rows) - 1) * rs + (ns_pad32(t.cols) - 1) * cs < most;       // (31-bit byte offsets, padding included)
+    }
+}
+
 extern "C" int mvit_ns_matrix_bytes(void) { return (int)sizeof(mvit_ns_matrix); }
 
 // sets of at most NS_MAX matrices run one after the other in the same workspace
 extern "C" int64_t mvit_newton_schulz_workspace_bytes(const mvit_ns_matrix* mats, int count, int split) {
     const int rc = ns_check(mats, count);
     if (rc != MVIT_OK) return rc;
+    bool pairs, small;
+    ns_plan(mats, count, split, pairs, small);
+    if (small) return 0;
+    split = pairs;
     int64_t most = 0;
     for (int s = 0; s < count; s += NS_MAX) {
         int64_t units = 0;
@@ -666,13 +983,67 @@ struct NsCall {
     const float *norm_coef, *hyper;
 };
 
+template <int PHASE, typename T, int TPW, bool SPLIT>
+static int ns_small_launch_as(const NsSmallArgs& g, int count, int lds, hipStream_t st) {
+    static DevFlags done;
+    DevFlag flag = dev_flag(done);
+    if (!flag) {
+        if (hipFuncSetAttribute(reinterpret_cast<const void*>(&ns_small_kernel<PHASE, T, TPW, SPLIT>), hipFuncAttributeMaxDynamicSharedMemorySize,
+                                NS_SMALL_LDS) != hipSuccess)
+            return MVIT_ELAUNCH;
+        flag = true;
+    }
+    hipLaunchKernelGGL((ns_small_kernel<PHASE, T, TPW, SPLIT>), dim3(count), dim3(64 * NS_SMALL_WAVES), lds, st, g);
+    return hipGetLastError() == hipSuccess ? MVIT_OK : MVIT_ELAUNCH;
+}
+template <int PHASE, typename T>
+static int ns_small_launch(const NsSmallArgs& g, int count, int lds, int tiles, bool split, hipStream_t st) {
+    if (split) return ns_small_launch_as<PHASE, T, 32 / NS_SMALL_WAVES, true>(g, count, lds, st);
+    return tiles <= 32 ? ns_small_launch_as<PHASE, T, 32 / NS_SMALL_WAVES, false>(g, count, lds, st)
+                       : ns_small_launch_as<PHASE, T, 48 / NS_SMALL_WAVES, false>(g, count, lds, st);
+}
+
+// All matrices small: one launch (of up to 56) does everything.  A set with a larger one takes the launches of the larger one's anyway.
+static int ns_run_small(const mvit_ns_matrix* mats, int count, const NsCall& k, bool split, hipStream_t st) {
+    const bool muon = k.last == NS_MUON;
+    for (int s = 0; s < count; s += NS_SMALL_MAX) {
+        NsSmallArgs g;
+        memset(&g, 0, sizeof g);
+        const int c = count - s < NS_SMALL_MAX ? count - s : NS_SMALL_MAX;
+        int64_t lds = 0;
+        int tiles = 0;
+        for (int i = 0; i < c; ++i) {
+            const mvit_ns_matrix& t = mats[s + i];
+            g.mat[i] = {t.u, muon ? t.momentum : nullptr, muon ? static_cast<void*>(t.w) : t.out, t.row_stride, t.col_stride, t.rows, t.cols, t.scale, 0};
+            lds = std::max(lds, ns_small_bytes(t.rows, t.cols, split));
+            tiles = std::max(tiles, ns_pad32(t.rows) / 32 * (ns_pad32(t.cols) / 32));
+        }
+        g.norm_coef = k.norm_coef; g.hyper = k.hyper;
+        g.mu = k.mu; g.eps = k.eps; g.a = k.a; g.b = k.b; g.c = k.c; g.lr = k.lr; g.wd = k.wd;
+        g.nesterov = k.nesterov; g.steps = k.steps;
+        int rc;
+        if (muon) rc = ns_small_launch<NS_MUON, float>(g, c, (int)lds, tiles, split, st);
+        else if (k.in_dtype == MVIT_F32)
+            rc = k.last == NS_LAST16 ? ns_small_launch<NS_LAST16, float>(g, c, (int)lds, tiles, split, st)
+                                     : ns_small_launch<NS_LAST32, float>(g, c, (int)lds, tiles, split, st);
+        else
+            rc = k.last == NS_LAST16 ? ns_small_launch<NS_LAST16, bf16_t>(g, c, (int)lds, tiles, split, st)
+                                     : ns_small_launch<NS_LAST32, bf16_t>(g, c, (int)lds, tiles, split, st);
+        if (rc != MVIT_OK) return rc;
+    }
+    return MVIT_OK;
+}
+
 static int ns_run(const mvit_ns_matrix* mats, int count, const NsCall& k, void* workspace, int64_t bytes, hipStream_t st) {
     const bool muon = k.last == NS_MUON;
     const int64_t need = mvit_newton_schulz_workspace_bytes(mats, count, k.split);
     if (need < 0) return (int)need;
-    if (!workspace || bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 127) || k.steps < 1) return MVIT_EINVAL;
+    if (bytes < need || (need && !workspace) || (reinterpret_cast<uintptr_t>(workspace) & 127) || k.steps < 1) return MVIT_EINVAL;
     for (int i = 0; i < count; ++i)
         if (!mats[i].u || (muon ? !mats[i].w || !mats[i].momentum : !mats[i].out)) return MVIT_EINVAL;
+    bool split, small;
+    ns_plan(mats, count, k.split, split, small);
+    if (small) return ns_run_small(mats, count, k, split, st);
     for (int s = 0; s < count; s += NS_MAX) {
         NsLoadArgs l;
         NsGemmArgs g;
@@ -699,7 +1070,7 @@ static int ns_run(const mvit_ns_matrix* mats, int count, const NsCall& k, void* 
             g.n[i] = t.rows < t.cols ? t.cols : t.rows;
             g.out[i] = muon ? static_cast<void*>(t.w) : t.out;
             g.scale[i] = t.scale;
-            off += ns_region_units(t.rows, t.cols, k.split);
+            off += ns_region_units(t.rows, t.cols, split);
             blocks += tiles < NS_PARTS ? tiles : NS_PARTS;
         }
         l.blocks = (uint32_t)blocks;
@@ -716,7 +1087,7 @@ static int ns_run(const mvit_ns_matrix* mats, int count, const NsCall& k, void* 
         if (k.in_dtype == MVIT_F32) hipLaunchKernelGGL(ns_start_kernel<float>, dim3(l.blocks), dim3(256), 0, st, l);
         else hipLaunchKernelGGL(ns_start_kernel<bf16_t>, dim3(l.blocks), dim3(256), 0, st, l);
         MVIT_LAUNCH_CHECK();
-        const int rc = k.split ? ns_iterate<true>(g, k.steps, k.last, st) : ns_iterate<false>(g, k.steps, k.last, st);
+        const int rc = split ? ns_iterate<true>(g, k.steps, k.last, st) : ns_iterate<false>(g, k.steps, k.last, st);
         if (rc != MVIT_OK) return rc;
     }
     return MVIT_OK;
