@@ -753,10 +753,11 @@ __device__ __forceinline__ void ns_small_body(const NsSmallArgs& a, const NsSmal
             const char* p0 = start(trp, P, ldp, M0);
             const char* q0 = start(trq, Q, ldq, N0);
             const int pk = decltype(trp)::value ? 16 * ldp : 32, qk = decltype(trq)::value ? 16 * ldq : 32;      // bytes of 16 steps of k
-            for (int k = 0; k < K; k += 32) {           // K is a multiple of 32
-                h16x8 fp[2][PL], fq[2][PL];
+            auto chunk = [&](auto steps) {              // that many times 16 steps of k: all fragments requested, then the products
+                constexpr int S = decltype(steps)::value;
+                h16x8 fp[S][PL], fq[S][PL];
 #pragma unroll
-                for (int s = 0; s < 2; ++s) {
+                for (int s = 0; s < S; ++s) {
 #pragma unroll
                     for (int pl = 0; pl < PL; ++pl) {
                         fp[s][pl] = fetch(trp, p0 + pl * ppl, ldp);
@@ -766,14 +767,17 @@ __device__ __forceinline__ void ns_small_body(const NsSmallArgs& a, const NsSmal
                     q0 += qk;
                 }
 #pragma unroll
-                for (int s = 0; s < 2; ++s) {
+                for (int s = 0; s < S; ++s) {
                     if (SPLIT) {
                         acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(fp[s][PL - 1], fq[s][0], acc, 0, 0, 0);
                         acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(fp[s][0], fq[s][PL - 1], acc, 0, 0, 0);
                     }
                     acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(fp[s][0], fq[s][0], acc, 0, 0, 0);
                 }
-            }
+            };
+            int k = 0;                                  // K is a multiple of 32
+            for (; k + 64 <= K; k += 64) chunk(std::integral_constant<int, 4>{});
+            if (k < K) chunk(std::integral_constant<int, 2>{});
             return acc;
         };
 #pragma unroll
