@@ -79,7 +79,7 @@ class AxialRotary(object):
         xs, ps = self._arguments(x, positions, k, k_positions)
         if torch.is_grad_enabled() and any(t.requires_grad for t in xs):
             held = [_leaf_on_one_stream(t) for t in xs]
-            ys = _RotaryFn.apply(self, ps, *xs)
+            ys = _RotaryFn.apply(self, ps, False, *xs)
             del held                                # the graph holds the nodes now
         else:
             ys = self.turn(xs, ps)
@@ -190,20 +190,26 @@ def _leaf_on_one_stream(t):
 
 
 class _RotaryFn(torch.autograd.Function):
-    """The turn is orthogonal: the gradient is turned back by the same angles.  Nothing of the input is kept."""
+    """The turn is orthogonal: the gradient is turned back by the same angles (and a gradient's gradient forth again).  Nothing of the
+    input is kept."""
 
     @staticmethod
-    def forward(ctx, plan, ps, *xs):
-        ctx.plan = plan
-        ctx.grids = [p if isinstance(p, TokenGrid) else None for p in ps]
-        ctx.save_for_backward(*[p for p in ps if not isinstance(p, TokenGrid)])
-        ctx.n = len(xs)
-        return tuple(plan.turn(xs, ps))
+    def forward(ctx, plan, ps, inverse, *xs):
+        ctx.plan, ctx.inverse = plan, inverse
+        ctx.ps = ps
+        listed = [p for p in ps if not isinstance(p, TokenGrid)]
+        if listed:                      # (kept by autograd, which notices a change of theirs in between)
+            ctx.ps = [p if isinstance(p, TokenGrid) else None for p in ps]
+            ctx.save_for_backward(*listed)
+        return tuple(plan.turn(xs, ps, inverse=inverse))
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, *grads):
-        saved = iter(ctx.saved_tensors)
-        ps = [g if g is not None else next(saved) for g in ctx.grids]
+        ps = ctx.ps
+        if None in ps:
+            saved = iter(ctx.saved_tensors)
+            ps = [p if p is not None else next(saved) for p in ps]
         gs = [g if g.stride(3) == 1 else g.contiguous() for g in grads]
-        return (None, None) + tuple(ctx.plan.turn(gs, ps, inverse=True))
+        if torch.is_grad_enabled():     # create_graph
+            return (None, None, None) + _RotaryFn.apply(ctx.plan, ps, not ctx.inverse, *gs)
+        return (None, None, None) + tuple(ctx.plan.turn(gs, ps, inverse=not ctx.inverse))

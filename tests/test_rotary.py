@@ -123,6 +123,21 @@ def test_gradient_against_differences():
 
 
 @gpu
+def test_gradient_of_a_gradient():
+    rot, grid = AxialRotary(12, (4, 4, 4), base=50.0), TokenGrid((2, 1, 3))
+    x = randn((1, 1, 6, 12), torch.float32, 14).requires_grad_(True)
+    w = randn((1, 1, 6, 12), torch.float32, 15)
+    y = rot(x, grid)
+    (g,) = torch.autograd.grad((y * y * w).sum(), x, create_graph=True)        # g = R^T (2 w R x)
+    (gg,) = torch.autograd.grad((g * g).sum(), x)                              # 2 R^T (2 w R (R^T (2 w R x)))
+    forth = lambda t, s: oracle(t, grid, rot.sections, 50.0, "half", s)[0]  # noqa: E731
+    wd = w.double().cpu()
+    want = 2 * forth(2 * wd * forth(forth(2 * wd * forth(x, 1.0), -1.0), 1.0), -1.0)
+    # four turns and three products, each 6e-7 of the pair at most
+    assert (gg.double().cpu() - want).abs().max() <= 7 * 6e-7 * 2 * want.abs().max()
+
+
+@gpu
 def test_in_place_and_back_and_addend():
     rot, grid = AxialRotary(96), TokenGrid((2, 3, 3))
     buf = randn((2, 18, 5, 96), torch.bfloat16, 1)
