@@ -22,8 +22,6 @@
 typedef _Float16 h16;
 typedef __attribute__((ext_vector_type(8))) _Float16 h16x8;
 typedef __attribute__((ext_vector_type(4))) _Float16 h16x4;
-typedef __attribute__((address_space(1))) const void ns_gptr_t;
-typedef __attribute__((address_space(3))) void ns_lptr_t;
 typedef __attribute__((address_space(3))) bf16x4 ns_lds_b4;
 
 #define NS_MAX 72            // matrices per set of launches (kernel arguments hold their table)
@@ -239,8 +237,8 @@ __global__ __launch_bounds__(256) void ns_start_kernel(const NsLoadArgs a) {
 // D[M][N] = sum_k P(k, M) Q[N][k]:  A = X X^T (P = Q = X) and A A (P = Q = A) with both operands contiguous in k, only tiles on and above
 // the diagonal computed and each written twice;  X^T B^T = (B X)^T with P = X as it lies, k down its rows, read through the transposing LDS
 // read, so that X is kept in one order.
-// One workgroup = one T x T tile.  A group of four waves (2 x 2) takes K steps of 64 from two LDS stages of its own: a step's fragments
-// are read into registers, the next step's tile is requested (LDS-DMA), then the matrix instructions run while it flies.  With G groups the
+// One workgroup = one T x T tile.  A group of four waves (2 x 2) takes K steps of 64 from two LDS stages of its own: the next
+// step's tile is requested (LDS-DMA), then a step's fragments are read and its matrix instructions run while it flies.  With G groups the
 // steps are dealt in turn and the groups' sums added in order at the end: for launches of few tiles, whose time is the latency of a step
 // times their number.
 // LDS: k-contiguous tiles have rows of 128 bytes, 16-byte chunk c of row r at c ^ ((r >> 1) & 7): the 16 rows that a read serves together
@@ -254,6 +252,14 @@ enum { NS_GRAM = 0, NS_POLY = 1, NS_STEP = 2, NS_LAST16 = 3, NS_LAST32 = 4, NS_M
 __device__ __forceinline__ uint32_t ns_tile_of(uint32_t wg, uint32_t run) {
     const uint32_t xcd = wg & 7, slot = wg >> 3, r = slot / run;
     return (r * 8 + xcd) * run + (slot - r * run);
+}
+
+// 64 lanes x 16 bytes from base (wave-uniform) + offset to 1 KiB of LDS at dst (wave-uniform).  In asm because the compiler, which cannot tell
+// these writes from the reads of the other stage, would wait for them in front of every read; the kernel waits itself (vmcnt) before its
+// barriers.  (M0 cannot be named as overwritten; nothing else in the kernel uses it.)
+__device__ __forceinline__ void ns_dma(const h16* base, uint32_t offset, const char* dst) {
+    const uint32_t to = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(const __attribute__((address_space(3))) char*)dst);
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(offset), "s"(base) : "memory");
 }
 
 template <int T, int G, int PHASE, bool SPLIT>
@@ -307,7 +313,7 @@ __global__ __launch_bounds__(256 * G, G == 1 ? (SPLIT && T == 128 ? 1 : 2) : G) 
     const bool by_k = !SYM && !is_q;               // the tile of X as it lies
     const int ldk = PHASE == NS_GRAM || !SYM ? np : mp;      // row length of P
     const int ld_src = is_q && !SYM ? mp : ldk;
-    int src_off[PW];                               // element offset of this lane's 16 bytes from the operand's tile
+    uint32_t src_off[PW];                          // byte offset of this lane's 16 bytes from the operand's tile
 #pragma unroll
     for (int i = 0; i < PW; ++i) {
         const int piece = (wave & 1) * PW + i;
@@ -315,10 +321,10 @@ __global__ __launch_bounds__(256 * G, G == 1 ? (SPLIT && T == 128 ? 1 : 2) : G) 
             const int row = piece * (512 / T) + lane / (T / 8), slot = lane % (T / 8);
             const int ch = T == 128 ? slot ^ ((row & 3) << 2) : slot ^ (((row >> 1) & 1) << 2);
             const int col = min(m0 + ch * 8, np - 8);
-            src_off[i] = row * ld_src + col;
+            src_off[i] = 2u * (uint32_t)(row * ld_src + col);
         } else {
             const int row = piece * 8 + (lane >> 3), ch = (lane & 7) ^ ((row >> 1) & 7);
-            src_off[i] = min((is_q ? n0 : m0) + row, mp - 1) * ld_src + ch * 8;
+            src_off[i] = 2u * (uint32_t)(min((is_q ? n0 : m0) + row, mp - 1) * ld_src + ch * 8);
         }
     }
     const int64_t k_step = by_k ? (int64_t)NS_BK * ld_src : NS_BK;
@@ -332,8 +338,7 @@ __global__ __launch_bounds__(256 * G, G == 1 ? (SPLIT && T == 128 ? 1 : 2) : G) 
         for (int pl = 0; pl < PL; ++pl) {
             const h16* base = (pl ? src_lo : src_hi) + kt * k_step;
 #pragma unroll
-            for (int i = 0; i < PW; ++i)
-                __builtin_amdgcn_global_load_lds((ns_gptr_t*)(base + src_off[i]), (ns_lptr_t*)(dst + pl * T * 128 + 1024 * i), 16, 0, 0);
+            for (int i = 0; i < PW; ++i) ns_dma(base, src_off[i], dst + pl * T * 128 + 1024 * i);
         }
     };
 
@@ -351,8 +356,8 @@ __global__ __launch_bounds__(256 * G, G == 1 ? (SPLIT && T == 128 ? 1 : 2) : G) 
             const int piece = wave * PIECES + i;
             const int row = piece * (512 / T) + lane / (T / 8), slot = lane % (T / 8);
             const int ch = T == 128 ? slot ^ (row & 15) : slot ^ ((row >> 1) & 7);
-            const int64_t at = (int64_t)min(n0 + row, lim_n - 1) * lim_m + min(m0 + ch * 8, lim_m - 8);
-            __builtin_amdgcn_global_load_lds((ns_gptr_t*)(src + at), (ns_lptr_t*)(lds + stage * STAGE + 1024 * piece), 16, 0, 0);
+            const int at = min(n0 + row, lim_n - 1) * lim_m + min(m0 + ch * 8, lim_m - 8);
+            ns_dma(src, 2u * (uint32_t)at, lds + stage * STAGE + 1024 * piece);
         }
     };
     auto res_read = [=](int stage, int i, int j, int e4) {
@@ -374,6 +379,8 @@ __global__ __launch_bounds__(256 * G, G == 1 ? (SPLIT && T == 128 ? 1 : 2) : G) 
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __syncthreads();                            // the step's tile has landed; everyone has read the stage refilled below
         if (G > 1 && kt >= steps) continue;
+        if (kt + G < steps) dma(kt + G, (it + 1) & 1);
+        else if (RES && grp == 0) res_dma(res, (it + 1) & 1);
         h16x8 fp[PL][F][4], fq[PL][F][4];
 #pragma unroll
         for (int pl = 0; pl < PL; ++pl) {
@@ -395,8 +402,6 @@ __global__ __launch_bounds__(256 * G, G == 1 ? (SPLIT && T == 128 ? 1 : 2) : G) 
                     fq[pl][i][ks] = *reinterpret_cast<const h16x8*>(sq + rq * 128 + (((2 * ks + h) ^ ((rq >> 1) & 7)) * 16));
                 }
         }
-        if (kt + G < steps) dma(kt + G, (it + 1) & 1);
-        else if (RES && grp == 0) res_dma(res, (it + 1) & 1);
 #pragma unroll
         for (int ks = 0; ks < 4; ++ks)
 #pragma unroll
