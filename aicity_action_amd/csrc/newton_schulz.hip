@@ -121,44 +121,77 @@ __global__ __launch_bounds__(256) void ns_square_kernel(const NsLoadArgs a) {
     const bool bad = ns_bad(a.norm_coef);
     const T* u = static_cast<const T*>(t.u);
     double s = 0.0;
-    auto one = [&](float g, int64_t flat) {
-        float v = g;
-        if (t.mom) {
-            const float m = a.mu * t.mom[flat] + (1.0f - a.mu) * (g * coef);
-            if (!bad) t.mom[flat] = m;
-            v = ns_update(a, g, m, coef);
-        }
-        s += (double)v * (double)v;
-    };
     const int64_t total = (int64_t)t.rows * t.cols;
     const bool flat_ok = t.cs == 1 && (t.rs == t.cols || t.rows == 1);
     if (flat_ok && sizeof(T) == 4 && ((reinterpret_cast<uintptr_t>(u) | reinterpret_cast<uintptr_t>(t.mom)) & 15) == 0) {
         const float4* u4 = reinterpret_cast<const float4*>(u);
         float4* m4 = reinterpret_cast<float4*>(t.mom);
-        const int64_t n4 = total >> 2;
-        for (int64_t i = (int64_t)part * 256 + threadIdx.x; i < n4; i += (int64_t)nparts * 256) {
-            const float4 g = u4[i];
-            float4 v = g;
-            if (t.mom) {
-                float4 m = m4[i];
-                m.x = a.mu * m.x + (1.0f - a.mu) * (g.x * coef); m.y = a.mu * m.y + (1.0f - a.mu) * (g.y * coef);
-                m.z = a.mu * m.z + (1.0f - a.mu) * (g.z * coef); m.w = a.mu * m.w + (1.0f - a.mu) * (g.w * coef);
-                if (!bad) m4[i] = m;
-                v.x = ns_update(a, g.x, m.x, coef); v.y = ns_update(a, g.y, m.y, coef);
-                v.z = ns_update(a, g.z, m.z, coef); v.w = ns_update(a, g.w, m.w, coef);
+        const int64_t n4 = total >> 2, step = (int64_t)nparts * 256;
+        for (int64_t i0 = (int64_t)part * 256 + threadIdx.x; i0 < n4; i0 += 4 * step) {
+            float4 g[4], m[4];                              // (four quads in flight; the last of them read again where there are fewer)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const int64_t i = i0 + q * step < n4 ? i0 + q * step : n4 - 1;
+                g[q] = u4[i];
+                if (t.mom) m[q] = m4[i];
             }
-            s += ((double)v.x * v.x + (double)v.y * v.y) + ((double)v.z * v.z + (double)v.w * v.w);
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                if (i0 + q * step >= n4) break;
+                float4 v = g[q];
+                if (t.mom) {
+                    float4 p = m[q];
+                    p.x = a.mu * p.x + (1.0f - a.mu) * (v.x * coef); p.y = a.mu * p.y + (1.0f - a.mu) * (v.y * coef);
+                    p.z = a.mu * p.z + (1.0f - a.mu) * (v.z * coef); p.w = a.mu * p.w + (1.0f - a.mu) * (v.w * coef);
+                    if (!bad) m4[i0 + q * step] = p;
+                    v.x = ns_update(a, v.x, p.x, coef); v.y = ns_update(a, v.y, p.y, coef);
+                    v.z = ns_update(a, v.z, p.z, coef); v.w = ns_update(a, v.w, p.w, coef);
+                }
+                s += ((double)v.x * v.x + (double)v.y * v.y) + ((double)v.z * v.z + (double)v.w * v.w);
+            }
         }
-        if (part == 0)
-            for (int64_t i = 4 * n4 + threadIdx.x; i < total; i += 256) one(ns_ld(u + i), i);
+        if (part == 0 && 4 * n4 + threadIdx.x < total) {     // at most three elements are left
+            const int64_t i = 4 * n4 + threadIdx.x;
+            float v = ns_ld(u + i);
+            if (t.mom) {
+                const float p = a.mu * t.mom[i] + (1.0f - a.mu) * (v * coef);
+                if (!bad) t.mom[i] = p;
+                v = ns_update(a, v, p, coef);
+            }
+            s += (double)v * (double)v;
+        }
     } else {
-        // neighbouring threads take neighbouring elements of u's own order
+        // neighbouring threads take neighbouring elements of u's own order, eight each in flight
         const bool by_col = t.cs == 1 || t.rs != 1;
-        const int64_t inner = by_col ? t.cols : t.rows;
-        for (int64_t i = (int64_t)part * 256 + threadIdx.x; i < total; i += (int64_t)nparts * 256) {
-            const int64_t o = i / inner, in = i - o * inner;
-            const int64_t r = by_col ? o : in, c = by_col ? in : o;
-            one(ns_ld(u + r * t.rs + c * t.cs), r * t.cols + c);
+        const int64_t inner = by_col ? t.cols : t.rows, step = (int64_t)nparts * 256;
+        for (int64_t i0 = (int64_t)part * 256 + threadIdx.x; i0 < total; i0 += 8 * step) {
+            float g[8], m[8];
+            int64_t at[8];
+#pragma unroll
+            for (int q = 0; q < 8; ++q) {
+                const int64_t i = i0 + q * step < total ? i0 + q * step : total - 1;
+                if (flat_ok) {
+                    at[q] = i;
+                    g[q] = ns_ld(u + i);
+                } else {
+                    const int64_t o = i / inner, in = i - o * inner;
+                    const int64_t r = by_col ? o : in, c = by_col ? in : o;
+                    at[q] = r * t.cols + c;
+                    g[q] = ns_ld(u + r * t.rs + c * t.cs);
+                }
+                if (t.mom) m[q] = t.mom[at[q]];
+            }
+#pragma unroll
+            for (int q = 0; q < 8; ++q) {
+                if (i0 + q * step >= total) break;
+                float v = g[q];
+                if (t.mom) {
+                    const float p = a.mu * m[q] + (1.0f - a.mu) * (v * coef);
+                    if (!bad) t.mom[at[q]] = p;
+                    v = ns_update(a, v, p, coef);
+                }
+                s += (double)v * (double)v;
+            }
         }
     }
     __shared__ double red[4];
@@ -200,17 +233,46 @@ __global__ __launch_bounds__(256) void ns_start_kernel(const NsLoadArgs a) {
     const T* u = static_cast<const T*>(t.u);
     const int r0 = (tall ? tj : ti) * 64, c0 = (tall ? ti : tj) * 64;   // the tile in U
     const bool by_col = t.cs == 1 || t.rs != 1;
-#pragma unroll 4
-    for (int k = 0; k < 16; ++k) {
-        const int e = k * 256 + tid;
-        const int lr = by_col ? e >> 6 : e & 63, lc = by_col ? e & 63 : e >> 6;
-        const int r = r0 + lr, c = c0 + lc;
-        float v = 0.f;
-        if (r < t.rows && c < t.cols) {
-            v = ns_ld(u + (int64_t)r * t.rs + (int64_t)c * t.cs);
-            if (t.mom) v = ns_update(a, v, t.mom[(int64_t)r * t.cols + c], coef);
+    // every load is issued before the first is used, at clamped places
+    const bool quads = sizeof(T) == 4 && t.cs == 1 && (t.rs & 3) == 0 && (t.cols & 3) == 0 &&
+                       ((reinterpret_cast<uintptr_t>(u) | reinterpret_cast<uintptr_t>(t.mom)) & 15) == 0;
+    if (quads) {
+        float4 gv[4], mv[4];
+        const int lc = (tid & 15) * 4, c = min(c0 + lc, t.cols - 4);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int r = min(r0 + (tid >> 4) + 16 * k, t.rows - 1);
+            gv[k] = load4(u + (int64_t)r * t.rs + c);
+            if (t.mom) mv[k] = load4(t.mom + (int64_t)r * t.cols + c);
         }
-        sh[lr][lc] = v;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int lr = (tid >> 4) + 16 * k;
+            float v[4] = {gv[k].x, gv[k].y, gv[k].z, gv[k].w};
+            if (t.mom) {
+                const float mm[4] = {mv[k].x, mv[k].y, mv[k].z, mv[k].w};
+#pragma unroll
+                for (int j = 0; j < 4; ++j) v[j] = ns_update(a, v[j], mm[j], coef);
+            }
+            const bool in = r0 + lr < t.rows && c0 + lc < t.cols;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) sh[lr][lc + j] = in ? v[j] : 0.f;
+        }
+    } else {
+        float gv[16], mv[16];
+#pragma unroll
+        for (int k = 0; k < 16; ++k) {
+            const int e = k * 256 + tid, lr = by_col ? e >> 6 : e & 63, lc = by_col ? e & 63 : e >> 6;
+            const int r = min(r0 + lr, t.rows - 1), c = min(c0 + lc, t.cols - 1);
+            gv[k] = ns_ld(u + (int64_t)r * t.rs + (int64_t)c * t.cs);
+            if (t.mom) mv[k] = t.mom[(int64_t)r * t.cols + c];
+        }
+#pragma unroll
+        for (int k = 0; k < 16; ++k) {
+            const int e = k * 256 + tid, lr = by_col ? e >> 6 : e & 63, lc = by_col ? e & 63 : e >> 6;
+            const float v = t.mom ? ns_update(a, gv[k], mv[k], coef) : gv[k];
+            sh[lr][lc] = r0 + lr < t.rows && c0 + lc < t.cols ? v : 0.f;
+        }
     }
     __syncthreads();
     const float f = s_inv * NS_S;
@@ -344,6 +406,19 @@ __global__ __launch_bounds__(256 * G, G == 1 ? (SPLIT && T == 128 ? 1 : 2) : G) 
 
     if (grp < steps) dma(grp, 0);
 
+    // the last iteration's result: its rows and columns; a weight's tile is requested here, to fly under the whole sum
+    constexpr int QUADS = T * T / 4 / (256 * G);
+    const bool tall = LAST && a.tall[id];
+    const int R = tall ? n : m, C = tall ? m : n, row0 = tall ? m0 : n0, col0 = tall ? n0 : m0;
+    const bool quads = LAST && (C & 3) == 0 && (reinterpret_cast<uintptr_t>(a.out[id]) & (PHASE == NS_LAST16 ? 7 : 15)) == 0;
+    float4 w[PHASE == NS_MUON ? QUADS : 1];
+    if (PHASE == NS_MUON && quads)
+#pragma unroll
+        for (int i = 0; i < QUADS; ++i) {
+            const int k = tid + 256 * G * i, row = k / (T / 4), c4 = (k - row * (T / 4)) * 4;
+            w[PHASE == NS_MUON ? i : 0] = load4(static_cast<const float*>(a.out[id]) + (int64_t)min(row0 + row, R - 1) * C + min(col0 + c4, C - 4));
+        }
+
     // What is added to the product -- a X or b A -- comes through LDS too, in whole rows: the tile's high half flies under the last step's
     // matrix instructions, its low half follows.  16-byte chunk c of row r lies at c ^ (r & 15) (T = 128) or c ^ ((r >> 1) & 7) (T = 64)
     constexpr bool RES = PHASE != NS_GRAM, RES_LO = RES && (PHASE != NS_POLY || SPLIT);
@@ -461,8 +536,6 @@ __global__ __launch_bounds__(256 * G, G == 1 ? (SPLIT && T == 128 ? 1 : 2) : G) 
 
     if (LAST) {       // the result's rows through LDS in single precision
         constexpr int ROWB = T * 4 + 16;
-        const bool tall = a.tall[id];
-        const int R = tall ? n : m, C = tall ? m : n, row0 = tall ? m0 : n0, col0 = tall ? n0 : m0;
         if (PHASE == NS_MUON && ns_bad(a.norm_coef)) return;
         __syncthreads();
         if (grp == 0)
@@ -483,22 +556,19 @@ __global__ __launch_bounds__(256 * G, G == 1 ? (SPLIT && T == 128 ? 1 : 2) : G) 
         __syncthreads();
         const float lr = a.hyper ? a.hyper[0] : a.lr;
         const float keep = 1.0f - lr * a.wd, step = lr * a.scale[id];
-        const bool quads = (C & 3) == 0 && (reinterpret_cast<uintptr_t>(a.out[id]) & (PHASE == NS_LAST16 ? 7 : 15)) == 0;
         if (quads) {
-#pragma unroll 4
-            for (int k = tid; k < T * T / 4; k += 256 * G) {
-                const int row = k / (T / 4), c4 = (k - row * (T / 4)) * 4;
+#pragma unroll
+            for (int i = 0; i < QUADS; ++i) {
+                const int k = tid + 256 * G * i, row = k / (T / 4), c4 = (k - row * (T / 4)) * 4;
                 if (row0 + row >= R || col0 + c4 >= C) continue;
                 const float4 v = *reinterpret_cast<const float4*>(smem + row * ROWB + c4 * 4);
                 const int64_t at = (int64_t)(row0 + row) * C + col0 + c4;
                 if (PHASE == NS_LAST16) store4(static_cast<bf16_t*>(a.out[id]) + at, v);
                 else if (PHASE == NS_LAST32) store4(static_cast<float*>(a.out[id]) + at, v);
                 else {
-                    float4* w = reinterpret_cast<float4*>(static_cast<float*>(a.out[id]) + at);
-                    float4 x = *w;
-                    x.x = x.x * keep - step * v.x; x.y = x.y * keep - step * v.y;
-                    x.z = x.z * keep - step * v.z; x.w = x.w * keep - step * v.w;
-                    *w = x;
+                    const float4 x = w[PHASE == NS_MUON ? i : 0];
+                    store4(static_cast<float*>(a.out[id]) + at,
+                           make_float4(x.x * keep - step * v.x, x.y * keep - step * v.y, x.z * keep - step * v.z, x.w * keep - step * v.w));
                 }
             }
         } else {
@@ -511,8 +581,8 @@ __global__ __launch_bounds__(256 * G, G == 1 ? (SPLIT && T == 128 ? 1 : 2) : G) 
                 if (PHASE == NS_LAST16) static_cast<bf16_t*>(a.out[id])[at] = f32_to_bf16(v);
                 else if (PHASE == NS_LAST32) static_cast<float*>(a.out[id])[at] = v;
                 else {
-                    float* w = static_cast<float*>(a.out[id]) + at;
-                    *w = *w * keep - step * v;
+                    float* p = static_cast<float*>(a.out[id]) + at;
+                    *p = *p * keep - step * v;
                 }
             }
         }
