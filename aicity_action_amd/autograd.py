@@ -326,7 +326,7 @@ class _BlockFn(torch.autograd.Function):
         q_plain = q
         if rot is not None:       # HIP.ROTARY: q and k turn by their places; the residual keeps the pooled query as it is
             plan, *grids = rot[g.index]
-            q, k = plan.turn([q, k], grids, outs=None if addq else [q, k])
+            q, k = plan.turn([q, k], grids, outs=[torch.empty_like(q) if addq else q, k])
         _hip.check(_hip.attention_fwd(L, q, k, v, o, lse, B, h, Lq, Lk, 96 ** -0.5, addq if rot is None else 0, act, _st()), "attention")
         o_att = o                 # what the attention backward reads (the kernels' own residual is taken out there)
         if rot is not None and addq:

@@ -579,7 +579,7 @@ class MViT(nn.Module):
         q_plain = q
         if self.rotary is not None:      # q and k turn by their places; the residual keeps the pooled query as it is
             plan, *grids = self.rotary[g.index]
-            q, k = plan.turn([q, k], grids, outs=None if addq else [q, k])
+            q, k = plan.turn([q, k], grids, outs=[torch.empty_like(q) if addq else q, k])
         # 4. fused attention (+ pooled-q residual), heads merged on store   attention.py:267-279
         if "attention" in ex:
             o = torch.empty(B * Lq, Cout, dtype=torch.float32, device=dev)

@@ -147,6 +147,8 @@ class MuonMatrices(object):
         for p, m, g in zip(self.params, self.momenta, grads):
             if g is None:
                 continue
+            if p.dtype != torch.float32 or p.device != device or not (p.is_contiguous() and m.is_contiguous()) or m.shape != p.shape:
+                raise ValueError("MuonMatrices.step: a parameter or its momentum has changed its type, device, shape or strides")
             if g.shape != p.shape or g.dtype != torch.float32 or g.device != device:
                 raise ValueError("MuonMatrices.step: a %s gradient of shape %s on %s for a float32 parameter of shape %s on %s"
                                  % (g.dtype, tuple(g.shape), g.device, tuple(p.shape), device))
@@ -155,6 +157,8 @@ class MuonMatrices(object):
             touched += [p, m]
         if not rows:
             return
+        if {r[0] for r in rows} & {x for r in rows for x in r[1:3]}:
+            raise ValueError("MuonMatrices.step: a gradient shares its memory with a parameter or a momentum")
         if not self.params[0].is_cuda:
             raise RuntimeError("MuonMatrices needs its parameters on a gfx950 device; there is no CPU fallback")
         rec = np.array(rows, dtype=_REC)

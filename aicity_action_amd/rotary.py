@@ -97,6 +97,8 @@ class AxialRotary(object):
         if k is not None and x.numel() and x.data_ptr() == k.data_ptr():
             raise ValueError("AxialRotary.rotate_: x and k are the same memory; they must not overlap")
         self.turn(xs, ps, outs=xs, inverse=inverse)
+        for t in xs:                    # written behind torch's back
+            torch.autograd.graph.increment_version(t)
         return tuple(xs) if k is not None else x
 
     # ---- checks ----------------------------------------------------------------------------------------------------------------------
@@ -127,6 +129,8 @@ class AxialRotary(object):
             want = (t.shape[2], len(self.sections))
             if tuple(p.shape) != want and tuple(p.shape) not in ((t.shape[0],) + want, (1,) + want):
                 raise ValueError("AxialRotary: positions must be [%d, %d] or [%d, %d, %d], got %s" % (want + (t.shape[0],) + want + (tuple(p.shape),)))
+            if p.requires_grad:
+                raise ValueError("AxialRotary: positions carry no gradient; detach them")
             if p.device != t.device:
                 raise ValueError("AxialRotary: positions on %s, the tensor on %s" % (p.device, t.device))
         else:
@@ -147,6 +151,7 @@ class AxialRotary(object):
 def add_(out, add):
     """out += add for two [batch, heads, tokens, channels] views of any strides with contiguous channels: the rotary kernel with no axis."""
     _launch([out], [out], [add], [None], out.shape[3], 0, None, None, 0, False)
+    torch.autograd.graph.increment_version(out)
     return out
 
 

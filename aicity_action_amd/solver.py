@@ -128,7 +128,7 @@ class HipAdamW(object):
         # all-reduce, so the global norm and the clip coefficient are the same everywhere), the AdamW kernel only the first _n_upd
         self._n_upd = len(rec)
         rec = rec + rec_other
-        dev = self.groups[0]["params"][0].device
+        dev = next(p for grp in self.groups for p in grp["params"]).device
         assert _hip.lib().mvit_mt_chunk_bytes() == _DT.itemsize
         host = np.array(rec, dtype=_DT).view(np.uint8)
         # With set_to_none the gradient addresses change every step, so this runs every step: the table goes up through a small

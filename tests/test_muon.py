@@ -116,6 +116,17 @@ def test_strides_batches_and_lists():
 
 
 @gpu
+def test_rows_far_apart():
+    """Offsets past 32 bits within one update, in one workgroup's matrix and in one of many tiles."""
+    buf = torch.empty(2 ** 30 + 8192, device=DEV)
+    for rows, cols, far in ((2, 300, 2 ** 30 + 8), (5, 40, 2 ** 28), (200, 150, 5 * 2 ** 20)):
+        v = buf.as_strided((rows, cols), (far, 1))
+        v.copy_(gradient(rows, cols, rows))
+        near(orthogonalize(v, dtype=torch.float32), v.clone(), True)
+        near(orthogonalize(v.t(), dtype=torch.float32), v.t().clone(), True)
+
+
+@gpu
 @pytest.mark.parametrize("shape", [(2048, 4096), (4160, 2112)])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 def test_large_matrices(shape, dtype):
@@ -139,6 +150,9 @@ def test_degenerate_values():
     outs = orthogonalize([u, zero, nan, u], dtype=torch.bfloat16)
     assert torch.equal(outs[1], zero.bfloat16()) and torch.equal(outs[0], outs[3]) and torch.isnan(outs[2].float()).all()
     near(outs[0], u, False)
+    inf = u.clone()
+    inf[0, 0] = math.inf
+    assert torch.isnan(orthogonalize(inf).float()).all()
     same = torch.ones(40, 60, device=DEV)       # rank one
     near(orthogonalize(same, dtype=torch.float32), same, True)
 
@@ -289,9 +303,18 @@ def test_refusals():
     for grads in ([], [u.half()], [u.t()]):
         with pytest.raises(ValueError):
             plan.step(grads, lr=0.1)
+    g = torch.zeros(4, 6)
     for kw in (dict(norm_coef=torch.zeros(1)), dict(norm_coef=torch.zeros(2).double())):
         with pytest.raises(ValueError, match="norm_coef"):
-            plan.step([u], lr=0.1, **kw)
+            plan.step([g], lr=0.1, **kw)
+    for own in (u, plan.momenta[0]):
+        with pytest.raises(ValueError, match="shares its memory"):
+            plan.step([own], lr=0.1)
+    moved = torch.zeros(4, 6)
+    other = MuonMatrices([moved])
+    moved.data = torch.zeros(6, 4).t()
+    with pytest.raises(ValueError, match="changed its"):
+        other.step([torch.zeros(4, 6)], lr=0.1)
     plan.step([None], lr=0.1)
     with pytest.raises(RuntimeError, match="no CPU fallback"):
-        plan.step([u], lr=0.1)
+        plan.step([g], lr=0.1)

@@ -210,6 +210,21 @@ def test_muon_checkpoint_resume_and_non_finite_steps(tmp_path):
 
 
 @gpu
+def test_muon_with_frozen_parts():
+    """Only the matrices, or only the others, receive gradients."""
+    for frozen in (lambda n, p: not (n.startswith("blocks.") and p.ndim == 2), lambda n, p: n.startswith("blocks.") and p.ndim == 2):
+        cfg, meta, model, clip, labels = model_and_batch("tiny_even", "fp32")
+        for n, p in model.named_parameters():
+            p.requires_grad_(not frozen(n, p))
+        opt = construct_optimizer(model.train(), cfg)
+        before = {n: p.detach().clone() for n, p in model.named_parameters()}
+        one_backward(model, clip, labels)
+        opt.step()
+        for n, p in model.named_parameters():
+            assert torch.equal(p, before[n]) == (frozen(n, p) or p.grad is None or not p.grad.any()), n
+
+
+@gpu
 def test_graphed_muon_rotary_step_reproduces_the_eager_step():
     """The whole step captured in a graph and replayed (graph_step.GraphedTrainStep) against the eager loop, bit for bit."""
     from aicity_action_amd.graph_step import GraphedTrainStep

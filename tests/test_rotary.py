@@ -264,5 +264,10 @@ def test_refusals_on_the_device():
         rot.rotate_(x.clone().requires_grad_(True), grid)
     with pytest.raises(ValueError, match="expanded"):
         rot.rotate_(x[:1].expand(3, 1, 8, 96), grid)
+    with pytest.raises(ValueError, match="no gradient"):
+        rot(x, torch.zeros(8, 3, device=DEV, requires_grad=True))
+    version = x._version
+    rot.rotate_(x, grid)
+    assert x._version > version
     with pytest.raises(ValueError, match="same memory"):
         rot.rotate_(x, grid, x, grid)
