@@ -330,8 +330,8 @@ class _BlockFn(torch.autograd.Function):
         _hip.check(_hip.attention_fwd(L, q, k, v, o, lse, B, h, Lq, Lk, 96 ** -0.5, addq if rot is None else 0, act, _st()), "attention")
         o_att = o                 # what the attention backward reads (the kernels' own residual is taken out there)
         if rot is not None and addq:
-            o = o_att.clone()
-            add_(o.view(B, Lq, h, 96).transpose(1, 2), q_plain)
+            o = torch.empty_like(o_att)
+            add_(o.view(B, Lq, h, 96).transpose(1, 2), q_plain, x=o_att.view(B, Lq, h, 96).transpose(1, 2))
         del q_plain
         r = x2
         r_full = None

@@ -148,9 +148,10 @@ class AxialRotary(object):
         return list(outs)
 
 
-def add_(out, add):
-    """out += add for two [batch, heads, tokens, channels] views of any strides with contiguous channels: the rotary kernel with no axis."""
-    _launch([out], [out], [add], [None], out.shape[3], 0, None, None, 0, False)
+def add_(out, add, x=None):
+    """out = (x or out) + add for [batch, heads, tokens, channels] views of any strides with contiguous channels: the rotary kernel with no
+    axis."""
+    _launch([out if x is None else x], [out], [add], [None], out.shape[3], 0, None, None, 0, False)
     torch.autograd.graph.increment_version(out)
     return out
 

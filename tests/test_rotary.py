@@ -154,6 +154,9 @@ def test_in_place_and_back_and_addend():
     out = a.clone()
     add_(out, want)
     assert torch.equal(out, (a.float() + want.float()).to(torch.bfloat16))
+    other = torch.empty_like(a)
+    add_(other, want, x=a)
+    assert torch.equal(other, out)
 
 
 @gpu
