@@ -72,6 +72,9 @@ class AxialRotary(object):
         self._turns = (ctypes.c_double * len(turns))(*turns)
         self._sections = (ctypes.c_int * len(self.sections))(*self.sections)
 
+    def __reduce__(self):                       # (models that hold a plan are copied and pickled)
+        return AxialRotary, (self.head_dim, self.sections, self.base, self.layout)
+
     def __call__(self, x, positions, k=None, k_positions=None):
         """Turned copies of ``x`` (and ``k``), differentiable.  Tensors [batch, heads, tokens, head_dim], float32 / bfloat16 / float16, any
         strides with contiguous channels (a token-major buffer goes in as its transposed view).  Positions: a TokenGrid, or a tensor

@@ -1,5 +1,7 @@
 """Rotary positions (aicity_action_amd/rotary.py) against the definition in 64 bits, and its refusals (those run on the CPU)."""
+import copy
 import math
+import pickle
 
 import pytest
 import torch
@@ -227,6 +229,13 @@ def test_capture_beside_a_living_eager_graph_is_refused(monkeypatch):
     y = x * 3 if rotary._leaf_on_one_stream(x) is not None else None
     assert rotary._leaf_on_one_stream(x) is not None
     assert rotary._leaf_on_one_stream(x * 2) is None and rotary._leaf_on_one_stream(torch.zeros(1)) is None
+
+
+def test_a_plan_is_copied_and_pickled():
+    plan = AxialRotary(40, (8, 12, 20), base=77.0, layout="interleaved")
+    for other in (copy.deepcopy(plan), pickle.loads(pickle.dumps(plan))):
+        assert (other.head_dim, other.sections, other.base, other.layout) == (plan.head_dim, plan.sections, plan.base, plan.layout)
+        assert list(other._turns) == list(plan._turns) and list(other._sections) == list(plan._sections)
 
 
 def test_refusals():
