@@ -299,10 +299,9 @@ __global__ __launch_bounds__(256) void ns_start_kernel(const NsLoadArgs a) {
 // D[M][N] = sum_k P(k, M) Q[N][k]:  A = X X^T (P = Q = X) and A A (P = Q = A) with both operands contiguous in k, only tiles on and above
 // the diagonal computed and each written twice;  X^T B^T = (B X)^T with P = X as it lies, k down its rows, read through the transposing LDS
 // read, so that X is kept in one order.
-// One workgroup = one T x T tile.  A group of four waves (2 x 2) takes K steps of 64 from two LDS stages of its own: the next
-// step's tile is requested (LDS-DMA), then a step's fragments are read and its matrix instructions run while it flies.  With G groups the
-// steps are dealt in turn and the groups' sums added in order at the end: for launches of few tiles, whose time is the latency of a step
-// times their number.
+// One workgroup = one T x T tile.  A group of four waves (2 x 2) takes K steps of 64 from a ring of D LDS stages of its own: the tile D - 1
+// steps ahead is requested (LDS-DMA), then a step's fragments are read and its matrix instructions run while those ahead fly.  With G groups the
+// steps are dealt in turn and the groups' sums added in order at the end.
 // LDS: k-contiguous tiles have rows of 128 bytes, 16-byte chunk c of row r at c ^ ((r >> 1) & 7): the 16 rows that a read serves together
 // fall on 16 different slots of the 256-byte bank period.  X tiles as they lie have rows of 2 T bytes (a k each), 64-byte unit u of row r at
 // u ^ (r & 3) (T = 128) or u ^ ((r >> 1) & 1) (T = 64): the four rows of a transposing read fall on different banks.
@@ -324,14 +323,22 @@ __device__ __forceinline__ void ns_dma(const h16* base, uint32_t offset, const c
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(offset), "s"(base) : "memory");
 }
 
-template <int T, int G, int PHASE, bool SPLIT>
+template <int T, int G, int D, int PHASE, bool SPLIT>
 constexpr int ns_lds_bytes() {
-    const int stages = G * 2 * (SPLIT ? 4 : 2) * T * 128;           // (the groups' sums lie within: behind the first group's stages)
+    const int stages = G * D * (SPLIT ? 4 : 2) * T * 128;           // (the groups' sums lie within: behind the first group's stages)
     const int out = PHASE >= NS_LAST16 ? T * (T * 4 + 16) : 2 * T * (T * 2 + 16);
     return stages > out ? stages : out;
 }
 
-template <int T, int G, int PHASE, bool SPLIT>
+// waits until at most n stages of PER requests each are still on their way
+template <int PER, int MOST>
+__device__ __forceinline__ void ns_wait_stages(int n) {
+    if constexpr (MOST == 0) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    else if (n >= MOST) asm volatile("s_waitcnt vmcnt(%0)" ::"i"(PER * MOST) : "memory");
+    else ns_wait_stages<PER, MOST - 1>(n);
+}
+
+template <int T, int G, int D, int PHASE, bool SPLIT>
 __global__ __launch_bounds__(256 * G, G == 1 ? (SPLIT && T == 128 ? 1 : 2) : G) void ns_gemm_kernel(const NsGemmArgs a) {
     constexpr int F = T / 64;                      // 32 x 32 accumulators per wave and direction
     constexpr int PL = SPLIT ? 2 : 1;              // planes of an operand: high halves, low halves
@@ -366,7 +373,7 @@ __global__ __launch_bounds__(256 * G, G == 1 ? (SPLIT && T == 128 ? 1 : 2) : G) 
     const int tid = threadIdx.x, grp = __builtin_amdgcn_readfirstlane(tid >> 8), wave = __builtin_amdgcn_readfirstlane((tid >> 6) & 3);
     const int lane = tid & 63, r = lane & 31, h = lane >> 5;
     const int wm = (wave & 1) * (T / 2), wn = (wave >> 1) * (T / 2);
-    char* const lds = smem + grp * 2 * STAGE;
+    char* const lds = smem + grp * D * STAGE;
 
     // LDS-DMA: a wave instruction brings 1 KiB; waves 0 and 1 move P, waves 2 and 3 Q, T/16 pieces each.  Rows or columns past the padded
     // matrix are read again from its last ones; what comes of them is never stored
@@ -390,8 +397,8 @@ __global__ __launch_bounds__(256 * G, G == 1 ? (SPLIT && T == 128 ? 1 : 2) : G) 
         }
     }
     const int64_t k_step = by_k ? (int64_t)NS_BK * ld_src : NS_BK;
-    const int nk = (PHASE == NS_GRAM ? np : mp) / NS_BK;
-    const int steps = nk;
+    const int steps = (PHASE == NS_GRAM ? np : mp) / NS_BK;
+    const int rounds = (steps + G - 1) / G, mine = (steps - grp + G - 1) / G;      // group 0 takes one in every round
     const h16* const src_hi = PHASE == NS_GRAM ? g.x(a.cur) : PHASE == NS_POLY ? g.a() : is_q ? g.b() : g.x(a.cur);
     const h16* const src_lo = PHASE == NS_GRAM ? g.xlo(a.cur) : PHASE == NS_POLY ? g.alo() : is_q ? g.blo() : g.xlo(a.cur);
     auto dma = [=](int kt, int stage) {
@@ -404,23 +411,8 @@ __global__ __launch_bounds__(256 * G, G == 1 ? (SPLIT && T == 128 ? 1 : 2) : G) 
         }
     };
 
-    if (grp < steps) dma(grp, 0);
-
-    // the last iteration's result: its rows and columns; a weight's tile is requested here, to fly under the whole sum
-    constexpr int QUADS = T * T / 4 / (256 * G);
-    const bool tall = LAST && a.tall[id];
-    const int R = tall ? n : m, C = tall ? m : n, row0 = tall ? m0 : n0, col0 = tall ? n0 : m0;
-    const bool quads = LAST && (C & 3) == 0 && (reinterpret_cast<uintptr_t>(a.out[id]) & (PHASE == NS_LAST16 ? 7 : 15)) == 0;
-    float4 w[PHASE == NS_MUON ? QUADS : 1];
-    if (PHASE == NS_MUON && quads)
-#pragma unroll
-        for (int i = 0; i < QUADS; ++i) {
-            const int k = tid + 256 * G * i, row = k / (T / 4), c4 = (k - row * (T / 4)) * 4;
-            w[PHASE == NS_MUON ? i : 0] = load4(static_cast<const float*>(a.out[id]) + (int64_t)min(row0 + row, R - 1) * C + min(col0 + c4, C - 4));
-        }
-
-    // What is added to the product -- a X or b A -- comes through LDS too, in whole rows: the tile's high half flies under the last step's
-    // matrix instructions, its low half follows.  16-byte chunk c of row r lies at c ^ (r & 15) (T = 128) or c ^ ((r >> 1) & 7) (T = 64)
+    // What is added to the product -- a X or b A -- comes through LDS too, in whole rows: the tile's halves are requested behind the last
+    // step's tile (with two stages the low half follows when the sum is done).  16-byte chunk c of row r lies at c ^ (r & 15) (T = 128) or c ^ ((r >> 1) & 7) (T = 64)
     constexpr bool RES = PHASE != NS_GRAM, RES_LO = RES && (PHASE != NS_POLY || SPLIT);
     const h16* const res = PHASE == NS_POLY ? g.a() : g.x(a.cur);
     const h16* const reslo = PHASE == NS_POLY ? g.alo() : g.xlo(SPLIT ? a.cur : 0);
@@ -435,6 +427,30 @@ __global__ __launch_bounds__(256 * G, G == 1 ? (SPLIT && T == 128 ? 1 : 2) : G) 
             ns_dma(src, 2u * (uint32_t)at, lds + stage * STAGE + 1024 * piece);
         }
     };
+    // a group's s-th request: its s-th step's tile, or behind the last one the residual's high half and low half
+    auto request = [=](int s, int slot) {
+        if (s < mine) dma(grp + s * G, slot);
+        else if (RES && grp == 0) {
+            if (s == mine) res_dma(res, slot);
+            else if (RES_LO && D > 2 && s == mine + 1) res_dma(reslo, slot);
+        }
+    };
+#pragma unroll
+    for (int s = 0; s < D - 1; ++s) request(s, s);
+
+    // the last iteration's result: its rows and columns; a weight's tile is requested here, to fly under the whole sum
+    constexpr int QUADS = T * T / 4 / (256 * G);
+    const bool tall = LAST && a.tall[id];
+    const int R = tall ? n : m, C = tall ? m : n, row0 = tall ? m0 : n0, col0 = tall ? n0 : m0;
+    const bool quads = LAST && (C & 3) == 0 && (reinterpret_cast<uintptr_t>(a.out[id]) & (PHASE == NS_LAST16 ? 7 : 15)) == 0;
+    float4 w[PHASE == NS_MUON ? QUADS : 1];
+    if (PHASE == NS_MUON && quads)
+#pragma unroll
+        for (int i = 0; i < QUADS; ++i) {
+            const int k = tid + 256 * G * i, row = k / (T / 4), c4 = (k - row * (T / 4)) * 4;
+            w[PHASE == NS_MUON ? i : 0] = load4(static_cast<const float*>(a.out[id]) + (int64_t)min(row0 + row, R - 1) * C + min(col0 + c4, C - 4));
+        }
+
     auto res_read = [=](int stage, int i, int j, int e4) {
         const int M = wm + 32 * i + 8 * e4 + 4 * h, N = wn + 32 * j + r;
         const int ch = T == 128 ? (M >> 3) ^ (N & 15) : (M >> 3) ^ ((N >> 1) & 7);
@@ -450,16 +466,15 @@ __global__ __launch_bounds__(256 * G, G == 1 ? (SPLIT && T == 128 ? 1 : 2) : G) 
 
     const int q4 = (lane & 15) >> 2;               // transposing read: this lane names four columns of row 8 h + q4 (+ 4)
     const int tr_row = 8 * h + q4, tr_col = (16 * ((lane >> 4) & 1) + 4 * (lane & 3)) * 2;
-    for (int kt = grp, it = 0; it * G < steps; kt += G, ++it) {
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    for (int it = 0, slot = 0, free = D - 1; it < rounds; ++it) {
+        ns_wait_stages<PW * PL, D - 2>(mine - 1 - it);
         __syncthreads();                            // the step's tile has landed; everyone has read the stage refilled below
-        if (G > 1 && kt >= steps) continue;
-        if (kt + G < steps) dma(kt + G, (it + 1) & 1);
-        else if (RES && grp == 0) res_dma(res, (it + 1) & 1);
+        if (G > 1 && it >= mine) continue;
+        request(it + D - 1, free);
         h16x8 fp[PL][F][4], fq[PL][F][4];
 #pragma unroll
         for (int pl = 0; pl < PL; ++pl) {
-            const char* sp = lds + (it & 1) * STAGE + pl * T * 128;
+            const char* sp = lds + slot * STAGE + pl * T * 128;
             const char* sq = sp + PL * T * 128;
 #pragma unroll
             for (int ks = 0; ks < 4; ++ks)
@@ -489,13 +504,15 @@ __global__ __launch_bounds__(256 * G, G == 1 ? (SPLIT && T == 128 ? 1 : 2) : G) 
                     }
                     acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fp[0][i][ks], fq[0][j][ks], acc[i][j], 0, 0, 0);
                 }
+        free = slot;
+        slot = slot + 1 == D ? 0 : slot + 1;
     }
 
-    const int last = ((steps + G - 1) / G - 1) & 1;          // the stage of the last step
-    float* const sums = reinterpret_cast<float*>(smem + 2 * STAGE);
+    const int res_slot = rounds % D, reslo_slot = (rounds + 1) % D;
+    float* const sums = reinterpret_cast<float*>(smem + D * STAGE);
     if (RES || G > 1) {
         __syncthreads();
-        if (RES_LO && grp == 0) res_dma(reslo, last);
+        if (RES_LO && D == 2 && grp == 0) res_dma(reslo, reslo_slot);
         if (G > 1 && grp > 0)
 #pragma unroll
             for (int i = 0; i < F; ++i)
@@ -522,8 +539,8 @@ __global__ __launch_bounds__(256 * G, G == 1 ? (SPLIT && T == 128 ? 1 : 2) : G) 
 #pragma unroll
                 for (int e4 = 0; e4 < 4; ++e4) {
                     h16x4 hi, lo;
-                    if (RES) hi = res_read(last ^ 1, i, j, e4);
-                    if (RES_LO) lo = res_read(last, i, j, e4);
+                    if (RES) hi = res_read(res_slot, i, j, e4);
+                    if (RES_LO) lo = res_read(reslo_slot, i, j, e4);
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         float& v = reinterpret_cast<float*>(&acc[i][j])[4 * e4 + e];
@@ -1003,13 +1020,13 @@ static int64_t ns_tiles(const NsGemmArgs& g, int side, bool sym, uint32_t* first
     return at;
 }
 
-template <int T, int G, int PHASE, bool SPLIT>
+template <int T, int G, int D, int PHASE, bool SPLIT>
 static int ns_launch_as(NsGemmArgs& g, hipStream_t st) {
-    constexpr int LDS = ns_lds_bytes<T, G, PHASE, SPLIT>();
+    constexpr int LDS = ns_lds_bytes<T, G, D, PHASE, SPLIT>();
     static DevFlags done;
     DevFlag flag = dev_flag(done);
     if (LDS > 65536 && !flag) {
-        if (hipFuncSetAttribute(reinterpret_cast<const void*>(&ns_gemm_kernel<T, G, PHASE, SPLIT>), hipFuncAttributeMaxDynamicSharedMemorySize,
+        if (hipFuncSetAttribute(reinterpret_cast<const void*>(&ns_gemm_kernel<T, G, D, PHASE, SPLIT>), hipFuncAttributeMaxDynamicSharedMemorySize,
                                 LDS) != hipSuccess)
             return MVIT_ELAUNCH;
         flag = true;
@@ -1020,23 +1037,42 @@ static int ns_launch_as(NsGemmArgs& g, hipStream_t st) {
     // runs of about 32 tiles (16 and 64 measured the same), as many for every XCD
     const uint32_t rounds = (g.blocks + 255) / 256;
     g.run = (g.blocks + 8 * rounds - 1) / (8 * rounds);
-    hipLaunchKernelGGL((ns_gemm_kernel<T, G, PHASE, SPLIT>), dim3(rounds * 8 * g.run), dim3(256 * G), LDS, st, g);
+    hipLaunchKernelGGL((ns_gemm_kernel<T, G, D, PHASE, SPLIT>), dim3(rounds * 8 * g.run), dim3(256 * G), LDS, st, g);
     return hipGetLastError() == hipSuccess ? MVIT_OK : MVIT_ELAUNCH;
 }
 
-// Tiles of 128 once there are two for each of the 256 CUs, else tiles of 64; four groups of waves per tile (SPLIT, whose
-// stages are twice as large: two) where even those leave CUs idle and the longest sum has steps for them.
+// Tiles of 128 (one pair of stages: two workgroups per CU, SPLIT one) read each operand half as often as tiles of 64, but are a quarter
+// as many and take longer each: they are taken from 512 tiles on, and where the sums are about equally long (one
+// that outlives the others leaves the rest of the chip idle: the model's A = X X^T, 300 tiles, 54 us against 46) from 192 on, which is three for
+// each four CUs; SPLIT: where every round of 256 is more than three quarters full.  All five iterations, in us, below 512 tiles with
+// tiles of 64 / with this rule: 3000 x 4000 1185 / 1015, 2500 x 2500 724 / 606, 2048 x 3000 503 / 460, 3 x 600 x 2000 173 / 179; SPLIT 2500 x 2500
+// 1550 / 1317, 3 x 1500 x 1500 995 / 877.
+// Tiles of 64: up to 512 of them two per CU, whose time is the latency of their steps, take five stages; from eight steps on and with at most one
+// tile per CU two groups of waves share them.  (All five iterations of 768 x 2304: 168 us with two stages and four groups / 156; 384 x 1536 118 /
+// 108; more tiles than that overlap each other: three stages measured as two.)  SPLIT, whose stages are twice as large, gains nothing from
+// their number (A = X X^T of 768 x 2304: two groups with two stages 22 us, one with five 24).
 template <int PHASE, bool SPLIT>
 static int ns_launch(NsGemmArgs& g, hipStream_t st) {
     constexpr bool SYM = PHASE == NS_GRAM || PHASE == NS_POLY;
-    if (ns_tiles(g, 128, SYM, nullptr) >= 512) return ns_launch_as<128, 1, PHASE, SPLIT>(g, st);
-    int steps = 0;
+    int longest = 0;
+    int64_t work = 0;                     // steps of all tiles of 128
     for (int i = 0; i < g.count; ++i) {
-        const int k = (int)(pad64(PHASE == NS_GRAM ? g.n[i] : g.m[i]) / NS_BK);
-        steps = k > steps ? k : steps;
+        const int64_t mt = (pad64(g.m[i]) + 127) / 128, nt = (pad64(g.n[i]) + 127) / 128;
+        const int steps = (int)(pad64(PHASE == NS_GRAM ? g.n[i] : g.m[i]) / NS_BK);
+        work += (SYM ? mt * (mt + 1) / 2 : mt * nt) * steps;
+        longest = std::max(longest, steps);
     }
-    if (steps >= 8 && ns_tiles(g, 64, SYM, nullptr) <= 256) return ns_launch_as<64, SPLIT ? 2 : 4, PHASE, SPLIT>(g, st);
-    return ns_launch_as<64, 1, PHASE, SPLIT>(g, st);
+    const int64_t t128 = ns_tiles(g, 128, SYM, nullptr), t64 = ns_tiles(g, 64, SYM, nullptr);
+    const bool even = 4 * work >= 3 * t128 * longest;
+    if (SPLIT) {
+        if (t128 > 192 * ((t128 + 255) / 256) && (even || t128 >= 512)) return ns_launch_as<128, 1, 2, PHASE, SPLIT>(g, st);
+        if (longest >= 8 && t64 <= 256) return ns_launch_as<64, 2, 2, PHASE, SPLIT>(g, st);
+    } else {
+        if (t128 >= 512 || (t128 >= 192 && even)) return ns_launch_as<128, 1, 2, PHASE, SPLIT>(g, st);
+        if (longest >= 8 && t64 <= 256) return ns_launch_as<64, 2, SPLIT ? 2 : 5, PHASE, SPLIT>(g, st);
+        if (t64 <= 512) return ns_launch_as<64, 1, SPLIT ? 2 : 5, PHASE, SPLIT>(g, st);
+    }
+    return ns_launch_as<64, 1, 2, PHASE, SPLIT>(g, st);
 }
 
 template <bool SPLIT>

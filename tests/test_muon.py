@@ -127,6 +127,29 @@ def test_rows_far_apart():
 
 
 @gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_sums_of_every_depth(dtype):
+    """1 to 12 steps of k in the products with few rows, more in the Gram matrix, wide and tall, alone and in a set of unequal ones."""
+    shapes = [(64 * k - 7, max(700 + 64 * k, 2700 - 500 * k)) for k in range(1, 13)]
+    for i, (r, c) in enumerate(shapes):
+        u = gradient(r, c, i)
+        u = u.t() if i % 2 else u
+        near(orthogonalize(u, dtype=dtype), u, dtype == torch.float32)
+    us = [gradient(r, c, i) for i, (r, c) in enumerate(shapes)]
+    for got, u in zip(orthogonalize(us, dtype=dtype), us):
+        near(got, u, dtype == torch.float32)
+
+
+@gpu
+@pytest.mark.parametrize("shapes", [[(2500, 2510)], [(500, 700)] * 5, [(768, 2304), (300, 2304)], [(1500, 1510)] * 3], ids=str)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_sets_between_the_tile_sizes(shapes, dtype):
+    us = [gradient(r, c, i) for i, (r, c) in enumerate(shapes)]
+    for got, u in zip(orthogonalize(us, dtype=dtype), us):
+        near(got, u, dtype == torch.float32)
+
+
+@gpu
 @pytest.mark.parametrize("shape", [(2048, 4096), (4160, 2112)])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 def test_large_matrices(shape, dtype):
