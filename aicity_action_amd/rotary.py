@@ -159,6 +159,12 @@ def add_(out, add, x=None):
     return out
 
 
+def _raw_stream(index):
+    """A device's current stream as the C entries take it.  torch.cuda.current_stream makes a Stream object for it: 4 us on the caller's thread
+    and 16 on a backward thread, a tenth of a small call with its gradients."""
+    return torch._C._cuda_getCurrentRawStream(index)
+
+
 def _launch(xs, outs, adds, ps, dim, axes, sections, turns, layout, inverse):
     x, rec = xs[0], b""
     for i, (t, y, p) in enumerate(zip(xs, outs, ps)):
@@ -175,11 +181,12 @@ def _launch(xs, outs, adds, ps, dim, axes, sections, turns, layout, inverse):
     lib = _hip.lib("fp16" if x.dtype == torch.float16 else "bf16")
     act = _hip.F32 if x.dtype == torch.float32 else _hip.BF16
     args = (rec, len(xs), dim, axes, sections, turns, layout, 1 if inverse else 0, act)
-    if x.device.index == torch.cuda.current_device():
-        rc = lib.mvit_rotary(*args, torch.cuda.current_stream().cuda_stream)
+    at = x.device.index
+    if at == torch.cuda.current_device():
+        rc = lib.mvit_rotary(*args, _raw_stream(at))
     else:
-        with torch.cuda.device(x.device):
-            rc = lib.mvit_rotary(*args, torch.cuda.current_stream().cuda_stream)
+        with torch.cuda.device(at):
+            rc = lib.mvit_rotary(*args, _raw_stream(at))
     _hip.check(rc, "rotary")
 
 
@@ -190,7 +197,7 @@ def _leaf_on_one_stream(t):
     if not (t.is_leaf and t.requires_grad):
         return None
     node = torch.autograd.graph.get_gradient_edge(t).node
-    stream = torch.cuda.current_stream(t.device).cuda_stream
+    stream = _raw_stream(t.device.index)
     if torch.cuda.is_current_stream_capturing() and node.metadata.get("rotary_stream", stream) != stream:
         raise RuntimeError("AxialRotary: an eager graph of this leaf tensor is still alive while its backward pass is being captured; "
                            "drop it (its outputs, its loss) before the capture")

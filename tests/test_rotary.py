@@ -216,7 +216,7 @@ def test_capture_beside_a_living_eager_graph_is_refused(monkeypatch):
     class Stream(object):
         cuda_stream = 1
     capturing = [False]
-    monkeypatch.setattr(torch.cuda, "current_stream", lambda device=None: Stream)
+    monkeypatch.setattr(rotary, "_raw_stream", lambda index: Stream.cuda_stream)
     monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: capturing[0])
     x = torch.zeros(3, requires_grad=True)
     node = rotary._leaf_on_one_stream(x)
