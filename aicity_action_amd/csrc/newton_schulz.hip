@@ -60,6 +60,7 @@ struct NsGemmArgs {
     uint8_t tall[NS_MAX];
     int count;
     uint32_t blocks, run;    // tiles, and how many in a row go to one XCD
+    uint32_t quarters;       // > 0: the tiles are the quarters of the tiles of 128 from quarters - 1 on (first counts tiles of 128)
     h16* ws;
     float a, b, c;
     int cur;                 // which of the two buffers holds the current X
@@ -348,10 +349,12 @@ __global__ __launch_bounds__(256 * G, G == 1 ? (SPLIT && T == 128 ? 1 : 2) : G) 
     extern __shared__ __attribute__((aligned(16))) char smem[];
     const uint32_t blk = ns_tile_of(blockIdx.x, a.run);
     if (blk >= a.blocks) return;
-    const int id = ns_find([&](int i) { return a.first[i]; }, a.count, blk);
+    const bool quarter = T == 64 && a.quarters;
+    const uint32_t unit = quarter ? a.quarters - 1 + blk / 4 : blk;
+    const int id = ns_find([&](int i) { return a.first[i]; }, a.count, unit);
     const int m = a.m[id], n = a.n[id], mp = ns_pad(m), np = ns_pad(n);
     const NsRegion g(a.ws, a.off[id], m, n);
-    const uint32_t tile = blk - a.first[id];
+    const uint32_t tile = unit - a.first[id];
 
     int tm, tn;
     if (SYM) {
@@ -362,14 +365,20 @@ __global__ __launch_bounds__(256 * G, G == 1 ? (SPLIT && T == 128 ? 1 : 2) : G) 
         tm = (int)(tile - (uint32_t)J * (J + 1) / 2);
     } else {
         // bands of eight tiles of B, through all of X: a run of tiles shares few of either
-        const uint32_t tiles_n = (mp + T - 1) / T, tiles_m = (np + T - 1) / T;
+        const int side = quarter ? 128 : T;
+        const uint32_t tiles_n = (mp + side - 1) / side, tiles_m = (np + side - 1) / side;
         const uint32_t band = tile / (8 * tiles_m), in_band = tile - band * 8 * tiles_m;
         const uint32_t width = min(8u, tiles_n - band * 8);
         tm = in_band / width;
         tn = band * 8 + (in_band - (uint32_t)tm * width);
     }
-    const int m0 = tm * T, n0 = tn * T;
     const int lim_m = SYM ? mp : np, lim_n = mp;   // extents of the output
+    if (quarter) {
+        tm = 2 * tm + (int)(blk & 1);
+        tn = 2 * tn + (int)(blk >> 1 & 1);
+        if (tm * T >= lim_m || tn * T >= lim_n || (SYM && tm > tn)) return;
+    }
+    const int m0 = tm * T, n0 = tn * T;
     const int tid = threadIdx.x, grp = __builtin_amdgcn_readfirstlane(tid >> 8), wave = __builtin_amdgcn_readfirstlane((tid >> 6) & 3);
     const int lane = tid & 63, r = lane & 31, h = lane >> 5;
     const int wm = (wave & 1) * (T / 2), wn = (wave >> 1) * (T / 2);
@@ -1021,7 +1030,8 @@ static int64_t ns_tiles(const NsGemmArgs& g, int side, bool sym, uint32_t* first
 }
 
 template <int T, int G, int D, int PHASE, bool SPLIT>
-static int ns_launch_as(NsGemmArgs& g, hipStream_t st) {
+static int ns_launch_as(NsGemmArgs& g, hipStream_t st, int64_t rest = 0) {
+    constexpr bool SYM = PHASE == NS_GRAM || PHASE == NS_POLY;
     constexpr int LDS = ns_lds_bytes<T, G, D, PHASE, SPLIT>();
     static DevFlags done;
     DevFlag flag = dev_flag(done);
@@ -1031,9 +1041,11 @@ static int ns_launch_as(NsGemmArgs& g, hipStream_t st) {
             return MVIT_ELAUNCH;
         flag = true;
     }
-    const int64_t tiles = ns_tiles(g, T, PHASE == NS_GRAM || PHASE == NS_POLY, g.first);
-    if (tiles > 0x7fffff00) return MVIT_EUNSUPPORTED;
-    g.blocks = (uint32_t)tiles;
+    // rest: that many tiles of 128 at the end are left to a second launch, which takes their quarters (T = 64)
+    const int64_t tiles = ns_tiles(g, rest ? 128 : T, SYM, g.first);
+    if (tiles > 0x1fffff00) return MVIT_EUNSUPPORTED;
+    g.quarters = T == 64 && rest ? (uint32_t)(tiles - rest) + 1 : 0;
+    g.blocks = (uint32_t)(T == 64 && rest ? 4 * rest : tiles - rest);
     // runs of about 32 tiles (16 and 64 measured the same), as many for every XCD
     const uint32_t rounds = (g.blocks + 255) / 256;
     g.run = (g.blocks + 8 * rounds - 1) / (8 * rounds);
@@ -1047,6 +1059,9 @@ static int ns_launch_as(NsGemmArgs& g, hipStream_t st) {
 // each four CUs; SPLIT: where every round of 256 is more than three quarters full.  All five iterations, in us, below 512 tiles with
 // tiles of 64 / with this rule: 3000 x 4000 1185 / 1015, 2500 x 2500 724 / 606, 2048 x 3000 503 / 460, 3 x 600 x 2000 173 / 179; SPLIT 2500 x 2500
 // 1550 / 1317, 3 x 1500 x 1500 995 / 877.
+// Up to 64 tiles of 128 behind the last full round (528 = 512 + 16 in the A of 4096 x 4096) would keep the chip waiting for a whole sum: a second
+// launch takes their quarters, on four times as many CUs and two groups of waves each.  4096 x 4096 1823 / 1697, 4000 x 4100 1989 / 1792; SPLIT
+// 4817 / 4371.  (Sums of 16 steps or more; shorter ones are over before a launch is.)
 // Tiles of 64: up to 512 of them two per CU, whose time is the latency of their steps, take five stages; from eight steps on and with at most one
 // tile per CU two groups of waves share them.  (All five iterations of 768 x 2304: 168 us with two stages and four groups / 156; 384 x 1536 118 /
 // 108; more tiles than that overlap each other: three stages measured as two.)  SPLIT, whose stages are twice as large, gains nothing from
@@ -1054,21 +1069,31 @@ static int ns_launch_as(NsGemmArgs& g, hipStream_t st) {
 template <int PHASE, bool SPLIT>
 static int ns_launch(NsGemmArgs& g, hipStream_t st) {
     constexpr bool SYM = PHASE == NS_GRAM || PHASE == NS_POLY;
-    int longest = 0;
+    int longest = 0, longest_rest = 0;
     int64_t work = 0;                     // steps of all tiles of 128
+    const int64_t t128 = ns_tiles(g, 128, SYM, nullptr), t64 = ns_tiles(g, 64, SYM, nullptr), slots = SPLIT ? 256 : 512;
+    int64_t rest = t128 % slots, at = 0;
     for (int i = 0; i < g.count; ++i) {
-        const int64_t mt = (pad64(g.m[i]) + 127) / 128, nt = (pad64(g.n[i]) + 127) / 128;
+        const int64_t mt = (pad64(g.m[i]) + 127) / 128, nt = (pad64(g.n[i]) + 127) / 128, tiles = SYM ? mt * (mt + 1) / 2 : mt * nt;
         const int steps = (int)(pad64(PHASE == NS_GRAM ? g.n[i] : g.m[i]) / NS_BK);
-        work += (SYM ? mt * (mt + 1) / 2 : mt * nt) * steps;
+        at += tiles;
+        work += tiles * steps;
         longest = std::max(longest, steps);
+        if (at > t128 - rest) longest_rest = std::max(longest_rest, steps);
     }
-    const int64_t t128 = ns_tiles(g, 128, SYM, nullptr), t64 = ns_tiles(g, 64, SYM, nullptr);
+    if (t128 < slots || rest > 64 || longest_rest < 16) rest = 0;
     const bool even = 4 * work >= 3 * t128 * longest;
     if (SPLIT) {
-        if (t128 > 192 * ((t128 + 255) / 256) && (even || t128 >= 512)) return ns_launch_as<128, 1, 2, PHASE, SPLIT>(g, st);
+        if (t128 - rest > 192 * ((t128 - rest + 255) / 256) && (even || t128 >= 512)) {
+            const int rc = ns_launch_as<128, 1, 2, PHASE, SPLIT>(g, st, rest);
+            return rc != MVIT_OK || !rest ? rc : ns_launch_as<64, 2, 2, PHASE, SPLIT>(g, st, rest);
+        }
         if (longest >= 8 && t64 <= 256) return ns_launch_as<64, 2, 2, PHASE, SPLIT>(g, st);
     } else {
-        if (t128 >= 512 || (t128 >= 192 && even)) return ns_launch_as<128, 1, 2, PHASE, SPLIT>(g, st);
+        if (t128 >= 512 || (t128 >= 192 && even)) {
+            const int rc = ns_launch_as<128, 1, 2, PHASE, SPLIT>(g, st, rest);
+            return rc != MVIT_OK || !rest ? rc : ns_launch_as<64, 2, SPLIT ? 2 : 5, PHASE, SPLIT>(g, st, rest);
+        }
         if (longest >= 8 && t64 <= 256) return ns_launch_as<64, 2, SPLIT ? 2 : 5, PHASE, SPLIT>(g, st);
         if (t64 <= 512) return ns_launch_as<64, 1, SPLIT ? 2 : 5, PHASE, SPLIT>(g, st);
     }

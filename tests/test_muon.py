@@ -141,7 +141,7 @@ def test_sums_of_every_depth(dtype):
 
 
 @gpu
-@pytest.mark.parametrize("shapes", [[(2500, 2510)], [(500, 700)] * 5, [(768, 2304), (300, 2304)], [(1500, 1510)] * 3], ids=str)
+@pytest.mark.parametrize("shapes", [[(2500, 2510)], [(500, 700)] * 5, [(768, 2304), (300, 2304)], [(1500, 1510)] * 3, [(2900, 3000)], [(4010, 1000), (3000, 2900)], [(4130, 4150)]], ids=str)
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 def test_sets_between_the_tile_sizes(shapes, dtype):
     us = [gradient(r, c, i) for i, (r, c) in enumerate(shapes)]
