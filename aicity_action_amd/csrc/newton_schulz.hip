@@ -14,6 +14,12 @@
 // wrong, with two 0.04 % (384 x 1536, against 64 bits).  The products' own operands are the high halves: their rounding is that of one
 // iteration and is not amplified (a full-rank gradient comes out 0.17 % wrong, which is their share).  SPLIT computes every product from
 // both halves (high high + high low + low high, three times the matrix work): 1e-6, for results wanted in single precision.
+//
+// Bound by the matrix cores where matrices are large: 4096 x 4096 takes 1.70 ms = 810 TFLOP/s counting A and A A half (a large library product of
+// this size: 1100), of which B X runs at 890; its LDS reads and LDS-DMA writes keep the LDS busy 1.5 times as long as the products the matrix
+// cores.  By memory as much as by them where they are many and shallow: the 34 M weights of the video model's blocks take 0.88 ms, of which a
+// launch of B X moves 360 MB in 79 us (4.5 TB/s, counted) beside its 33 GFLOP, the squares and X_0 406 MB each in 74 and 71 us (5.5 and 5.7).
+// By the latency of the chain of launches where they are few and small: 5 to 8 us each for three 1000 x 257.
 #include "common.h"
 #include <string.h>
 #include <algorithm>
@@ -421,7 +427,8 @@ __global__ __launch_bounds__(256 * G, G == 1 ? (SPLIT && T == 128 ? 1 : 2) : G) 
     };
 
     // What is added to the product -- a X or b A -- comes through LDS too, in whole rows: the tile's halves are requested behind the last
-    // step's tile (with two stages the low half follows when the sum is done).  16-byte chunk c of row r lies at c ^ (r & 15) (T = 128) or c ^ ((r >> 1) & 7) (T = 64)
+    // step's tile (with two stages the low half follows when the sum is done).  16-byte chunk c of row r lies at c ^ (r & 15) (T = 128) or
+    // c ^ ((r >> 1) & 7) (T = 64)
     constexpr bool RES = PHASE != NS_GRAM, RES_LO = RES && (PHASE != NS_POLY || SPLIT);
     const h16* const res = PHASE == NS_POLY ? g.a() : g.x(a.cur);
     const h16* const reslo = PHASE == NS_POLY ? g.alo() : g.xlo(SPLIT ? a.cur : 0);
@@ -665,11 +672,12 @@ __global__ __launch_bounds__(256 * G, G == 1 ? (SPLIT && T == 128 ? 1 : 2) : G) 
 
 // ---- 4. small matrices: everything in one workgroup -------------------------------------------------------------------------------------
 // A matrix of at most 48 (SPLIT: 32) tiles of 32 x 32 that fits into the 160 KB of LDS with A and B takes all iterations in one workgroup of
-// sixteen waves, and a call of such matrices is one launch instead of seventeen of 4 to 7 us each (96 x 288).  X stays in the accumulators
-// in single precision.  A lane holds a column of the array the matrix comes from, an accumulator quad four of its rows, so that global
-// accesses are whole lines; LDS holds the fp16 copy (SPLIT: both halves) as Y[column][row], which is X where the matrix is tall and X^T
-// where it is wide, and the products read it along its rows or, with the transposing read, down them as that asks.  Rows in LDS are 16
-// bytes longer than their values, so that the 16 rows a read serves together fall on different banks.
+// sixteen waves, and a call of such matrices is one launch instead of seventeen of 4 to 7 us each (96 x 288: 25.5 us; the four of the video
+// model's first block with their momenta: 37 us, of which the LDS reads of A and of B X, at 128 bytes a clock, are 1.4 us each per iteration).
+// X stays in the accumulators in single precision.  A lane holds a column of the array the matrix comes from, an accumulator quad four of
+// its rows, so that global accesses are whole lines; LDS holds the fp16 copy (SPLIT: both halves) as Y[column][row], which is X where the matrix
+// is tall and X^T where it is wide, and the products read it along its rows or, with the transposing read, down them as that asks.  Rows in
+// LDS are 16 bytes longer than their values, so that the 16 rows a read serves together fall on different banks.
 #define NS_SMALL_MAX 56
 #define NS_SMALL_WAVES 16
 #define NS_SMALL_LDS 163840

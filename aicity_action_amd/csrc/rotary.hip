@@ -9,7 +9,9 @@
 // turns) is one product in 64 bits -- a place of a million turns the fastest pair 160,000 times, which 32 bits would round to a hundredth
 // of a turn -- whose fraction goes on in 32 bits (off by at most 2^-26 of a turn).  Sine and cosine of an eighth of a turn either way are
 // their Taylor polynomials (next terms: 1.8e-9 and 1e-10), the quarter turn is put back by a swap and two signs.  All of it is shared by
-// the rows that a thread walks: the heads of a batch entry, or of all of them where their places are the same.
+// the rows that a thread walks: the heads of a batch entry, or of all of them where their places are the same.  Measured: 313 MB (bf16, one
+// head, 8 clips of 8 x 112 x 112 tokens and their pooled keys) 69 us = 4.5 TB/s, 96 MB (8 x 28 x 28, four heads) 18.3 us = 5.3 TB/s, 658 MB
+// (fp16, listed places around a million) 131 us = 5.0 TB/s; a large copy reaches 5.3 TB/s.  A call's time on the host is 12 us.
 #include "common.h"
 
 struct RotaryArgs {

@@ -1,9 +1,9 @@
 """Orthogonalised updates for weight matrices: Newton-Schulz products and the Muon step, on csrc/newton_schulz.hip.
 
 ``orthogonalize`` pushes the singular values of matrices to about one; ``MuonMatrices`` renews the momenta of a set of weights and steps
-each weight by its orthogonalised momentum, all matrices in the same 17 launches whatever their sizes.  ``solver.construct_optimizer``
-builds a train step on it (``SOLVER.OPTIMIZING_METHOD muon``); the reference's own methods are those of slowfast/models/optimizer.py:140-206.
-Everything runs on the tensors' device and its current stream; there is no CPU fallback."""
+each weight by its orthogonalised momentum, all matrices in the same launches whatever their sizes (one for a set of small ones, else 17 or a
+few more).  ``solver.construct_optimizer`` builds a train step on it (``SOLVER.OPTIMIZING_METHOD muon``); the reference's own methods are
+those of slowfast/models/optimizer.py:140-206.  Everything runs on the tensors' device and its current stream; there is no CPU fallback."""
 import math
 
 import numpy as np
@@ -39,8 +39,10 @@ def orthogonalize(update, steps=5, coefficients=QUINTIC, eps=1e-7, dtype=torch.b
     """Newton-Schulz orthogonalisation of one matrix, a batch [..., rows, columns] or a list of either (sizes may differ; one set of
     launches for all).  float32 / bfloat16 / float16, any strides.  Returns contiguous tensors of ``dtype``.
 
-    ``arithmetic``: "fp16" (default for 16-bit results; within about 2e-3) computes the products from fp16 operands, "split" (default for
-    float32; 1e-5) from pairs of them at three times the work.  A matrix of zeros stays zero; one with NaN or infinity gives NaN."""
+    ``arithmetic``: "fp16" (default for 16-bit results; within about 2e-3, 4e-3 where a matrix of few rows or columns stands beside larger
+    ones) computes the products from fp16 operands, "split" (default for float32; 1e-5) from pairs of them at three times the work; calls with
+    only matrices of at most 32 rows or columns always take pairs.  A matrix of zeros stays zero; one with NaN or infinity gives NaN.  A
+    matrix' last bits depend on the call it is in (which order its sums are taken in)."""
     many = isinstance(update, (list, tuple))
     ts = list(update) if many else [update]
     if arithmetic is None:
@@ -92,7 +94,7 @@ class MuonMatrices(object):
 
     ``step``:  M <- mu M + (1 - mu) g;  U = (1 - mu) g + mu M (Nesterov) or M;  W <- W (1 - lr weight_decay) - lr rms sqrt(max(rows,
     columns)) NS(U).  ``rms`` 0.2 gives the update the size that AdamW's typically has, so that one learning rate and weight decay serve
-    both.  Weights and momenta: contiguous float32 matrices, updated in place; gradients: float32, any strides."""
+    both.  Weights and momenta: contiguous float32 matrices, updated in place; gradients: float32, any strides, in memory of their own."""
 
     def __init__(self, params, momenta=None, momentum=0.95, nesterov=True, weight_decay=0.0, rms=0.2, steps=5, coefficients=QUINTIC,
                  eps=1e-7, arithmetic="fp16"):
