@@ -10,9 +10,10 @@
 // of a turn -- whose fraction goes on in 32 bits (off by at most 2^-26 of a turn).  Sine and cosine of an eighth of a turn either way are
 // their Taylor polynomials (next terms: 1.8e-9 and 1e-10), the quarter turn is put back by a swap and two signs.  All of it is shared by
 // the rows that a thread walks: the heads of a batch entry, or of all of them where their places are the same.  Measured: 313 MB (bf16, one
-// head, 8 clips of 8 x 112 x 112 tokens and their pooled keys) 69 us = 4.5 TB/s, 96 MB (8 x 28 x 28, four heads) 18.3 us = 5.3 TB/s, 658 MB
-// (fp16, listed places around a million) 131 us = 5.0 TB/s; a large copy reaches 5.3 TB/s.  A call's time on the host is 12 us.
+// head, 8 clips of 8 x 112 x 112 tokens and their pooled keys) 63 us = 5.0 TB/s, 96 MB (8 x 28 x 28, four heads) 18.6 us = 5.2 TB/s, 658 MB
+// (fp16, listed places around a million) 129 us = 5.1 TB/s; a large copy reaches 5.3 TB/s.  A call's time on the host is 12 us.
 #include "common.h"
+#include <algorithm>
 
 struct RotaryArgs {
     mvit_rotary_tensor t[2];
@@ -292,8 +293,12 @@ extern "C" int mvit_rotary(const mvit_rotary_tensor* tensors, int ntensors, int 
         }
     }
     a.tasks = a.pairs / (int)fit + (dim - channels + 2 * (int)fit - 1) / (2 * (int)fit);
-    // Rows per thread: as many (up to 8) as leave 1024 workgroups, four for each of the 256 CUs, so that a turn serves several
-    // rows (four heads on 8 x 28 x 28, B = 8: 19.0 us with 2048, 18.5 with 1024, 18.8 with 512; six heads of 4099 packed tokens 32.6, 29.6, 29.4)
+    // Rows per thread, so that a turn and its addresses serve several: until a thread moves 64 bytes each way (two rows of 16-byte vectors, at
+    // most 8), as long as that leaves 1024 workgroups, four for each of the 256 CUs.  (1, 2, 4, 8 rows: one bf16 head on 8 x 112 x 112,
+    // B = 8, 71, 62.7, 65.7, 68.5 us, in fp32 108, 112, 117, 122; 16 fp16 heads of 20011 listed tokens 163, 129, 129, 131; 8-byte vectors of four
+    // heads on 8 x 28 x 28 20.5, 14.5, 13.4, 13.4; fp32 pairs by themselves 51, 37.7, 32.6, 29.4.  With 2048 / 1024 / 512 workgroups left: 19.0 / 18.5 /
+    // 18.8.  The loads of two or four rows ahead of their stores: 62 to 176 us where one by one takes 63 to 131.)
+    const int most = std::min(8, 32 / ((int)fit * itemsize));
     for (int i = 0; i < ntensors; ++i) {
         const mvit_rotary_tensor& t = a.t[i];
         if (i == 1) a.first_block_1 = (uint32_t)total_blocks;
@@ -304,7 +309,7 @@ extern "C" int mvit_rotary(const mvit_rotary_tensor* tensors, int ntensors, int 
         const bool shared = !t.pos || t.ps[0] == 0;
         const int span = shared ? t.B * t.H : t.H, spans = shared ? 1 : t.B;
         int rpt = 1;
-        while (rpt < 8 && rpt < span && per * spans * (uint64_t)((span + 2 * rpt - 1) / (2 * rpt)) >= 1024) rpt *= 2;
+        while (rpt < most && rpt < span && per * spans * (uint64_t)((span + 2 * rpt - 1) / (2 * rpt)) >= 1024) rpt *= 2;
         a.rows_per_thread[i] = rpt;
         a.span[i] = span;
         a.groups[i] = (uint32_t)((span + rpt - 1) / rpt);
