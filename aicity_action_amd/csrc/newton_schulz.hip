@@ -240,7 +240,8 @@ __global__ __launch_bounds__(256) void ns_start_kernel(const NsLoadArgs a) {
     const T* u = static_cast<const T*>(t.u);
     const int r0 = (tall ? tj : ti) * 64, c0 = (tall ? ti : tj) * 64;   // the tile in U
     const bool by_col = t.cs == 1 || t.rs != 1;
-    // every load is issued before the first is used, at clamped places
+    // every load is issued before the first is used, at clamped places; without Nesterov the update is the momentum itself
+    const bool from_u = !t.mom || a.nesterov;
     const bool quads = sizeof(T) == 4 && t.cs == 1 && (t.rs & 3) == 0 && (t.cols & 3) == 0 &&
                        ((reinterpret_cast<uintptr_t>(u) | reinterpret_cast<uintptr_t>(t.mom)) & 15) == 0;
     if (quads) {
@@ -249,7 +250,7 @@ __global__ __launch_bounds__(256) void ns_start_kernel(const NsLoadArgs a) {
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
             const int r = min(r0 + (tid >> 4) + 16 * k, t.rows - 1);
-            gv[k] = load4(u + (int64_t)r * t.rs + c);
+            if (from_u) gv[k] = load4(u + (int64_t)r * t.rs + c);
             if (t.mom) mv[k] = load4(t.mom + (int64_t)r * t.cols + c);
         }
 #pragma unroll
@@ -271,7 +272,7 @@ __global__ __launch_bounds__(256) void ns_start_kernel(const NsLoadArgs a) {
         for (int k = 0; k < 16; ++k) {
             const int e = k * 256 + tid, lr = by_col ? e >> 6 : e & 63, lc = by_col ? e & 63 : e >> 6;
             const int r = min(r0 + lr, t.rows - 1), c = min(c0 + lc, t.cols - 1);
-            gv[k] = ns_ld(u + (int64_t)r * t.rs + (int64_t)c * t.cs);
+            if (from_u) gv[k] = ns_ld(u + (int64_t)r * t.rs + (int64_t)c * t.cs);
             if (t.mom) mv[k] = t.mom[(int64_t)r * t.cols + c];
         }
 #pragma unroll
