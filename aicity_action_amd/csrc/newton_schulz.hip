@@ -15,7 +15,7 @@
 // iteration and is not amplified (a full-rank gradient comes out 0.17 % wrong, which is their share).  SPLIT computes every product from
 // both halves (high high + high low + low high, three times the matrix work): 1e-6, for results wanted in single precision.
 //
-// Bound by the matrix cores where matrices are large: 4096 x 4096 takes 1.70 ms = 810 TFLOP/s counting A and A A half (a large library product of
+// Bound by the matrix cores where matrices are large: 4096 x 4096 takes 1.7 ms = 800 TFLOP/s counting A and A A half (a large library product of
 // this size: 1100), of which B X runs at 890; its LDS reads and LDS-DMA writes keep the LDS busy 1.5 times as long as the products the matrix
 // cores.  By memory as much as by them where they are many and shallow: the 34 M weights of the video model's blocks take 0.88 ms, of which a
 // launch of B X moves 360 MB in 79 us (4.5 TB/s, counted) beside its 33 GFLOP, the squares and X_0 406 MB each in 74 and 71 us (5.5 and 5.7).
