@@ -226,6 +226,18 @@ def test_muon_step(nesterov, arithmetic):
 
 
 @gpu
+@pytest.mark.parametrize("nesterov,arithmetic", [(True, "fp16"), (False, "fp16"), (True, "split")])
+@pytest.mark.parametrize("shapes", [[(4160, 2110)], [(768, 2304), (2304, 766)], [(1510, 1500)] * 3], ids=str)
+def test_muon_step_of_large_matrices(shapes, nesterov, arithmetic):
+    """Sets that take large tiles, some in a second launch."""
+    ws, ms, gs = [[f * gradient(r, c, s + i) for i, (r, c) in enumerate(shapes)] for f, s in ((0.02, 10), (1e-3, 30), (1.0, 50))]
+    w0, m0 = [w.clone() for w in ws], [m.clone() for m in ms]
+    MuonMatrices(ws, ms, momentum=0.9, nesterov=nesterov, weight_decay=0.05, arithmetic=arithmetic).step(gs, lr=0.01)
+    for w, m, wo, mo, g in zip(ws, ms, w0, m0, gs):
+        check_step(w, m, wo, mo, g, 0.01, 0.9, nesterov, 0.05, split=arithmetic == "split")
+
+
+@gpu
 def test_muon_factor_guard_and_grad_attribute():
     w, g = torch.nn.Parameter(0.02 * gradient(40, 60, 1)), gradient(40, 60, 2)
     plan, w0 = MuonMatrices([w], weight_decay=0.1), w.detach().clone()
