@@ -672,9 +672,10 @@ __global__ __launch_bounds__(256 * G, G == 1 ? (SPLIT && T == 128 ? 1 : 2) : G) 
 }
 
 // ---- 4. small matrices: everything in one workgroup -------------------------------------------------------------------------------------
-// A matrix of at most 48 (SPLIT: 32) tiles of 32 x 32 that fits into the 160 KB of LDS with A and B takes all iterations in one workgroup of
-// sixteen waves, and a call of such matrices is one launch instead of seventeen of 4 to 7 us each (96 x 288: 25.5 us; the four of the video
-// model's first block with their momenta: 37 us, of which the LDS reads of A and of B X, at 128 bytes a clock, are 1.4 us each per iteration).
+// A matrix of at most 48 (SPLIT: 32) tiles of 32 x 32 that fits into the 160 KB of LDS with A (B takes its place) takes all iterations in one
+// workgroup of sixteen waves, and a call of such matrices is one launch instead of seventeen of 4 to 7 us each (96 x 288 26 us, 128 x 384
+// 56 / 70, in SPLIT 96 x 288 47 / 93; the four of the video model's first block with their momenta 37).  Its time is the latency of reads,
+// products and barriers in a row: A from its upper tiles alone, a third fewer reads, took as long.
 // X stays in the accumulators in single precision.  A lane holds a column of the array the matrix comes from, an accumulator quad four of
 // its rows, so that global accesses are whole lines; LDS holds the fp16 copy (SPLIT: both halves) as Y[column][row], which is X where the matrix
 // is tall and X^T where it is wide, and the products read it along its rows or, with the transposing read, down them as that asks.  Rows in
@@ -703,7 +704,7 @@ static inline int64_t ns_small_bytes(int rows, int cols, bool split) {
     const int64_t mp = ns_pad32(rows < cols ? rows : cols), np = ns_pad32(rows < cols ? cols : rows);
     if (mp > 128 || mp * np > (split ? 32 : 48) * 1024) return -1;
     const int64_t y = rows > cols ? mp * (np * 2 + 16) : np * (mp * 2 + 16);
-    const int64_t bytes = (split ? 2 : 1) * (y + 2 * mp * (mp * 2 + 16)) + 256;
+    const int64_t bytes = (split ? 2 : 1) * (y + mp * (mp * 2 + 16)) + 256;
     return bytes <= NS_SMALL_LDS ? bytes : -1;
 }
 
@@ -739,7 +740,6 @@ __device__ __forceinline__ void ns_small_body(const NsSmallArgs& a, const NsSmal
     const int ypl = cp * ldy, apl = mp * lda;                   // bytes of a plane
     char* const sy = smem + 256;
     char* const sa = sy + PL * ypl;
-    char* const sb = sa + PL * apl;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane0 = threadIdx.x & 63;
     const float coef = a.norm_coef ? a.norm_coef[1] : 1.0f;
     const bool bad = ns_bad(a.norm_coef);
@@ -912,6 +912,7 @@ __device__ __forceinline__ void ns_small_body(const NsSmallArgs& a, const NsSmal
         __syncthreads();
         if (wave < nb * nb) {
             const f32x16 acc = product(along, along, sa, lda, apl, sa, lda, apl, 32 * ti, 32 * tj, mp);
+            __syncthreads();                                    // everyone has read A: each wave puts its tile of B in its tile's place
 #pragma unroll
             for (int e4 = 0; e4 < 4; ++e4) {
                 const int N = 32 * tj + r, M = 32 * ti + 8 * e4 + 4 * h;
@@ -926,16 +927,17 @@ __device__ __forceinline__ void ns_small_body(const NsSmallArgs& a, const NsSmal
                 }
 #pragma unroll
                 for (int e = 0; e < 4; ++e) v[e] = a.b * v[e] + a.c / NS_S * acc[4 * e4 + e];
-                put(sb, lda, apl, v, N, M);
+                put(sa, lda, apl, v, N, M);
             }
-        }
+        } else
+            __syncthreads();                                    // (a wave goes one way as a whole)
         __syncthreads();
 #pragma unroll
         for (int k = 0; k < TPW; ++k) {
             int rt, ct;
             if (tile_of(k, rt, ct)) {
-                const f32x16 acc = TALL ? product(down, along, sy, ldy, ypl, sb, lda, apl, 32 * rt, 32 * ct, mp)
-                                        : product(along, along, sb, lda, apl, sy, ldy, ypl, 32 * rt, 32 * ct, mp);
+                const f32x16 acc = TALL ? product(down, along, sy, ldy, ypl, sa, lda, apl, 32 * rt, 32 * ct, mp)
+                                        : product(along, along, sa, lda, apl, sy, ldy, ypl, 32 * rt, 32 * ct, mp);
 #pragma unroll
                 for (int e = 0; e < 16; ++e) x[k][e] = a.a * x[k][e] + acc[e] * (1.0f / NS_S);
             }

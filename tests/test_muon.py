@@ -128,6 +128,19 @@ def test_rows_far_apart():
 
 @gpu
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_around_what_fits_one_workgroup(dtype):
+    for i, (r, c) in enumerate([(128, 128), (128, 160), (100, 190), (128, 384), (127, 383), (128, 400), (64, 448), (60, 500), (96, 297), (96, 512), (32, 1024),
+                                (32, 1600), (5, 1500)]):
+        u = gradient(r, c, i)
+        near(orthogonalize(u, dtype=dtype), u, dtype == torch.float32)
+        near(orthogonalize(u.t(), dtype=dtype), u.t(), dtype == torch.float32)
+    us = [gradient(20 + 9 * i, 130 - 3 * i, i) for i in range(12)]
+    for got, u in zip(orthogonalize(us, dtype=dtype), us):
+        near(got, u, dtype == torch.float32)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 def test_sums_of_every_depth(dtype):
     """1 to 12 steps of k in the products with few rows, more in the Gram matrix, wide and tall, alone and in a set of unequal ones."""
     shapes = [(64 * k - 7, max(700 + 64 * k, 2700 - 500 * k)) for k in range(1, 13)]
