@@ -417,7 +417,10 @@ __global__ __launch_bounds__(256 * G, G == 1 ? (SPLIT && T == 128 ? 1 : 2) : G) 
     const int rounds = (steps + G - 1) / G, mine = (steps - grp + G - 1) / G;      // group 0 takes one in every round
     const h16* const src_hi = PHASE == NS_GRAM ? g.x(a.cur) : PHASE == NS_POLY ? g.a() : is_q ? g.b() : g.x(a.cur);
     const h16* const src_lo = PHASE == NS_GRAM ? g.xlo(a.cur) : PHASE == NS_POLY ? g.alo() : is_q ? g.blo() : g.xlo(a.cur);
+    // a tile on the diagonal: Q is P, and is not loaded (20 x 2500, a single tile: 143 -> 127 us; nothing to gain where there are many)
+    const bool same = SYM && T == 64 && tm == tn;
     auto dma = [=](int kt, int stage) {
+        if (same && is_q) return;
         char* dst = lds + stage * STAGE + (is_q ? PL * T * 128 : 0) + (wave & 1) * PW * 1024;
 #pragma unroll
         for (int pl = 0; pl < PL; ++pl) {
@@ -492,7 +495,7 @@ __global__ __launch_bounds__(256 * G, G == 1 ? (SPLIT && T == 128 ? 1 : 2) : G) 
 #pragma unroll
         for (int pl = 0; pl < PL; ++pl) {
             const char* sp = lds + slot * STAGE + pl * T * 128;
-            const char* sq = sp + PL * T * 128;
+            const char* sq = same ? sp : sp + PL * T * 128;
 #pragma unroll
             for (int ks = 0; ks < 4; ++ks)
 #pragma unroll
