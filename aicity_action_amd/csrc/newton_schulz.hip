@@ -32,6 +32,7 @@ typedef __attribute__((address_space(3))) bf16x4 ns_lds_b4;
 
 #define NS_MAX 72            // matrices per set of launches (kernel arguments hold their table)
 #define NS_PARTS 256         // partial sums of squares per matrix
+#define NS_SUMS 256          // partial tiles of 64 x 64 in the workspace
 #define NS_BK 64             // depth of a K step; every matrix is padded with zeros to a multiple of it
 // X, A and B are held times 2^12: their entries are at most their largest singular values (1.3, 1.6, 2.8 for the usual coefficients), so
 // there is room to 16, and the low halves of entries down to 1e-4 are still normal fp16 numbers, which the matrix cores want
@@ -67,6 +68,8 @@ struct NsGemmArgs {
     int count;
     uint32_t blocks, run;    // tiles, and how many in a row go to one XCD
     uint32_t quarters;       // > 0: the tiles are the quarters of the tiles of 128 from quarters - 1 on (first counts tiles of 128)
+    uint32_t cuts;           // NS_PART, NS_JOIN: pieces of every sum
+    float* sums;             // ... and their partial tiles
     h16* ws;
     float a, b, c;
     int cur;                 // which of the two buffers holds the current X
@@ -315,7 +318,10 @@ __global__ __launch_bounds__(256) void ns_start_kernel(const NsLoadArgs a) {
 // u ^ (r & 3) (T = 128) or u ^ ((r >> 1) & 1) (T = 64): the four rows of a transposing read fall on different banks.
 // The tile leaves through LDS in whole rows.  An accumulator register quad is four values along M, so [N][M] is the straight order:
 // X itself, A, B, and the result of a wide matrix; the mirrored tiles of A and B and the result of a tall matrix are turned on the way.
-enum { NS_GRAM = 0, NS_POLY = 1, NS_STEP = 2, NS_LAST16 = 3, NS_LAST32 = 4, NS_MUON = 5 };
+// NS_PART computes one of the pieces of every sum of A = X X^T into the workspace, NS_JOIN adds them in order and goes on as NS_GRAM.
+enum { NS_GRAM = 0, NS_POLY = 1, NS_STEP = 2, NS_LAST16 = 3, NS_LAST32 = 4, NS_MUON = 5, NS_PART = 6, NS_JOIN = 7 };
+__host__ __device__ constexpr bool ns_is_gram(int phase) { return phase == NS_GRAM || phase >= NS_PART; }
+__host__ __device__ constexpr bool ns_is_last(int phase) { return phase >= NS_LAST16 && phase <= NS_MUON; }
 
 // Workgroups go to the eight XCDs in turn, each with an L2 of its own: a run of tiles, which share operand tiles, goes to one XCD.
 __device__ __forceinline__ uint32_t ns_tile_of(uint32_t wg, uint32_t run) {
@@ -334,7 +340,7 @@ __device__ __forceinline__ void ns_dma(const h16* base, uint32_t offset, const c
 template <int T, int G, int D, int PHASE, bool SPLIT>
 constexpr int ns_lds_bytes() {
     const int stages = G * D * (SPLIT ? 4 : 2) * T * 128;           // (the groups' sums lie within: behind the first group's stages)
-    const int out = PHASE >= NS_LAST16 ? T * (T * 4 + 16) : 2 * T * (T * 2 + 16);
+    const int out = ns_is_last(PHASE) ? T * (T * 4 + 16) : 2 * T * (T * 2 + 16);
     return stages > out ? stages : out;
 }
 
@@ -351,13 +357,12 @@ __global__ __launch_bounds__(256 * G, G == 1 ? (SPLIT && T == 128 ? 1 : 2) : G) 
     constexpr int F = T / 64;                      // 32 x 32 accumulators per wave and direction
     constexpr int PL = SPLIT ? 2 : 1;              // planes of an operand: high halves, low halves
     constexpr int STAGE = 2 * PL * T * 128;        // bytes of the P tiles + Q tiles of a step
-    constexpr bool SYM = PHASE == NS_GRAM || PHASE == NS_POLY;
-    constexpr bool LAST = PHASE >= NS_LAST16;
+    constexpr bool GRAM = ns_is_gram(PHASE), SYM = GRAM || PHASE == NS_POLY, LAST = ns_is_last(PHASE);
     extern __shared__ __attribute__((aligned(16))) char smem[];
     const uint32_t blk = ns_tile_of(blockIdx.x, a.run);
     if (blk >= a.blocks) return;
     const bool quarter = T == 64 && a.quarters;
-    const uint32_t unit = quarter ? a.quarters - 1 + blk / 4 : blk;
+    const uint32_t unit = quarter ? a.quarters - 1 + blk / 4 : PHASE == NS_PART ? blk / a.cuts : blk;
     const int id = ns_find([&](int i) { return a.first[i]; }, a.count, unit);
     const int m = a.m[id], n = a.n[id], mp = ns_pad(m), np = ns_pad(n);
     const NsRegion g(a.ws, a.off[id], m, n);
@@ -396,7 +401,7 @@ __global__ __launch_bounds__(256 * G, G == 1 ? (SPLIT && T == 128 ? 1 : 2) : G) 
     constexpr int PW = T / 16;
     const bool is_q = wave >= 2;
     const bool by_k = !SYM && !is_q;               // the tile of X as it lies
-    const int ldk = PHASE == NS_GRAM || !SYM ? np : mp;      // row length of P
+    const int ldk = GRAM || !SYM ? np : mp;      // row length of P
     const int ld_src = is_q && !SYM ? mp : ldk;
     uint32_t src_off[PW];                          // byte offset of this lane's 16 bytes from the operand's tile
 #pragma unroll
@@ -413,10 +418,16 @@ __global__ __launch_bounds__(256 * G, G == 1 ? (SPLIT && T == 128 ? 1 : 2) : G) 
         }
     }
     const int64_t k_step = by_k ? (int64_t)NS_BK * ld_src : NS_BK;
-    const int steps = (PHASE == NS_GRAM ? np : mp) / NS_BK;
+    int steps = (GRAM ? np : mp) / NS_BK, first_step = 0;
+    if (PHASE == NS_PART) {
+        const int per = (steps + (int)a.cuts - 1) / (int)a.cuts;
+        first_step = (int)(blk - unit * a.cuts) * per;
+        steps = max(0, min(per, steps - first_step));
+    }
+    if (PHASE == NS_JOIN) steps = 0;
     const int rounds = (steps + G - 1) / G, mine = (steps - grp + G - 1) / G;      // group 0 takes one in every round
-    const h16* const src_hi = PHASE == NS_GRAM ? g.x(a.cur) : PHASE == NS_POLY ? g.a() : is_q ? g.b() : g.x(a.cur);
-    const h16* const src_lo = PHASE == NS_GRAM ? g.xlo(a.cur) : PHASE == NS_POLY ? g.alo() : is_q ? g.blo() : g.xlo(a.cur);
+    const h16* const src_hi = GRAM ? g.x(a.cur) : PHASE == NS_POLY ? g.a() : is_q ? g.b() : g.x(a.cur);
+    const h16* const src_lo = GRAM ? g.xlo(a.cur) : PHASE == NS_POLY ? g.alo() : is_q ? g.blo() : g.xlo(a.cur);
     // a tile on the diagonal: Q is P, and is not loaded (20 x 2500, a single tile: 143 -> 127 us; nothing to gain where there are many)
     const bool same = SYM && T == 64 && tm == tn;
     auto dma = [=](int kt, int stage) {
@@ -424,7 +435,7 @@ __global__ __launch_bounds__(256 * G, G == 1 ? (SPLIT && T == 128 ? 1 : 2) : G) 
         char* dst = lds + stage * STAGE + (is_q ? PL * T * 128 : 0) + (wave & 1) * PW * 1024;
 #pragma unroll
         for (int pl = 0; pl < PL; ++pl) {
-            const h16* base = (pl ? src_lo : src_hi) + kt * k_step;
+            const h16* base = (pl ? src_lo : src_hi) + (kt + first_step) * k_step;
 #pragma unroll
             for (int i = 0; i < PW; ++i) ns_dma(base, src_off[i], dst + pl * T * 128 + 1024 * i);
         }
@@ -433,7 +444,7 @@ __global__ __launch_bounds__(256 * G, G == 1 ? (SPLIT && T == 128 ? 1 : 2) : G) 
     // What is added to the product -- a X or b A -- comes through LDS too, in whole rows: the tile's halves are requested behind the last
     // step's tile (with two stages the low half follows when the sum is done).  16-byte chunk c of row r lies at c ^ (r & 15) (T = 128) or
     // c ^ ((r >> 1) & 7) (T = 64)
-    constexpr bool RES = PHASE != NS_GRAM, RES_LO = RES && (PHASE != NS_POLY || SPLIT);
+    constexpr bool RES = !GRAM, RES_LO = RES && (PHASE != NS_POLY || SPLIT);
     const h16* const res = PHASE == NS_POLY ? g.a() : g.x(a.cur);
     const h16* const reslo = PHASE == NS_POLY ? g.alo() : g.xlo(SPLIT ? a.cur : 0);
     auto res_dma = [=](const h16* src, int stage) {
@@ -483,6 +494,12 @@ __global__ __launch_bounds__(256 * G, G == 1 ? (SPLIT && T == 128 ? 1 : 2) : G) 
         for (int j = 0; j < F; ++j)
 #pragma unroll
             for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
+    float* const piece = PHASE >= NS_PART ? a.sums + (int64_t)(PHASE == NS_PART ? blk : unit * a.cuts) * 4096 + wave * 1024 + lane : nullptr;
+    if (PHASE == NS_JOIN)
+#pragma unroll 4
+        for (uint32_t c = 0; c < a.cuts; ++c)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) acc[0][0][e] += piece[(int64_t)c * 4096 + e * 64];
 
     const int q4 = (lane & 15) >> 2;               // transposing read: this lane names four columns of row 8 h + q4 (+ 4)
     const int tr_row = 8 * h + q4, tr_col = (16 * ((lane >> 4) & 1) + 4 * (lane & 3)) * 2;
@@ -544,6 +561,17 @@ __global__ __launch_bounds__(256 * G, G == 1 ? (SPLIT && T == 128 ? 1 : 2) : G) 
         __syncthreads();
     }
     // ---- the new values, times 2^12 but for the last iteration's ---------------------------------------------------------------------------
+    if (PHASE == NS_PART) {
+        if (grp == 0)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                float v = acc[0][0][e];
+#pragma unroll
+                for (int o = 0; o < G - 1; ++o) v += sums[(o * 4 + wave) * 1024 + e * 64 + lane];
+                piece[e * 64] = v;
+            }
+        return;
+    }
     const float f_acc = PHASE == NS_POLY ? a.c / NS_S : LAST ? 1.0f / (NS_S * NS_S) : 1.0f / NS_S;
     const float f_res = PHASE == NS_POLY ? a.b : LAST ? a.a / NS_S : a.a;
     if (grp == 0)
@@ -633,7 +661,7 @@ __global__ __launch_bounds__(256 * G, G == 1 ? (SPLIT && T == 128 ? 1 : 2) : G) 
     char* const o2 = smem + T * ROWB;
 #pragma unroll
     for (int pass = 0; pass < (SYM && SPLIT ? 2 : 1); ++pass) {
-        h16* const d1 = PHASE == NS_STEP ? g.x(a.cur ^ 1) : PHASE == NS_GRAM ? (pass ? g.alo() : g.a()) : (pass ? g.blo() : g.b());
+        h16* const d1 = PHASE == NS_STEP ? g.x(a.cur ^ 1) : GRAM ? (pass ? g.alo() : g.a()) : (pass ? g.blo() : g.b());
         h16* const d2 = PHASE == NS_STEP ? g.xlo(SPLIT ? a.cur ^ 1 : 0) : d1;
         __syncthreads();
         if (grp == 0)
@@ -1029,7 +1057,7 @@ extern "C" int64_t mvit_newton_schulz_workspace_bytes(const mvit_ns_matrix* mats
         if (units > most) most = units;
     }
     if (most > 0xffffffffLL) return MVIT_EUNSUPPORTED;
-    return most * 128 + (int64_t)NS_MAX * NS_PARTS * 8;
+    return most * 128 + (int64_t)NS_MAX * NS_PARTS * 8 + (split ? NS_SUMS * 16384 : 0);
 }
 
 // tiles of a launch at a tile side
@@ -1045,7 +1073,7 @@ static int64_t ns_tiles(const NsGemmArgs& g, int side, bool sym, uint32_t* first
 
 template <int T, int G, int D, int PHASE, bool SPLIT>
 static int ns_launch_as(NsGemmArgs& g, hipStream_t st, int64_t rest = 0) {
-    constexpr bool SYM = PHASE == NS_GRAM || PHASE == NS_POLY;
+    constexpr bool SYM = ns_is_gram(PHASE) || PHASE == NS_POLY;
     constexpr int LDS = ns_lds_bytes<T, G, D, PHASE, SPLIT>();
     static DevFlags done;
     DevFlag flag = dev_flag(done);
@@ -1059,7 +1087,7 @@ static int ns_launch_as(NsGemmArgs& g, hipStream_t st, int64_t rest = 0) {
     const int64_t tiles = ns_tiles(g, rest ? 128 : T, SYM, g.first);
     if (tiles > 0x1fffff00) return MVIT_EUNSUPPORTED;
     g.quarters = T == 64 && rest ? (uint32_t)(tiles - rest) + 1 : 0;
-    g.blocks = (uint32_t)(T == 64 && rest ? 4 * rest : tiles - rest);
+    g.blocks = (uint32_t)(T == 64 && rest ? 4 * rest : tiles - rest) * (PHASE == NS_PART ? g.cuts : 1);
     // runs of about 32 tiles (16 and 64 measured the same), as many for every XCD
     const uint32_t rounds = (g.blocks + 255) / 256;
     g.run = (g.blocks + 8 * rounds - 1) / (8 * rounds);
@@ -1079,7 +1107,9 @@ static int ns_launch_as(NsGemmArgs& g, hipStream_t st, int64_t rest = 0) {
 // Tiles of 64: up to 512 of them two per CU, whose time is the latency of their steps, take five stages; from eight steps on and with at most one
 // tile per CU two groups of waves share them.  (All five iterations of 768 x 2304: 168 us with two stages and four groups / 156; 384 x 1536 118 /
 // 108; more tiles than that overlap each other: three stages measured as two.)  SPLIT, whose stages are twice as large, gains nothing from
-// their number (A = X X^T of 768 x 2304: two groups with two stages 22 us, one with five 24).
+// their number (A = X X^T of 768 x 2304: two groups with two stages 22 us, one with five 24).  There a sum of 16 steps or more on few tiles is
+// cut, so that up to 256 CUs share it and a second launch adds the pieces: 768 x 2304 248 / 224, 200 x 2400 195 / 144, 100 x 2500 183 / 117,
+// 20 x 2500 126 / 92.  (A step of fp16 operands takes a third of that: a launch more would cost what cutting saves.)
 template <int PHASE, bool SPLIT>
 static int ns_launch(NsGemmArgs& g, hipStream_t st) {
     constexpr bool SYM = PHASE == NS_GRAM || PHASE == NS_POLY;
@@ -1101,6 +1131,14 @@ static int ns_launch(NsGemmArgs& g, hipStream_t st) {
         if (t128 - rest > 192 * ((t128 - rest + 255) / 256) && (even || t128 >= 512)) {
             const int rc = ns_launch_as<128, 1, 2, PHASE, SPLIT>(g, st, rest);
             return rc != MVIT_OK || !rest ? rc : ns_launch_as<64, 2, 2, PHASE, SPLIT>(g, st, rest);
+        }
+        if constexpr (PHASE == NS_GRAM && SPLIT) {
+            const int64_t cuts = std::min<int64_t>(std::min<int64_t>(8, NS_SUMS / t64), longest / 4);
+            if (cuts >= 2 && longest >= 16) {
+                g.cuts = (uint32_t)cuts;
+                const int rc = ns_launch_as<64, 2, 2, NS_PART, SPLIT>(g, st);
+                return rc != MVIT_OK ? rc : ns_launch_as<64, 1, 2, NS_JOIN, SPLIT>(g, st);
+            }
         }
         if (longest >= 8 && t64 <= 256) return ns_launch_as<64, 2, 2, PHASE, SPLIT>(g, st);
     } else {
@@ -1205,7 +1243,8 @@ static int ns_run(const mvit_ns_matrix* mats, int count, const NsCall& k, void* 
         memset(&g, 0, sizeof g);
         l.n = g.count = count - s < NS_MAX ? count - s : NS_MAX;
         l.parts = static_cast<double*>(workspace);
-        l.ws = g.ws = reinterpret_cast<h16*>(static_cast<char*>(workspace) + (int64_t)NS_MAX * NS_PARTS * 8);
+        g.sums = reinterpret_cast<float*>(static_cast<char*>(workspace) + (int64_t)NS_MAX * NS_PARTS * 8);
+        l.ws = g.ws = reinterpret_cast<h16*>(reinterpret_cast<char*>(g.sums) + (split ? NS_SUMS * 16384 : 0));
         l.norm_coef = g.norm_coef = k.norm_coef;
         l.mu = k.mu; l.nesterov = k.nesterov; l.eps = k.eps;
         g.a = k.a; g.b = k.b; g.c = k.c; g.hyper = k.hyper; g.lr = k.lr; g.wd = k.wd;

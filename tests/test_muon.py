@@ -154,6 +154,20 @@ def test_sums_of_every_depth(dtype):
 
 
 @gpu
+def test_sums_in_pieces():
+    """Long sums on few tiles, in single precision: every number of pieces, and a set whose shorter sums leave pieces empty."""
+    for i, (r, c) in enumerate([(20, 2500), (33, 1040), (70, 1100), (130, 1030), (200, 2400), (330, 1000), (450, 1300), (700, 1100), (768, 2304)]):
+        u = gradient(r, c, i)
+        near(orthogonalize(u, dtype=torch.float32), u, True)
+        near(orthogonalize(u.t(), dtype=torch.float32), u.t(), True)
+    us = [gradient(r, c, r) for r, c in ((20, 2500), (20, 30), (200, 500), (1, 1), (64, 64), (7, 1600))]
+    for got, u in zip(orthogonalize(us, dtype=torch.float32), us):
+        near(got, u, True)
+    again = orthogonalize(us, dtype=torch.float32)
+    assert all(torch.equal(a, b) for a, b in zip(again, orthogonalize(us, dtype=torch.float32)))
+
+
+@gpu
 @pytest.mark.parametrize("shapes", [[(2500, 2510)], [(500, 700)] * 5, [(768, 2304), (300, 2304)], [(1500, 1510)] * 3, [(2900, 3000)], [(4010, 1000), (3000, 2900)], [(4130, 4150)]], ids=str)
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 def test_sets_between_the_tile_sizes(shapes, dtype):
