@@ -179,6 +179,17 @@ def check(rc, what=""):
         raise RuntimeError("mvit HIP kernel %s failed: %s (code %d)" % (what, msg, rc))
 
 
+def refuse_tangents(what, *tensors):
+    """A dual tensor (torch.autograd.forward_ad) carries its tangent beside requires_grad; a kernel that fills fresh memory, or its input in
+    place, would drop it, which torch reads as a tangent of zero.  Checked only inside a dual level."""
+    from torch.autograd import forward_ad
+    if forward_ad._current_level < 0:
+        return
+    for t in tensors:
+        if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+            raise RuntimeError("%s has no forward-mode derivative: the tensor carries a tangent" % what)
+
+
 def ptr(t):
     return None if t is None else ctypes.c_void_p(t.data_ptr())
 

@@ -76,7 +76,7 @@ class AxialRotary(object):
         return AxialRotary, (self.head_dim, self.sections, self.base, self.layout)
 
     def __call__(self, x, positions, k=None, k_positions=None):
-        """Turned copies of ``x`` (and ``k``), differentiable.  Tensors [batch, heads, tokens, head_dim], float32 / bfloat16 / float16, any
+        """Turned copies of ``x`` (and ``k``), differentiable in reverse mode (a tensor with a forward-mode tangent is refused).  Tensors [batch, heads, tokens, head_dim], float32 / bfloat16 / float16, any
         strides with contiguous channels (a token-major buffer goes in as its transposed view).  Positions: a TokenGrid, or a tensor
         [tokens, axes] or [batch, tokens, axes] of int32 / int64 / float32 on the same device."""
         xs, ps = self._arguments(x, positions, k, k_positions)
@@ -117,6 +117,7 @@ class AxialRotary(object):
         return xs, ps
 
     def _check(self, t, p):
+        _hip.refuse_tangents("AxialRotary", t, p if isinstance(p, torch.Tensor) else None)
         if t.dim() != 4 or t.shape[3] != self.head_dim:
             raise ValueError("AxialRotary: expected [batch, heads, tokens, %d], got %s" % (self.head_dim, tuple(t.shape)))
         if t.dtype not in (torch.float32, torch.bfloat16, torch.float16):

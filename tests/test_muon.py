@@ -380,3 +380,16 @@ def test_refusals():
     plan.step([None], lr=0.1)
     with pytest.raises(RuntimeError, match="no CPU fallback"):
         plan.step([g], lr=0.1)
+
+
+def test_forward_mode_tangents_are_refused(monkeypatch):
+    from torch.autograd import forward_ad
+    u, w = torch.randn(4, 6), torch.zeros(4, 6)
+    plan = MuonMatrices([w])
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(u, torch.ones_like(u))
+        for call in (lambda: orthogonalize(dual), lambda: orthogonalize([u, dual]), lambda: plan.step([dual], lr=0.1)):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                call()
+        with pytest.raises(RuntimeError, match="no CPU fallback"):
+            orthogonalize(u)

@@ -283,3 +283,23 @@ def test_refusals_on_the_device():
     assert x._version > version
     with pytest.raises(ValueError, match="same memory"):
         rot.rotate_(x, grid, x, grid)
+
+
+def test_forward_mode_tangents_are_refused(monkeypatch):
+    """A dual tensor does not require a gradient, and a kernel's output has no tangent: torch would read zero.  With the launch replaced, on
+    the host."""
+    from torch.autograd import forward_ad
+
+    from aicity_action_amd import rotary
+    rot, grid = AxialRotary(96), TokenGrid((2, 2, 2))
+    monkeypatch.setattr(rotary, "_launch", lambda *a: None)
+    monkeypatch.setattr(torch.Tensor, "is_cuda", True)
+    x, at = torch.zeros(1, 1, 8, 96), torch.zeros(8, 3)
+    assert rot(x, grid).shape == x.shape and rot.rotate_(x, at) is x
+    with forward_ad.dual_level():
+        dual, places = forward_ad.make_dual(x, torch.ones_like(x)), forward_ad.make_dual(at, torch.ones_like(at))
+        for call in (lambda: rot(dual, grid), lambda: rot.rotate_(dual, grid), lambda: rot(x, grid, dual, grid), lambda: rot(x, places),
+                     lambda: rot(dual.transpose(0, 1), grid)):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                call()
+        assert rot(dual.detach(), grid).shape == rot(x, grid).shape == x.shape
