@@ -194,15 +194,15 @@ def _launch(xs, outs, adds, ps, dim, axes, sections, turns, layout, inverse):
 def _leaf_on_one_stream(t):
     """A leaf's gradient node belongs to the stream it was made on and lives as long as any graph of the leaf.  A backward pass that is
     captured into a HIP graph while an eager graph of the same leaf is alive would make the capture wait for a stream outside it, which
-    ends the process when the capture ends: refused here, as far as this operator has seen the leaf."""
+    ends the process when the capture ends: refused here, as far as this operator has seen the leaf.  The first stream that a node is seen on
+    is the one that counts: later calls on others (a warm-up before the capture) find the same node."""
     if not (t.is_leaf and t.requires_grad):
         return None
     node = torch.autograd.graph.get_gradient_edge(t).node
     stream = _raw_stream(t.device.index)
-    if torch.cuda.is_current_stream_capturing() and node.metadata.get("rotary_stream", stream) != stream:
+    if node.metadata.setdefault("rotary_stream", stream) != stream and torch.cuda.is_current_stream_capturing():
         raise RuntimeError("AxialRotary: an eager graph of this leaf tensor is still alive while its backward pass is being captured; "
                            "drop it (its outputs, its loss) before the capture")
-    node.metadata["rotary_stream"] = stream
     return node
 
 

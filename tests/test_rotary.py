@@ -231,6 +231,29 @@ def test_capture_beside_a_living_eager_graph_is_refused(monkeypatch):
     assert rotary._leaf_on_one_stream(x * 2) is None and rotary._leaf_on_one_stream(torch.zeros(1)) is None
 
 
+def test_a_warm_up_on_the_capture_stream_does_not_hide_a_living_eager_graph(monkeypatch):
+    """Eager graph on stream 1, kept; warm-up on stream 2, dropped; capture on stream 2: the node is still stream 1's."""
+    from aicity_action_amd import rotary
+    stream, capturing = [1], [False]
+    monkeypatch.setattr(rotary, "_raw_stream", lambda index: stream[0])
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: capturing[0])
+    x = torch.zeros(3, requires_grad=True)
+
+    def call():
+        node = rotary._leaf_on_one_stream(x)
+        return x * 2, node
+    kept = call()[0]
+    stream[0] = 2
+    for _ in range(2):
+        call()
+    capturing[0] = True
+    with pytest.raises(RuntimeError, match="eager graph"):
+        call()
+    del kept                                     # with the last graph of stream 1 the node goes, and the next one is stream 2's
+    again = call()[0]
+    assert call() and again is not None
+
+
 def test_a_plan_is_copied_and_pickled():
     plan = AxialRotary(40, (8, 12, 20), base=77.0, layout="interleaved")
     for other in (copy.deepcopy(plan), pickle.loads(pickle.dumps(plan))):
