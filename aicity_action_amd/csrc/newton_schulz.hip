@@ -13,7 +13,8 @@
 // others, which five iterations amplify by up to a^5 = 485 -- with X in one fp16 value a rank-8 gradient over 1 % noise came out 4 %
 // wrong, with two 0.04 % (384 x 1536, against 64 bits).  The products' own operands are the high halves: their rounding is that of one
 // iteration and is not amplified (a full-rank gradient comes out 0.17 % wrong, which is their share).  SPLIT computes every product from
-// both halves (high high + high low + low high, three times the matrix work): 1e-6, for results wanted in single precision.
+// both halves (high high + high low + low high, three times the matrix work): 5e-6 to 1e-5, for results wanted in single precision (4e-5 where one
+// direction dominates: a rounding of X_0 is amplified by those 485, in single precision throughout as well).
 //
 // Bound by the matrix cores where matrices are large: 4096 x 4096 takes 1.7 ms = 800 TFLOP/s counting A and A A half (a large library product of
 // this size: 1100), of which B X runs at 890; its LDS reads and LDS-DMA writes keep the LDS busy 1.5 times as long as the products the matrix
@@ -1024,20 +1025,41 @@ static int ns_check(const mvit_ns_matrix* mats, int count) {
     return MVIT_OK;
 }
 
-// What a set is computed with: matrices of at most 32 rows or columns always from pairs -- the rounding of their few entries of A and B does
-// not average out (3 x 2: 0.4 %), and their products are short.  small: every matrix fits one workgroup.
-static void ns_plan(const mvit_ns_matrix* mats, int count, int asked, bool& split, bool& small) {
-    split = asked != 0;
-    small = true;
-    bool tiny = true;
-    for (int i = 0; i < count; ++i) tiny = tiny && (mats[i].rows <= 32 || mats[i].cols <= 32);
-    if (tiny) split = true;
-    for (int i = 0; i < count; ++i) {
-        const mvit_ns_matrix& t = mats[i];
-        const int64_t rs = t.row_stride, cs = t.col_stride, most = (int64_t)1 << 28;
-        small = small && ns_small_bytes(t.rows, t.cols, split) > 0 && rs >= 0 && cs >= 0 && rs < most && cs < most &&
-                (ns_pad32(t.rows) - 1) * rs + (ns_pad32(t.cols) - 1) * cs < most;       // (31-bit byte offsets, padding included)
+// What a matrix is computed with is its own: matrices of at most 32 rows or columns always from pairs -- the rounding of their few entries of A and
+// B does not average out (2 x 7: up to 1.4 % from single fp16 values), and their products are short.  A call that has such matrices beside larger ones and
+// asks for fp16 products therefore runs as two parts, one behind the other in the same workspace; any other call is one part.
+// (18x768, 1x300 and 77x1 beside 130x70, 513x129 and 200x333, a Muon step: 138 us, from single values in one part 99.)
+struct NsPart {
+    const mvit_ns_matrix* mats;
+    int count, only;             // only: -1 all matrices, 0 the larger ones, 1 those of few rows or columns
+    bool split, small;           // small: every matrix of the part fits one workgroup
+    static bool few(const mvit_ns_matrix& t) { return t.rows <= 32 || t.cols <= 32; }
+    NsPart(const mvit_ns_matrix* m, int n, int which, bool pairs) : mats(m), count(n), only(which), split(pairs), small(true) {
+        for (int i = 0; i < count; ++i) {
+            if (!has(i)) continue;
+            const mvit_ns_matrix& t = mats[i];
+            const int64_t rs = t.row_stride, cs = t.col_stride, most = (int64_t)1 << 28;
+            small = small && ns_small_bytes(t.rows, t.cols, split) > 0 && rs >= 0 && cs >= 0 && rs < most && cs < most &&
+                    (ns_pad32(t.rows) - 1) * rs + (ns_pad32(t.cols) - 1) * cs < most;       // (31-bit byte offsets, padding included)
+        }
     }
+    bool has(int i) const { return only < 0 || only == (int)few(mats[i]); }
+    // the next matrices of the part from `from` on, at most `most` of them; `from` moves behind the last one looked at
+    int take(int& from, int most, int* which) const {
+        int n = 0;
+        for (; from < count && n < most; ++from)
+            if (has(from)) which[n++] = from;
+        return n;
+    }
+};
+// calls f(part) for the call's parts in order, until one does not return MVIT_OK
+template <typename F>
+static int ns_parts(const mvit_ns_matrix* mats, int count, int asked, F f) {
+    int few = 0;
+    for (int i = 0; i < count; ++i) few += NsPart::few(mats[i]);
+    if (asked || few == 0 || few == count) return f(NsPart(mats, count, -1, asked || few));
+    const int rc = f(NsPart(mats, count, 1, true));
+    return rc != MVIT_OK ? rc : f(NsPart(mats, count, 0, false));
 }
 
 extern "C" int mvit_ns_matrix_bytes(void) { return (int)sizeof(mvit_ns_matrix); }
@@ -1046,18 +1068,21 @@ extern "C" int mvit_ns_matrix_bytes(void) { return (int)sizeof(mvit_ns_matrix); 
 extern "C" int64_t mvit_newton_schulz_workspace_bytes(const mvit_ns_matrix* mats, int count, int split) {
     const int rc = ns_check(mats, count);
     if (rc != MVIT_OK) return rc;
-    bool pairs, small;
-    ns_plan(mats, count, split, pairs, small);
-    if (small) return 0;
-    split = pairs;
-    int64_t most = 0;
-    for (int s = 0; s < count; s += NS_MAX) {
-        int64_t units = 0;
-        for (int i = s; i < count && i < s + NS_MAX; ++i) units += ns_region_units(mats[i].rows, mats[i].cols, split);
-        if (units > most) most = units;
-    }
-    if (most > 0xffffffffLL) return MVIT_EUNSUPPORTED;
-    return most * 128 + (int64_t)NS_MAX * NS_PARTS * 8 + (split ? NS_SUMS * 16384 : 0);
+    int64_t bytes = 0;
+    const int rc2 = ns_parts(mats, count, split, [&](const NsPart& part) {
+        if (part.small) return (int)MVIT_OK;
+        int64_t most = 0;
+        int which[NS_MAX], n;
+        for (int from = 0; (n = part.take(from, NS_MAX, which)) > 0;) {
+            int64_t units = 0;
+            for (int i = 0; i < n; ++i) units += ns_region_units(mats[which[i]].rows, mats[which[i]].cols, part.split);
+            most = std::max(most, units);
+        }
+        if (most > 0xffffffffLL) return (int)MVIT_EUNSUPPORTED;
+        bytes = std::max(bytes, most * 128 + (int64_t)NS_MAX * NS_PARTS * 8 + (part.split ? NS_SUMS * 16384 : 0));
+        return (int)MVIT_OK;
+    });
+    return rc2 != MVIT_OK ? rc2 : bytes;
 }
 
 // tiles of a launch at a tile side
@@ -1195,17 +1220,17 @@ static int ns_small_launch(const NsSmallArgs& g, int count, int lds, int tiles, 
                        : ns_small_launch_as<PHASE, T, 48 / NS_SMALL_WAVES, false>(g, count, lds, st);
 }
 
-// All matrices small: one launch (of up to 56) does everything.  A set with a larger one takes the launches of the larger one's anyway.
-static int ns_run_small(const mvit_ns_matrix* mats, int count, const NsCall& k, bool split, hipStream_t st) {
-    const bool muon = k.last == NS_MUON;
-    for (int s = 0; s < count; s += NS_SMALL_MAX) {
+// All matrices of a part small: one launch (of up to 56) does everything.  A part with a larger one takes the launches of the larger one's anyway.
+static int ns_run_small(const NsPart& part, const NsCall& k, hipStream_t st) {
+    const bool muon = k.last == NS_MUON, split = part.split;
+    int which[NS_SMALL_MAX], c;
+    for (int from = 0; (c = part.take(from, NS_SMALL_MAX, which)) > 0;) {
         NsSmallArgs g;
         memset(&g, 0, sizeof g);
-        const int c = count - s < NS_SMALL_MAX ? count - s : NS_SMALL_MAX;
         int64_t lds = 0;
         int tiles = 0;
         for (int i = 0; i < c; ++i) {
-            const mvit_ns_matrix& t = mats[s + i];
+            const mvit_ns_matrix& t = part.mats[which[i]];
             g.mat[i] = {t.u, muon ? t.momentum : nullptr, muon ? static_cast<void*>(t.w) : t.out, t.row_stride, t.col_stride, t.rows, t.cols, t.scale, 0};
             lds = std::max(lds, ns_small_bytes(t.rows, t.cols, split));
             tiles = std::max(tiles, ns_pad32(t.rows) / 32 * (ns_pad32(t.cols) / 32));
@@ -1226,22 +1251,16 @@ static int ns_run_small(const mvit_ns_matrix* mats, int count, const NsCall& k, 
     return MVIT_OK;
 }
 
-static int ns_run(const mvit_ns_matrix* mats, int count, const NsCall& k, void* workspace, int64_t bytes, hipStream_t st) {
-    const bool muon = k.last == NS_MUON;
-    const int64_t need = mvit_newton_schulz_workspace_bytes(mats, count, k.split);
-    if (need < 0) return (int)need;
-    if (bytes < need || (need && !workspace) || (reinterpret_cast<uintptr_t>(workspace) & 127) || k.steps < 1) return MVIT_EINVAL;
-    for (int i = 0; i < count; ++i)
-        if (!mats[i].u || (muon ? !mats[i].w || !mats[i].momentum : !mats[i].out)) return MVIT_EINVAL;
-    bool split, small;
-    ns_plan(mats, count, k.split, split, small);
-    if (small) return ns_run_small(mats, count, k, split, st);
-    for (int s = 0; s < count; s += NS_MAX) {
+static int ns_run_tiled(const NsPart& part, const NsCall& k, void* workspace, hipStream_t st) {
+    const bool muon = k.last == NS_MUON, split = part.split;
+    const mvit_ns_matrix* const mats = part.mats;
+    int order[NS_MAX], n;
+    for (int from = 0; (n = part.take(from, NS_MAX, order)) > 0;) {
         NsLoadArgs l;
         NsGemmArgs g;
         memset(&l, 0, sizeof l);
         memset(&g, 0, sizeof g);
-        l.n = g.count = count - s < NS_MAX ? count - s : NS_MAX;
+        l.n = g.count = n;
         l.parts = static_cast<double*>(workspace);
         g.sums = reinterpret_cast<float*>(static_cast<char*>(workspace) + (int64_t)NS_MAX * NS_PARTS * 8);
         l.ws = g.ws = reinterpret_cast<h16*>(reinterpret_cast<char*>(g.sums) + (split ? NS_SUMS * 16384 : 0));
@@ -1249,8 +1268,6 @@ static int ns_run(const mvit_ns_matrix* mats, int count, const NsCall& k, void* 
         l.mu = k.mu; l.nesterov = k.nesterov; l.eps = k.eps;
         g.a = k.a; g.b = k.b; g.c = k.c; g.hyper = k.hyper; g.lr = k.lr; g.wd = k.wd;
         // the matrices with the longest sums first, so that no launch ends on them
-        int order[NS_MAX];
-        for (int i = 0; i < l.n; ++i) order[i] = s + i;
         std::stable_sort(order, order + l.n, [&](int x, int y) { return (int64_t)mats[x].rows + mats[x].cols > (int64_t)mats[y].rows + mats[y].cols; });
         int64_t off = 0, blocks = 0;
         for (int i = 0; i < l.n; ++i) {
@@ -1284,6 +1301,17 @@ static int ns_run(const mvit_ns_matrix* mats, int count, const NsCall& k, void* 
         if (rc != MVIT_OK) return rc;
     }
     return MVIT_OK;
+}
+
+static int ns_run(const mvit_ns_matrix* mats, int count, const NsCall& k, void* workspace, int64_t bytes, hipStream_t st) {
+    const bool muon = k.last == NS_MUON;
+    const int64_t need = mvit_newton_schulz_workspace_bytes(mats, count, k.split);
+    if (need < 0) return (int)need;
+    if (bytes < need || (need && !workspace) || (reinterpret_cast<uintptr_t>(workspace) & 127) || k.steps < 1) return MVIT_EINVAL;
+    for (int i = 0; i < count; ++i)
+        if (!mats[i].u || (muon ? !mats[i].w || !mats[i].momentum : !mats[i].out)) return MVIT_EINVAL;
+    return ns_parts(mats, count, k.split,
+                    [&](const NsPart& part) { return part.small ? ns_run_small(part, k, st) : ns_run_tiled(part, k, workspace, st); });
 }
 
 extern "C" int mvit_newton_schulz(const mvit_ns_matrix* mats, int count, int in_dtype, int out_dtype, float a, float b, float c, int steps,

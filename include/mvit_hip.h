@@ -395,9 +395,10 @@ int mvit_rotary(const mvit_rotary_tensor* tensors, int ntensors, int dim, int ax
  *       w <- w (1 - lr weight_decay) - lr scale NS(update);   w, momentum [rows][cols] contiguous, updated in place.
  *       norm_coef: NULL (f = 1) or mvit_grad_norm's out2 (f = out2[1]; a non-finite norm or factor leaves w and momentum as they are);
  *       hyper: NULL or device memory whose first float is the learning rate (captured steps, as mvit_adamw_step_dev).
- * split 0: products from fp16 operands (result within about 2e-3 of the exact one, 4e-3 for few rows beside larger matrices), 1: from pairs of them (1e-5; three times the work).
- * Sets of matrices with at most 32 rows or columns are always computed from pairs; sets of matrices that each fit a workgroup's LDS (about
- * 48 K elements, smaller side up to 128) are one launch and need no workspace.
+ * split 0: products from fp16 operands (result within 3e-3 of the exact one, relative to its norm, after five steps of the usual coefficients), 1: from pairs
+ * of them (1e-4; three times the work).  Matrices of at most 32 rows or columns are always computed from pairs: beside larger ones they run
+ * by themselves ahead of those.  Matrices that each fit a workgroup's LDS (about 48 K elements, 32 K from pairs, smaller side up to 128) are one launch and
+ * need no workspace.
  * workspace: mvit_newton_schulz_workspace_bytes(mats, count, split) bytes (negative: MVIT_E*), 128-byte aligned, used by this call alone. */
 typedef struct {
     const void* u;

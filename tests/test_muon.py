@@ -393,3 +393,55 @@ def test_forward_mode_tangents_are_refused(monkeypatch):
                 call()
         with pytest.raises(RuntimeError, match="no CPU fallback"):
             orthogonalize(u)
+
+
+# What the documentation promises, as numbers: relative to the result's norm, after five steps of the default coefficients
+FP16_BOUND, PAIRS_BOUND = 3e-3, 1e-4
+
+
+def spectra(r, c, seed):
+    """Flat, falling over noise, one direction alone, eight directions over little noise."""
+    g = torch.Generator().manual_seed(1000 + seed)
+    yield gradient(r, c, seed, 0.0, 1.0)
+    yield gradient(r, c, seed, 2.0, 0.1)
+    yield (torch.randn(r, 1, generator=g) @ torch.randn(1, c, generator=g)).to(DEV)
+    yield (torch.randn(r, 8, generator=g) @ torch.randn(8, c, generator=g) + 1e-4 * torch.randn(r, c, generator=g)).to(DEV)
+
+
+def off(got, u):
+    want = definition(u)
+    return ((got.double() - want).norm() / want.norm()).item()
+
+
+@gpu
+@pytest.mark.parametrize("shape", [(33, 33), (40, 60), (33, 700), (100, 64), (96, 288), (300, 200), (130, 1500)], ids=str)
+def test_documented_bounds(shape):
+    """The roundings' model (``rounded``) over 600 updates per shape leaves 2.0e-3 at 33 rows and less behind; one direction alone 4.3e-5 from
+    pairs.  The fp32 sums add under 2e-5 (see ``near``)."""
+    for seed in range(4):
+        for u in spectra(*shape, seed):
+            assert off(orthogonalize(u, dtype=torch.float32, arithmetic="fp16"), u) <= FP16_BOUND
+            assert off(orthogonalize(u, dtype=torch.float32), u) <= PAIRS_BOUND
+
+
+FEW = [(1, 1), (1, 5), (3, 2), (2, 7), (7, 1), (5, 40), (16, 16), (32, 32), (20, 900), (768, 18), (32, 33)]
+
+
+@gpu
+@pytest.mark.parametrize("beside", [(40, 60), (300, 400), (20, 2500)], ids=str)
+def test_few_rows_beside_larger_matrices(beside):
+    """A matrix of few rows or columns is as exact beside a larger one (in one workgroup, in tiles) as alone, and so is its weight's step."""
+    for seed in range(4):
+        us = [u for shape in FEW for u in spectra(*shape, seed)]
+        larger = gradient(*beside, seed)
+        got = orthogonalize(us[:20] + [larger] + us[20:], dtype=torch.float32, arithmetic="fp16")
+        assert off(got.pop(20), larger) <= FP16_BOUND
+        worst = max(off(g, u) for g, u in zip(got, us))
+        assert worst <= PAIRS_BOUND, worst
+        # momenta of zero without decay or a weight to add to: the step is the orthogonalised gradient itself
+        ws = [torch.zeros_like(u) for u in us + [larger]]
+        MuonMatrices(ws, rms=1.0).step(us + [larger], lr=1.0)
+        stepped = lambda w, u: off(-w / math.sqrt(max(w.shape)), 0.05 * 1.95 * u.double())  # noqa: E731
+        worst = max(stepped(w, u) for w, u in zip(ws, us))
+        assert worst <= PAIRS_BOUND, worst
+        assert stepped(ws[-1], larger) <= FP16_BOUND
