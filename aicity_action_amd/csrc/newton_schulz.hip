@@ -113,6 +113,18 @@ __device__ __forceinline__ bool ns_bad(const float* norm_coef) {       // (bit t
                          ((__float_as_uint(norm_coef[1]) & 0x7f800000u) == 0x7f800000u));
 }
 
+// 2^12 / (norm + eps) as a mantissa and a power of two, applied one after the other: the factor itself leaves the range of fp32 for norms below
+// 1e-35 and its precision for norms above 1e38.  An update of zeros stays one, however small eps is.
+struct NsFactor {
+    float mant;
+    int exp;
+    __device__ __forceinline__ float operator()(float v) const { return __builtin_ldexpf(v, exp) * mant; }
+};
+__device__ __forceinline__ NsFactor ns_factor(double squares, float eps) {
+    const double f = squares == 0.0 ? 0.0 : (double)NS_S / (sqrt(squares) + (double)eps);
+    return {(float)__builtin_amdgcn_frexp_mant(f), __builtin_amdgcn_frexp_exp(f)};
+}
+
 template <typename T> __device__ __forceinline__ float ns_ld(const T* p) { return ActIO<T>::load(p); }
 
 // ---- 1. squares, and the momentum -------------------------------------------------------------------------------------------------
@@ -229,7 +241,7 @@ __global__ __launch_bounds__(256) void ns_start_kernel(const NsLoadArgs a) {
     const int tid = threadIdx.x;
     __shared__ float sh[64][65];                                    // [row of U][column of U] within the tile
     __shared__ double red[4];
-    __shared__ float s_inv;
+    __shared__ NsFactor s_f;
     {
         const int64_t tiles = (int64_t)((t.rows + 63) / 64) * ((t.cols + 63) / 64);
         const int nparts = (int)(tiles < NS_PARTS ? tiles : NS_PARTS);
@@ -238,7 +250,7 @@ __global__ __launch_bounds__(256) void ns_start_kernel(const NsLoadArgs a) {
         for (int off = 32; off >= 1; off >>= 1) s += __shfl_xor(s, off, 64);
         if ((tid & 63) == 0) red[tid >> 6] = s;
         __syncthreads();
-        if (tid == 0) s_inv = (float)(1.0 / (sqrt((red[0] + red[1]) + (red[2] + red[3])) + (double)a.eps));
+        if (tid == 0) s_f = ns_factor((red[0] + red[1]) + (red[2] + red[3]), a.eps);
     }
     const float coef = a.norm_coef ? a.norm_coef[1] : 1.0f;
     const T* u = static_cast<const T*>(t.u);
@@ -287,7 +299,7 @@ __global__ __launch_bounds__(256) void ns_start_kernel(const NsLoadArgs a) {
         }
     }
     __syncthreads();
-    const float f = s_inv * NS_S;
+    const NsFactor f = s_f;
     const NsRegion g(a.ws, t.off, m, n);
     // eight consecutive values of a row of X per thread
 #pragma unroll
@@ -296,7 +308,7 @@ __global__ __launch_bounds__(256) void ns_start_kernel(const NsLoadArgs a) {
         h16x8 hi, lo;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            float v = (tall ? sh[ch + j][row] : sh[row][ch + j]) * f;           // X[ti*64 + row][tj*64 + ch + j]
+            float v = f(tall ? sh[ch + j][row] : sh[row][ch + j]);              // X[ti*64 + row][tj*64 + ch + j]
             ns_pin(v);
             hi[j] = (h16)v;
             lo[j] = (h16)(v - (float)hi[j]);
@@ -850,11 +862,11 @@ __device__ __forceinline__ void ns_small_body(const NsSmallArgs& a, const NsSmal
         double s = 0.0;
 #pragma unroll
         for (int k = 0; k < NS_SMALL_WAVES; ++k) s += red[k];
-        const float f = (float)(1.0 / (sqrt(s) + (double)a.eps)) * NS_S;
+        const NsFactor f = ns_factor(s, a.eps);
 #pragma unroll
         for (int k = 0; k < TPW; ++k)
 #pragma unroll
-            for (int e = 0; e < 16; ++e) x[k][e] *= f;
+            for (int e = 0; e < 16; ++e) x[k][e] = f(x[k][e]);
     }
 
     const std::true_type down{};

@@ -445,3 +445,20 @@ def test_few_rows_beside_larger_matrices(beside):
         worst = max(stepped(w, u) for w, u in zip(ws, us))
         assert worst <= PAIRS_BOUND, worst
         assert stepped(ws[-1], larger) <= FP16_BOUND
+
+
+@gpu
+@pytest.mark.parametrize("shape", [(50, 70), (300, 400)], ids=str)
+def test_factors_outside_the_range_of_single_precision(shape):
+    """1 / (norm + eps) is no fp32 number where eps and the update are small, and less than one where the update is large."""
+    zero = torch.zeros(shape, device=DEV)
+    for eps in (1e-30, 1e-36, 1e-44, 1e-60):                     # (the last is zero in single precision)
+        assert torch.equal(orthogonalize(zero, eps=eps, dtype=torch.float32), zero)
+        w = torch.ones(shape, device=DEV)
+        MuonMatrices([w], eps=eps).step([zero], lr=0.5)
+        assert (w == 1.0).all()
+    for scale, eps in ((1e-30, 1e-44), (1e-37, 1e-44), (1e-37, 1e-60), (5e37, 1e-7)):
+        u = gradient(*shape, 4, 0.0, 0.2)
+        u = u / u.abs().max() * (5 * scale)
+        want = definition(u, eps=0.0)                            # (eps is below 1e-8 of every norm here)
+        assert ((orthogonalize(u, eps=eps, dtype=torch.float32).double() - want).norm() / want.norm()).item() <= PAIRS_BOUND
