@@ -4,6 +4,7 @@
 each weight by its orthogonalised momentum, all matrices in the same launches whatever their sizes (one for a set of small ones, else 17 or a
 few more).  ``solver.construct_optimizer`` builds a train step on it (``SOLVER.OPTIMIZING_METHOD muon``); the reference's own methods are
 those of slowfast/models/optimizer.py:140-206.  Everything runs on the tensors' device and its current stream; there is no CPU fallback."""
+import bisect
 import math
 
 import numpy as np
@@ -91,6 +92,18 @@ def orthogonalize(update, steps=5, coefficients=QUINTIC, eps=1e-7, dtype=torch.b
     return outs if many else outs[0]
 
 
+def _apart(written, read=()):
+    """Spans (first byte, byte behind the last one): what a step writes must not overlap, nor what it reads begin or end in it."""
+    written = sorted(written)
+    if any(a[1] > b[0] for a, b in zip(written, written[1:])):
+        raise ValueError("MuonMatrices: parameters and momenta must not share memory (the same tensor twice?)")
+    ends = [b for _, b in written]
+    for a, b in read:
+        i = bisect.bisect_right(ends, a)                 # the first span that ends behind the gradient's beginning
+        if i < len(ends) and written[i][0] < b:
+            raise ValueError("MuonMatrices.step: a gradient shares its memory with a parameter or a momentum")
+
+
 class MuonMatrices(object):
     """A set of weight matrices and their momenta, stepped together.
 
@@ -117,9 +130,7 @@ class MuonMatrices(object):
             self._check_matrix(m, "momentum")
             if m.shape != p.shape:
                 raise ValueError("MuonMatrices: a momentum of shape %s for a parameter of shape %s" % (tuple(m.shape), tuple(p.shape)))
-        spans = sorted((t.data_ptr(), t.data_ptr() + 4 * t.numel()) for t in self.params + self.momenta)
-        if any(a[1] > b[0] for a, b in zip(spans, spans[1:])):
-            raise ValueError("MuonMatrices: parameters and momenta must not share memory (the same tensor twice?)")
+        _apart((t.data_ptr(), t.data_ptr() + 4 * t.numel()) for t in self.params + self.momenta)
         self.momentum, self.nesterov, self.weight_decay, self.rms = float(momentum), bool(nesterov), float(weight_decay), float(rms)
         self.steps, self.coefficients, self.eps, self.arithmetic = int(steps), tuple(float(c) for c in coefficients), float(eps), arithmetic
 
@@ -152,7 +163,8 @@ class MuonMatrices(object):
         for p, m, g in zip(self.params, self.momenta, grads):
             if g is None:
                 continue
-            if p.dtype != torch.float32 or p.device != device or not (p.is_contiguous() and m.is_contiguous()) or m.shape != p.shape:
+            if (p.dtype != torch.float32 or m.dtype != torch.float32 or p.device != device or m.device != device or m.shape != p.shape
+                    or not (p.is_contiguous() and m.is_contiguous())):
                 raise ValueError("MuonMatrices.step: a parameter or its momentum has changed its type, device, shape or strides")
             if g.shape != p.shape or g.dtype != torch.float32 or g.device != device:
                 raise ValueError("MuonMatrices.step: a %s gradient of shape %s on %s for a float32 parameter of shape %s on %s"
@@ -162,8 +174,8 @@ class MuonMatrices(object):
             touched += [p, m]
         if not rows:
             return
-        if {r[0] for r in rows} & {x for r in rows for x in r[1:3]}:
-            raise ValueError("MuonMatrices.step: a gradient shares its memory with a parameter or a momentum")
+        _apart([(at, at + 4 * r * c) for _, p, m, _, _, _, r, c, _, _ in rows for at in (p, m)],
+               [(g, g + 4 * (1 + (r - 1) * rs + (c - 1) * cs)) for g, _, _, _, rs, cs, r, c, _, _ in rows])
         if not self.params[0].is_cuda:
             raise RuntimeError("MuonMatrices needs its parameters on a gfx950 device; there is no CPU fallback")
         rec = np.array(rows, dtype=_REC)

@@ -462,3 +462,28 @@ def test_factors_outside_the_range_of_single_precision(shape):
         u = u / u.abs().max() * (5 * scale)
         want = definition(u, eps=0.0)                            # (eps is below 1e-8 of every norm here)
         assert ((orthogonalize(u, eps=eps, dtype=torch.float32).double() - want).norm() / want.norm()).item() <= PAIRS_BOUND
+
+
+def test_gradients_that_overlap_what_a_step_writes_are_refused():
+    flat = torch.zeros(100)
+    w, far = flat[10:34].view(4, 6), torch.zeros(4, 6)
+    plan = MuonMatrices([w], [flat[40:64].view(4, 6)])
+    for first in (0, 11, 33, 39, 63):                      # ends or begins inside the weight or the momentum, or lies across one
+        with pytest.raises(ValueError, match="shares its memory"):
+            plan.step([flat.as_strided((4, 6), (6, 1), first)], lr=0.1)
+    with pytest.raises(ValueError, match="shares its memory"):
+        plan.step([flat.as_strided((4, 6), (1, 16), 0)], lr=0.1)
+    for g in (flat[64:88].view(4, 6), flat[66:90].view(6, 4).t(), far, far[:1].expand(4, 6)):
+        with pytest.raises(RuntimeError, match="no CPU fallback"):
+            plan.step([g], lr=0.1)
+    both = MuonMatrices([torch.zeros(4, 6), torch.zeros(4, 6)])
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        both.step([far, far], lr=0.1)                      # (one gradient for two weights is only read)
+    both.params[1].data = both.params[0].data              # moved onto each other since the set was made
+    with pytest.raises(ValueError, match="share memory"):
+        both.step([far, far], lr=0.1)
+    for replaced in (torch.zeros(4, 6, dtype=torch.float64), torch.zeros(4, 6, device="meta"), torch.zeros(6, 4).t()):
+        other = MuonMatrices([torch.zeros(4, 6)])
+        other.momenta[0] = replaced
+        with pytest.raises(ValueError, match="changed its"):
+            other.step([far], lr=0.1)
