@@ -14,6 +14,7 @@ LIB_PATH_F16 = os.environ.get("MVIT_HIP_LIB_F16") or os.path.join(_HERE, "lib", 
 CSRC = os.path.join(_HERE, "csrc")
 
 F32, BF16 = 0, 1
+EINVAL = -1
 EPI_BIAS, EPI_GELU, EPI_RESIDUAL = 1, 2, 4
 
 _lib = None
@@ -88,6 +89,7 @@ _SIGS = {
     "mvit_adamw_step": (c_i, [c_p, c_i, c_p, c_f, c_f, c_f, c_f, c_i, c_p]),
     "mvit_adamw_step_dev": (c_i, [c_p, c_i, c_p, c_p, c_f, c_f, c_f, c_p]),
     "mvit_rotary_tensor_bytes": (c_i, []),
+    "mvit_rotary_overlap": (c_i, [c_p, c_i, c_i, c_i]),
     "mvit_rotary": (c_i, [c_p, c_i, c_i, c_i, c_p, c_p, c_i, c_i, c_i, c_p]),
     "mvit_ns_matrix_bytes": (c_i, []),
     "mvit_newton_schulz_workspace_bytes": (c_l, [c_p, c_i, c_i]),

@@ -235,6 +235,111 @@ static void rotary_launch(const RotaryArgs& a, uint32_t blocks, int layout, hipS
     else hipLaunchKernelGGL((rotary_kernel<T, V, false>), dim3(blocks), dim3(256), 0, st, a);
 }
 
+// ---- host side: whether two tensors [B][H][L][dim] share an element ------------------------------------------------------------------------
+// Their extents may interleave (heads of one fused buffer), so the question is whether indices exist whose addresses are equal: a sum of strides
+// times bounded whole numbers, searched from the largest stride down within what the smaller ones can still make up.
+struct RotView {
+    int64_t at;                    // address in elements
+    int64_t n[3], s[3], dim;
+    bool same(const RotView& o) const {
+        for (int d = 0; d < 3; ++d)
+            if (n[d] != o.n[d] || (n[d] > 1 && s[d] != o.s[d])) return false;
+        return at == o.at;
+    }
+};
+struct RotSum {
+    enum { MOST = 7 };
+    int64_t s[MOST], lo[MOST], hi[MOST], rest_lo[MOST + 1], rest_hi[MOST + 1];   // stride, least and most it is taken; what those behind make up
+    int n = 0, budget = 0;
+    void add(int64_t stride, int64_t low, int64_t high) {
+        if (stride < 0) { stride = -stride; std::swap(low, high); low = -low; high = -high; }
+        if (stride == 0) return;
+        int i = 0;
+        while (i < n && s[i] != stride) ++i;
+        if (i == n) { s[n] = stride; lo[n] = hi[n] = 0; ++n; }
+        lo[i] += low;
+        hi[i] += high;
+    }
+    // may answer true where the budget ends, never false where there is a way
+    bool makes(int64_t sum) {
+        for (int i = 1; i < n; ++i)                      // largest stride first
+            for (int j = i; j > 0 && s[j] > s[j - 1]; --j) { std::swap(s[j], s[j - 1]); std::swap(lo[j], lo[j - 1]); std::swap(hi[j], hi[j - 1]); }
+        rest_lo[n] = rest_hi[n] = 0;
+        for (int i = n - 1; i >= 0; --i) { rest_lo[i] = rest_lo[i + 1] + s[i] * lo[i]; rest_hi[i] = rest_hi[i + 1] + s[i] * hi[i]; }
+        budget = 2000;
+        return from(0, sum);
+    }
+    static int64_t down(int64_t a, int64_t b) { return a / b - (a % b != 0 && a < 0); }      // floor of a / b, b > 0
+    bool from(int i, int64_t left) {
+        if (left < rest_lo[i] || left > rest_hi[i]) return false;
+        if (i == n || --budget < 0) return true;
+        const int64_t a = std::max(lo[i], -down(rest_hi[i + 1] - left, s[i])), b = std::min(hi[i], down(left - rest_lo[i + 1], s[i]));
+        for (int64_t k = a; k <= b; ++k)
+            if (from(i + 1, left - k * s[i])) return true;
+        return false;
+    }
+};
+static bool rot_meet(const RotView& x, const RotView& y) {
+    RotSum t;
+    t.add(1, 1 - y.dim, x.dim - 1);
+    for (int d = 0; d < 3; ++d) {
+        t.add(x.s[d], 0, x.n[d] - 1);
+        t.add(y.s[d], 1 - y.n[d], 0);
+    }
+    if (!t.makes(y.at - x.at)) return false;
+    if (t.budget >= 0) return true;
+    // Too many ways to try (every fourth token of a buffer beside all of them).  With the strides that are multiples of one of them counted as
+    // that one, more sums can be made, not fewer: if there is no way then, there is none.
+    for (int g = 0; g < t.n; ++g) {
+        RotSum m;
+        for (int i = 0; i < t.n; ++i) {
+            const int64_t f = t.s[g] > 1 && t.s[i] % t.s[g] == 0 ? t.s[i] / t.s[g] : 1;
+            m.add(t.s[i] / f, t.lo[i] * f, t.hi[i] * f);
+        }
+        if (!m.makes(y.at - x.at)) return false;
+    }
+    return true;
+}
+// two indices of one tensor name one element: not where every stride spans all that lies within it
+static bool rot_meets_itself(const RotView& v) {
+    int order[3] = {0, 1, 2};
+    std::sort(order, order + 3, [&](int i, int j) { return std::abs(v.s[i]) < std::abs(v.s[j]); });
+    int64_t extent = v.dim;
+    for (int d : order) {
+        if (v.n[d] == 1) continue;
+        if (std::abs(v.s[d]) < extent) return true;
+        extent += (v.n[d] - 1) * std::abs(v.s[d]);
+    }
+    return false;
+}
+
+extern "C" int mvit_rotary_overlap(const mvit_rotary_tensor* tensors, int ntensors, int dim, int act_dtype) {
+    if (!tensors || ntensors < 1 || ntensors > 2 || dim < 1) return MVIT_EINVAL;
+    if (act_dtype != MVIT_F32 && act_dtype != MVIT_BF16) return MVIT_EDTYPE;
+    const int64_t itemsize = act_dtype == MVIT_F32 ? 4 : 2;
+    RotView v[2][3];               // x, y, add
+    bool there[2][3] = {};
+    for (int i = 0; i < ntensors; ++i) {
+        const mvit_rotary_tensor& t = tensors[i];
+        if (t.B <= 0 || t.H <= 0 || t.L <= 0) continue;
+        const void* at[3] = {t.x, t.y, t.add};
+        const int64_t* strides[3] = {t.xs, t.ys, t.as};
+        for (int k = 0; k < 3; ++k)
+            if (at[k]) {
+                there[i][k] = true;
+                v[i][k] = {(int64_t)(reinterpret_cast<uintptr_t>(at[k]) / itemsize), {t.B, t.H, t.L}, {strides[k][0], strides[k][1], strides[k][2]}, dim};
+            }
+    }
+    for (int i = 0; i < ntensors; ++i) {
+        if (!there[i][1]) continue;
+        if (rot_meets_itself(v[i][1])) return 1;
+        for (int j = 0; j < ntensors; ++j)
+            for (int k = 0; k < 3; ++k)
+                if (there[j][k] && !(i == j && (k == 1 || v[i][1].same(v[j][k]))) && rot_meet(v[i][1], v[j][k])) return 1;
+    }
+    return 0;
+}
+
 extern "C" int mvit_rotary_tensor_bytes(void) { return (int)sizeof(mvit_rotary_tensor); }
 
 extern "C" int mvit_rotary(const mvit_rotary_tensor* tensors, int ntensors, int dim, int axes, const int* sections, const double* turns,
@@ -292,6 +397,7 @@ extern "C" int mvit_rotary(const mvit_rotary_tensor* tensors, int ntensors, int 
                 if (extent[d] > 1) narrow((uint64_t)(strides[k][d] < 0 ? -strides[k][d] : strides[k][d]));
         }
     }
+    if (mvit_rotary_overlap(tensors, ntensors, dim, act_dtype)) return MVIT_EINVAL;
     a.tasks = a.pairs / (int)fit + (dim - channels + 2 * (int)fit - 1) / (2 * (int)fit);
     // Rows per thread, so that a turn and its addresses serve several: until a thread moves 64 bytes each way (two rows of 16-byte vectors, at
     // most 8), as long as that leaves 1024 workgroups, four for each of the 256 CUs.  (1, 2, 4, 8 rows: one bf16 head on 8 x 112 x 112,

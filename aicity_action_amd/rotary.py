@@ -89,16 +89,14 @@ class AxialRotary(object):
         return tuple(ys) if k is not None else ys[0]
 
     def rotate_(self, x, positions, k=None, k_positions=None, inverse=False):
-        """The same in place, without a graph (serving: queries and keys are turned where they stand;
-        they must not overlap each other)."""
+        """The same in place, without a graph (serving: queries and keys are turned where they stand, heads of one fused buffer for instance;
+        they must not overlap each other, nor a tensor itself)."""
         xs, ps = self._arguments(x, positions, k, k_positions)
         for t in xs:
             if torch.is_grad_enabled() and t.requires_grad:
                 raise RuntimeError("AxialRotary.rotate_: the tensor requires a gradient; use the plan's call, which makes a turned copy")
             if any(s == 0 and n > 1 for s, n in zip(t.stride(), t.shape)):
                 raise ValueError("AxialRotary.rotate_: an expanded tensor (stride 0) cannot be turned in place")
-        if k is not None and x.numel() and x.data_ptr() == k.data_ptr():
-            raise ValueError("AxialRotary.rotate_: x and k are the same memory; they must not overlap")
         self.turn(xs, ps, outs=xs, inverse=inverse)
         for t in xs:                    # written behind torch's back
             torch.autograd.graph.increment_version(t)
@@ -166,8 +164,9 @@ def _raw_stream(index):
     return torch._C._cuda_getCurrentRawStream(index)
 
 
-def _launch(xs, outs, adds, ps, dim, axes, sections, turns, layout, inverse):
-    x, rec = xs[0], b""
+def _records(xs, outs, adds, ps):
+    """The array of mvit_rotary_tensor that the C entries take."""
+    rec = b""
     for i, (t, y, p) in enumerate(zip(xs, outs, ps)):
         add = adds[i] if adds is not None else None
         place, kind, steps, grid = 0, 0, (0, 0, 0), _NO_GRID
@@ -179,6 +178,11 @@ def _launch(xs, outs, adds, ps, dim, axes, sections, turns, layout, inverse):
         B, H, L, _ = t.shape
         rec += _RECORD.pack(t.data_ptr(), y.data_ptr(), add.data_ptr() if add is not None else 0, place, *t.stride()[:3], *y.stride()[:3],
                             *(add.stride()[:3] if add is not None else (0, 0, 0)), *steps, L, B, H, kind, *grid)
+    return rec
+
+
+def _launch(xs, outs, adds, ps, dim, axes, sections, turns, layout, inverse):
+    x, rec = xs[0], _records(xs, outs, adds, ps)
     lib = _hip.lib("fp16" if x.dtype == torch.float16 else "bf16")
     act = _hip.F32 if x.dtype == torch.float32 else _hip.BF16
     args = (rec, len(xs), dim, axes, sections, turns, layout, 1 if inverse else 0, act)
@@ -188,6 +192,8 @@ def _launch(xs, outs, adds, ps, dim, axes, sections, turns, layout, inverse):
     else:
         with torch.cuda.device(at):
             rc = lib.mvit_rotary(*args, _raw_stream(at))
+    if rc == _hip.EINVAL and outs is xs:        # (everything else has been checked)
+        raise ValueError("AxialRotary.rotate_: the tensors are the same memory in part, or one of them shares elements with itself; they must not overlap")
     _hip.check(rc, "rotary")
 
 

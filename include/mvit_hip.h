@@ -360,7 +360,7 @@ int mvit_cast_transpose_multi(const void* desc_table, int ntensors, int total_ti
 /* Rotary positions with up to four axes (csrc/rotary.hip): y = rot(x) (+ add), every head's channels cut into one section per axis.
  *   tensors: HOST array of 1 or 2 records (a query and a key tensor share one launch); x, y, add are act-typed device tensors
  *            [B][H][L][dim] with the element strides of batch, head and token given and channels contiguous; add may be NULL; y may be x
- *            itself (same strides), any other overlap is the caller's error.
+ *            or add itself (same strides); any other memory that y shares, within itself or with a tensor of the call, is MVIT_EINVAL.
  *   places:  pos = NULL: token l stands on the grid grid[0] x ... (last axis fastest, product = L) at origin[n] + step[n] * index;
  *            else device places [B][L][axes] of pos_type with element strides ps (0 = shared by the batch).
  *   sections: HOST, channels per axis, even, sum <= dim (the rest passes through); axes may be 0 (y = x + add).
@@ -383,6 +383,9 @@ typedef struct {
     double origin[4], step[4];
 } mvit_rotary_tensor;
 int mvit_rotary_tensor_bytes(void);
+/* 1 where mvit_rotary would find that overlap, 0 where there is none.  Views that interleave (heads of one fused buffer) are told apart; where a search
+ * of 2000 steps cannot, the answer is 1. */
+int mvit_rotary_overlap(const mvit_rotary_tensor* tensors, int ntensors, int dim, int act_dtype);
 int mvit_rotary(const mvit_rotary_tensor* tensors, int ntensors, int dim, int axes, const int* sections, const double* turns, int layout,
                 int inverse, int act_dtype, void* stream);
 

@@ -2,6 +2,7 @@
 import copy
 import math
 import pickle
+import random
 
 import pytest
 import torch
@@ -326,3 +327,70 @@ def test_forward_mode_tangents_are_refused(monkeypatch):
             with pytest.raises(RuntimeError, match="forward-mode"):
                 call()
         assert rot(dual.detach(), grid).shape == rot(x, grid).shape == x.shape
+
+
+def _overlap(xs, outs=None, adds=None):
+    from aicity_action_amd import _hip, rotary
+    outs = xs if outs is None else outs
+    rec = rotary._records(xs, outs, adds, [TokenGrid((t.shape[2], 1, 1)) if t.shape[2] else torch.zeros(0, 3) for t in xs])
+    return _hip.lib().mvit_rotary_overlap(rec, len(xs), xs[0].shape[3], _hip.F32 if xs[0].dtype == torch.float32 else _hip.BF16)
+
+
+def test_overlap_of_views_against_their_elements():
+    """Random views of one buffer: an overlap is always found, and none is seen where there is none."""
+    rng, flat = random.Random(1), torch.zeros(4000)
+
+    def view(dim):
+        sizes = [rng.choice([1, 1, 2, 3, 4]) for _ in range(3)]
+        unit = dim if rng.random() < 0.6 else 1
+        strides = [unit * rng.choice([1, 2, 3, 4, 6, 12, 24]) for _ in range(3)]
+        return flat.as_strided(sizes + [dim], strides + [1], rng.randint(0, 30) * unit)
+
+    def elements(t):
+        return torch.arange(4000).as_strided(t.shape, t.stride(), t.storage_offset()).flatten().tolist()
+    seen = [0, 0]
+    for _ in range(3000):
+        dim = rng.choice([2, 4, 8])
+        x, k = view(dim), view(dim)
+        a, b = elements(x), elements(k)
+        if len(set(a)) < len(a) or len(set(b)) < len(b):
+            assert _overlap([x, k]) == 1
+            continue
+        want = int(bool(set(a) & set(b)))
+        nested = all(_overlap([t]) == 0 for t in (x, k))     # (strides that neither nest nor collide count as a collision)
+        assert _overlap([x, k]) == (want if nested else 1)
+        seen[want] += nested
+    assert min(seen) > 100
+    # written, read, added
+    x, y, z = flat[:96].view(1, 2, 6, 8), flat[96:192].view(1, 2, 6, 8), flat[8:104].view(1, 2, 6, 8)
+    assert _overlap([x], [y]) == 0 and _overlap([x], [x], [x]) == 0 and _overlap([x], [y], [z]) == 1 and _overlap([x], [z]) == 1
+    assert _overlap([x, y], [y, x]) == 1 and _overlap([x, x], [y, flat[192:288].view(1, 2, 6, 8)]) == 0
+
+
+def test_heads_of_a_fused_buffer_do_not_overlap():
+    for dtype in (torch.float32, torch.bfloat16):
+        buf = torch.zeros(4, 784, 12, 96, dtype=dtype)
+        q, k = buf[:, :, :4].transpose(1, 2), buf[:, :, 4:8].transpose(1, 2)
+        assert _overlap([q, k]) == 0 and _overlap([q, buf[:, :, 3:5].transpose(1, 2)]) == 1
+        assert _overlap([q, k[:, :, ::4]]) == 0 and _overlap([q, q[:, 3:, 5::4]]) == 1     # every fourth token
+        assert _overlap([q[:2], k[1:]]) == 0 and _overlap([q[:2], q[2:]]) == 0 and _overlap([q[:2], q[1:]]) == 1
+        assert _overlap([q[..., :48], q[..., 48:]]) == 0 and _overlap([q[..., :50], q[..., 46:]]) == 1
+        assert _overlap([q[:, :0], q]) == 0 and _overlap([q[:, :, :, :2].expand(4, 4, 784, 2)]) == 0
+        assert _overlap([q[:, :1].expand(4, 3, 784, 96)]) == 1 and _overlap([buf.as_strided((1, 1, 9, 96), (1, 1, 95, 1))]) == 1
+
+
+@gpu
+def test_in_place_turns_of_overlapping_views_are_refused():
+    rot, grid = AxialRotary(96), TokenGrid((2, 2, 2))
+    buf = randn((2, 8, 6, 96), torch.bfloat16, 4)
+    before = buf.clone()
+    views = lambda b: (b[:, :, :3].transpose(1, 2), b[:, :, 2:4].transpose(1, 2), b[:, :, 3:5].transpose(1, 2))  # noqa: E731
+    q, near, k = views(buf)
+    with pytest.raises(ValueError, match="must not overlap"):
+        rot.rotate_(q, grid, near, grid)
+    with pytest.raises(ValueError, match="must not overlap"):
+        rot.rotate_(buf.as_strided((1, 1, 8, 96), (768, 768, 64, 1)), grid)
+    assert torch.equal(buf, before)
+    want = [rot(t, grid) for t in views(before)]
+    rot.rotate_(q, grid, k, grid)
+    assert torch.equal(q, want[0]) and torch.equal(k, want[2]) and torch.equal(buf[:, :, 5:], before[:, :, 5:])
