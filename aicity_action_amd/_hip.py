@@ -183,10 +183,8 @@ def check(rc, what=""):
 
 def refuse_tangents(what, *tensors):
     """A dual tensor (torch.autograd.forward_ad) carries its tangent beside requires_grad; a kernel that fills fresh memory, or its input in
-    place, would drop it, which torch reads as a tangent of zero.  Checked only inside a dual level."""
+    place, would drop it, which torch reads as a tangent of zero."""
     from torch.autograd import forward_ad
-    if forward_ad._current_level < 0:
-        return
     for t in tensors:
         if t is not None and forward_ad.unpack_dual(t).tangent is not None:
             raise RuntimeError("%s has no forward-mode derivative: the tensor carries a tangent" % what)

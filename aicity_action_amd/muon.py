@@ -9,6 +9,7 @@ import math
 
 import numpy as np
 import torch
+from torch.autograd import forward_ad
 
 from . import _hip
 
@@ -63,7 +64,8 @@ def orthogonalize(update, steps=5, coefficients=QUINTIC, eps=1e-7, dtype=torch.b
             raise ValueError("orthogonalize: all updates must have one dtype and one device")
         if t.requires_grad and torch.is_grad_enabled():
             raise RuntimeError("orthogonalize has no backward pass: call it under torch.no_grad() or on detached updates")
-    _hip.refuse_tangents("orthogonalize", *ts)
+    if forward_ad._current_level >= 0:
+        _hip.refuse_tangents("orthogonalize", *ts)
     if not ts[0].is_cuda:
         raise RuntimeError("orthogonalize needs its updates on a gfx950 device; there is no CPU fallback")
     if ts[0].dtype != torch.float32 and dtype != torch.float32 and ts[0].dtype != dtype:
@@ -159,7 +161,8 @@ class MuonMatrices(object):
         for t, n, what in ((norm_coef, 2, "norm_coef"), (hyper, 1, "hyper")):
             if t is not None and (t.dtype != torch.float32 or t.numel() < n or not t.is_contiguous() or t.device != device):
                 raise ValueError("MuonMatrices.step: %s must be %d contiguous float32 values or more on %s" % (what, n, device))
-        _hip.refuse_tangents("MuonMatrices.step", norm_coef, hyper, *self.params, *self.momenta, *grads)
+        if forward_ad._current_level >= 0:
+            _hip.refuse_tangents("MuonMatrices.step", norm_coef, hyper, *self.params, *self.momenta, *grads)
         for p, m, g in zip(self.params, self.momenta, grads):
             if g is None:
                 continue

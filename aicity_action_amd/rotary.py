@@ -16,6 +16,7 @@ import math
 import struct
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _hip
 
@@ -115,7 +116,8 @@ class AxialRotary(object):
         return xs, ps
 
     def _check(self, t, p):
-        _hip.refuse_tangents("AxialRotary", t, p if isinstance(p, torch.Tensor) else None)
+        if forward_ad._current_level >= 0:      # (within a dual level)
+            _hip.refuse_tangents("AxialRotary", t, p if isinstance(p, torch.Tensor) else None)
         if t.dim() != 4 or t.shape[3] != self.head_dim:
             raise ValueError("AxialRotary: expected [batch, heads, tokens, %d], got %s" % (self.head_dim, tuple(t.shape)))
         if t.dtype not in (torch.float32, torch.bfloat16, torch.float16):
