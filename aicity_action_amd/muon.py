@@ -5,6 +5,7 @@ each weight by its orthogonalised momentum, all matrices in the same launches wh
 few more).  ``solver.construct_optimizer`` builds a train step on it (``SOLVER.OPTIMIZING_METHOD muon``); the reference's own methods are
 those of slowfast/models/optimizer.py:140-206.  Everything runs on the tensors' device and its current stream; there is no CPU fallback."""
 import bisect
+import functools
 import math
 
 import numpy as np
@@ -16,7 +17,26 @@ from . import _hip
 QUINTIC = (3.4445, -4.7750, 2.0315)       # a, b, c of X <- a X + (b A + c A A) X: steep at zero, between 0.68 and 1.21 from 0.1 on after five steps
 _REC = np.dtype([("u", "u8"), ("w", "u8"), ("m", "u8"), ("out", "u8"), ("rs", "i8"), ("cs", "i8"), ("rows", "i4"), ("cols", "i4"),
                  ("scale", "f4"), ("pad", "i4")])
+_ROOM = 15.0                  # X, A and B are fp16 values times 2^12: 65504 / 4096, less a margin for their rounding
 _ARITHMETIC = {"fp16": 0, "split": 1}
+
+
+@functools.lru_cache(maxsize=64)
+def _largest(steps, a, b, c):
+    """The largest value that X, A or B can hold while ``steps`` are taken: no entry is larger than the largest singular value, those of X_0 are at
+    most one, and every step is one polynomial of each.  (The last X is the result and not held.)"""
+    top, most = 1.0, 1.0
+    for _ in range(steps):
+        t = top * top
+        vertex = [-b / (2 * c)] if c else []
+        disc = 9 * b * b - 20 * a * c
+        ends = [(-3 * b + s * math.sqrt(disc)) / (10 * c) for s in (-1, 1)] if c and disc >= 0 else [-a / (3 * b)] if b and not c else []
+        inside = lambda points: [p for p in points if 0 < p < t] + [t]  # noqa: E731
+        most = max(most, top, t, max(abs(b * p + c * p * p) for p in inside(vertex)))
+        top = max(abs(math.sqrt(p) * (a + b * p + c * p * p)) for p in inside(ends))
+        if not most < _ROOM:
+            break
+    return most
 
 
 def _check_iteration(steps, coefficients, eps, arithmetic):
@@ -24,6 +44,9 @@ def _check_iteration(steps, coefficients, eps, arithmetic):
         raise ValueError("Newton-Schulz: 1 to 100 steps, got %r" % (steps,))
     if len(coefficients) != 3 or not all(math.isfinite(c) for c in coefficients):
         raise ValueError("Newton-Schulz: three finite coefficients, got %r" % (coefficients,))
+    if not _largest(int(steps), *coefficients) < _ROOM:
+        raise ValueError("Newton-Schulz: coefficients %r grow values of %.3g in %d steps, and the products hold up to %g"
+                         % (tuple(coefficients), _largest(int(steps), *coefficients), steps, _ROOM))
     if not (math.isfinite(eps) and eps > 0.0):
         raise ValueError("Newton-Schulz: eps must be positive, got %r" % (eps,))
     if arithmetic not in _ARITHMETIC:
@@ -39,7 +62,8 @@ def _workspace(L, rec, split, device):
 
 def orthogonalize(update, steps=5, coefficients=QUINTIC, eps=1e-7, dtype=torch.bfloat16, arithmetic=None):
     """Newton-Schulz orthogonalisation of one matrix, a batch [..., rows, columns] or a list of either (sizes may differ; one set of
-    launches for all).  float32 / bfloat16 / float16, any strides.  Returns contiguous tensors of ``dtype``.
+    launches for all).  float32 / bfloat16 / float16, any strides.  Returns contiguous tensors of ``dtype``.  Coefficients under which a singular
+    value or its polynomial would reach 15 on the way are refused.
 
     ``arithmetic``: "fp16" (default for 16-bit results) computes the products from fp16 operands, which leaves the result within 3e-3 of the exact one
     relative to its norm (five steps, these coefficients; about 1.4e-3 from a hundred rows on).  "split" (default for float32) computes them

@@ -391,6 +391,8 @@ int mvit_rotary(const mvit_rotary_tensor* tensors, int ntensors, int dim, int ax
 
 /* Newton-Schulz orthogonalisation of a set of matrices and the Muon step around it (csrc/newton_schulz.hip):
  *   X = u / (|u|_F + eps);  steps times:  A = X X^T, X <- a X + (b A + c A A) X   (on the transposed matrix where rows > cols).
+ * X, A and b A + c A A are held in fp16 times 2^12: coefficients must keep the singular values of all three below 15 in every step but the last X (the
+ * caller's duty; those of X_0 are at most 1, and each step is one polynomial of every one).
  * mats: HOST array of count records; the matrices may have any sizes (MVIT_EUNSUPPORTED from 2^31 padded elements on) and run together,
  * in sets of 72.  u: in_dtype-typed, element strides given.
  *   mvit_newton_schulz: out [rows][cols] of out_dtype.

@@ -487,3 +487,33 @@ def test_gradients_that_overlap_what_a_step_writes_are_refused():
         other.momenta[0] = replaced
         with pytest.raises(ValueError, match="changed its"):
             other.step([far], lr=0.1)
+
+
+def test_coefficients_that_leave_the_products_range_are_refused():
+    """Against the polynomials on a fine grid of singular values."""
+    from aicity_action_amd import muon
+    grid = torch.linspace(0.0, 1.0, 20001, dtype=torch.float64)
+    some = [QUINTIC, (1.5, -0.5, 0.0), (2.0, -1.5, 0.5), (4.0848, -6.8946, 2.9270), (1.0, 0.0, 0.0), (15.0 / 8, -10.0 / 8, 3.0 / 8), (0.5, 0.1, -0.2),
+            (2.0, 0.0, 0.0), (3.0, 3.0, 3.0), (-3.0, 5.0, -2.5), (0.0, 0.0, 1.0), (20.0, 0.0, 0.0), (1.0, 16.0, -16.0), (3.0, -4.0, 0.0)]
+    refused = 0
+    for co in some:
+        for steps in (1, 2, 3, 5, 12):
+            s, most = grid, 1.0
+            for _ in range(steps):
+                t = s * s
+                most = max(most, s.abs().max().item(), t.max().item(), (co[1] * t + co[2] * t * t).abs().max().item())
+                s = s * (co[0] + co[1] * t + co[2] * t * t)
+            got = muon._largest(steps, *co)
+            # the bound follows one interval, not every value, so it may be above what any singular value meets, never below
+            assert got >= most * (1 - 1e-6) or got >= muon._ROOM
+            if co in some[:7]:
+                assert got == pytest.approx(most, rel=0.3) and got < muon._ROOM
+            if most >= muon._ROOM:
+                refused += 1
+                for call in (lambda: orthogonalize(torch.zeros(4, 6), steps=steps, coefficients=co),
+                             lambda: MuonMatrices([torch.zeros(4, 6)], steps=steps, coefficients=co)):
+                    with pytest.raises(ValueError, match="Newton-Schulz: coefficients"):
+                        call()
+    assert refused > 10
+    MuonMatrices([torch.zeros(4, 6)], steps=1, coefficients=(40.0, 0.0, 0.0))      # (the result itself has single precision's range)
+    MuonMatrices([torch.zeros(4, 6)], steps=100)
