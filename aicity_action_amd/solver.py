@@ -62,8 +62,10 @@ def param_groups(model, cfg):
 class HipAdamW(object):
     """AdamW(betas (0.9, 0.999), eps 1e-8) with fused global-norm clipping, fp32 state."""
 
+    METHODS = ("adamw", "zero_adamw")        # of SOLVER.OPTIMIZING_METHOD, that this class takes
+
     def __init__(self, model, cfg):
-        if cfg.SOLVER.OPTIMIZING_METHOD not in ("adamw", "zero_adamw", "muon"):
+        if cfg.SOLVER.OPTIMIZING_METHOD not in self.METHODS:
             raise NotImplementedError("Does not support {} optimizer".format(cfg.SOLVER.OPTIMIZING_METHOD))
         self.cfg = cfg
         self.lr = cfg.SOLVER.BASE_LR
@@ -454,6 +456,8 @@ class HipMuon(HipAdamW):
     Every rank of a DistributedDataParallel run takes the whole step on the gradients it holds (the kernels add in a fixed order, so the
     ranks stay equal bit by bit).  Gradient clipping, the loss scaler, the guard against a non-finite norm and the captured step
     (HIP.GRAPH_STEP) work as for AdamW."""
+
+    METHODS = ("muon",)
 
     def __init__(self, model, cfg):
         super().__init__(model, cfg)

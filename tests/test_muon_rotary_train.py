@@ -285,3 +285,18 @@ def test_rotary_option_and_muon_groups_on_the_host():
     cfg.SOLVER.OPTIMIZING_METHOD = "lion"
     with pytest.raises(NotImplementedError):
         construct_optimizer(model, cfg)
+
+
+def test_an_optimizer_takes_its_own_methods_only():
+    """HipAdamW on a configuration that asks for muon would step the matrices by AdamW without a word."""
+    from aicity_action_amd.solver import HipAdamW, HipMuon, HipZeroAdamW
+    cfg, _ = config("tiny_even", "fp32", gpus=0)
+    model = MViT(cfg)
+    for method, takes in (("muon", (HipMuon,)), ("adamw", (HipAdamW, HipZeroAdamW)), ("zero_adamw", (HipAdamW, HipZeroAdamW)), ("sgd", ())):
+        cfg.SOLVER.OPTIMIZING_METHOD = method
+        for kind in (HipAdamW, HipZeroAdamW, HipMuon):
+            if kind in takes:
+                kind(model, cfg)
+                continue
+            with pytest.raises(NotImplementedError, match=method):
+                kind(model, cfg)
