@@ -143,8 +143,6 @@ class MuonMatrices(object):
         if not self.params:
             raise ValueError("MuonMatrices: no parameters")
         _check_iteration(steps, coefficients, eps, arithmetic)
-        if not 0.0 <= momentum < 1.0:
-            raise ValueError("MuonMatrices: momentum must be in [0, 1), got %r" % (momentum,))
         if not (weight_decay >= 0.0 and math.isfinite(weight_decay)) or not (rms > 0.0 and math.isfinite(rms)):
             raise ValueError("MuonMatrices: weight_decay must not be negative and rms must be positive")
         if momenta is not None and len(momenta) != len(self.params):
@@ -157,8 +155,16 @@ class MuonMatrices(object):
             if m.shape != p.shape:
                 raise ValueError("MuonMatrices: a momentum of shape %s for a parameter of shape %s" % (tuple(m.shape), tuple(p.shape)))
         _apart((t.data_ptr(), t.data_ptr() + 4 * t.numel()) for t in self.params + self.momenta)
-        self.momentum, self.nesterov, self.weight_decay, self.rms = float(momentum), bool(nesterov), float(weight_decay), float(rms)
-        self.steps, self.coefficients, self.eps, self.arithmetic = int(steps), tuple(float(c) for c in coefficients), float(eps), arithmetic
+        self.weight_decay, self.rms, self.coefficients = float(weight_decay), float(rms), tuple(float(c) for c in coefficients)
+        self.eps, self.arithmetic = float(eps), arithmetic
+        self.configure(momentum, nesterov, steps)
+
+    def configure(self, momentum, nesterov, steps):
+        """Takes other values for the steps to come (a loaded state's)."""
+        _check_iteration(steps, self.coefficients, self.eps, self.arithmetic)
+        if not 0.0 <= momentum < 1.0:
+            raise ValueError("MuonMatrices: momentum must be in [0, 1), got %r" % (momentum,))
+        self.momentum, self.nesterov, self.steps = float(momentum), bool(nesterov), int(steps)
 
     def _check_matrix(self, t, what):
         if t.dim() != 2 or t.numel() == 0:

@@ -504,6 +504,7 @@ class HipMuon(HipAdamW):
         return sd
 
     def load_state_dict(self, sd):
+        """As for AdamW; momentum, Nesterov and the number of steps come with the state, as torch's optimizers take them."""
         if "param_groups" not in sd:
             raise ValueError("loaded optimizer state is not one of SOLVER.OPTIMIZING_METHOD muon")
         n = len(self.groups[0]["params"])
@@ -514,6 +515,9 @@ class HipMuon(HipAdamW):
                 raise ValueError("optimizer state %d (%s): momentum_buffer has shape %s, the parameter %s" % (
                     i, self.groups[0]["names"][i], have, tuple(self.groups[0]["params"][i].shape)))
         super().load_state_dict(sd)
+        if self._matrices is not None:
+            grp, m = sd["param_groups"][0], self._matrices
+            m.configure(grp.get("momentum", m.momentum), grp.get("nesterov", m.nesterov), grp.get("ns_steps", m.steps))
         for i, ent in enumerate(entries):
             if ent is not None:
                 self._matrices.momenta[i].copy_(ent["momentum_buffer"])

@@ -300,3 +300,39 @@ def test_an_optimizer_takes_its_own_methods_only():
                 continue
             with pytest.raises(NotImplementedError, match=method):
                 kind(model, cfg)
+
+
+def test_a_loaded_state_brings_its_momentum_and_steps():
+    cfg, _ = config("tiny_even", "fp32", gpus=0)
+    model = MViT(cfg)
+    cfg.HIP.MUON_MOMENTUM, cfg.HIP.MUON_STEPS, cfg.HIP.MUON_NESTEROV = 0.8, 4, False
+    saved = construct_optimizer(model, cfg)
+    saved.step_count = 7
+    sd = saved.state_dict()
+    cfg.HIP.MUON_MOMENTUM, cfg.HIP.MUON_STEPS, cfg.HIP.MUON_NESTEROV = 0.95, 5, True
+    opt = construct_optimizer(model, cfg)
+    opt.load_state_dict(sd)
+    assert (opt._matrices.momentum, opt._matrices.steps, opt._matrices.nesterov) == (0.8, 4, False)
+    assert opt.step_count == 7
+    assert opt.state_dict()["param_groups"] == sd["param_groups"]
+    for key in ("momentum", "nesterov", "ns_steps"):               # a state without them leaves the configuration's
+        del sd["param_groups"][0][key]
+    opt = construct_optimizer(model, cfg)
+    opt.load_state_dict(sd)
+    assert (opt._matrices.momentum, opt._matrices.steps, opt._matrices.nesterov) == (0.95, 5, True)
+    sd["param_groups"][0]["momentum"] = 1.0
+    with pytest.raises(ValueError, match="momentum"):
+        opt.load_state_dict(sd)
+
+
+def test_a_loaded_state_brings_its_step_count():
+    """The matrices' entries alone, and AdamW's beside them."""
+    cfg, _ = config("tiny_even", "fp32", gpus=0)
+    opt = construct_optimizer(MViT(cfg), cfg)
+    n = len(opt.groups[0]["params"])
+    for keep in (lambda i: True, lambda i: i < n):
+        sd = opt.state_dict()
+        sd["state"] = {i: dict(ent, step=ent["step"] + 7) for i, ent in sd["state"].items() if keep(i)}
+        other = construct_optimizer(MViT(cfg), cfg)
+        other.load_state_dict(sd)
+        assert other.step_count == 7
