@@ -954,9 +954,10 @@ __device__ __forceinline__ void ns_small_body(const NsSmallArgs& a, const NsSmal
             }
         }
         __syncthreads();
+        // (a wave without a tile sums nothing, so that all of them come to the one barrier; a sum that only some carry across it spills)
+        const f32x16 square = product(along, along, sa, lda, apl, sa, lda, apl, 32 * ti, 32 * tj, wave < nb * nb ? mp : 0);
+        __syncthreads();                                        // everyone has read A: each wave puts its tile of B in its tile's place
         if (wave < nb * nb) {
-            const f32x16 acc = product(along, along, sa, lda, apl, sa, lda, apl, 32 * ti, 32 * tj, mp);
-            __syncthreads();                                    // everyone has read A: each wave puts its tile of B in its tile's place
 #pragma unroll
             for (int e4 = 0; e4 < 4; ++e4) {
                 const int N = 32 * tj + r, M = 32 * ti + 8 * e4 + 4 * h;
@@ -970,11 +971,10 @@ __device__ __forceinline__ void ns_small_body(const NsSmallArgs& a, const NsSmal
                     for (int e = 0; e < 4; ++e) v[e] += (float)lo[e];
                 }
 #pragma unroll
-                for (int e = 0; e < 4; ++e) v[e] = a.b * v[e] + a.c / NS_S * acc[4 * e4 + e];
+                for (int e = 0; e < 4; ++e) v[e] = a.b * v[e] + a.c / NS_S * square[4 * e4 + e];
                 put(sa, lda, apl, v, N, M);
             }
-        } else
-            __syncthreads();                                    // (a wave goes one way as a whole)
+        }
         __syncthreads();
 #pragma unroll
         for (int k = 0; k < TPW; ++k) {
