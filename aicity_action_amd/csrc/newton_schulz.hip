@@ -344,7 +344,7 @@ __device__ __forceinline__ uint32_t ns_tile_of(uint32_t wg, uint32_t run) {
 
 // 64 lanes x 16 bytes from base (wave-uniform) + offset to 1 KiB of LDS at dst (wave-uniform).  In asm because the compiler, which cannot tell
 // these writes from the reads of the other stage, would wait for them in front of every read; the kernel waits itself (vmcnt) before its
-// barriers.  (M0 cannot be named as overwritten; nothing else in the kernel uses it.)
+// barriers.  (M0 cannot be named as overwritten; nothing else in the compiled kernels uses it, which a test reads from the object.)
 __device__ __forceinline__ void ns_dma(const h16* base, uint32_t offset, const char* dst) {
     const uint32_t to = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(const __attribute__((address_space(3))) char*)dst);
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(offset), "s"(base) : "memory");

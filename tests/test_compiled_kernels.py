@@ -1,0 +1,44 @@
+"""What the comments in the kernels' sources promise of the compiled code, read from the objects that the build leaves (no device needed)."""
+import os
+import re
+import subprocess
+
+import pytest
+
+from aicity_action_amd import _hip
+
+LLVM = "/opt/rocm/llvm/bin"
+OBJECTS = [os.path.join(os.path.dirname(_hip.LIB_PATH), d) for d in ("obj", "obj_f16")]
+
+
+def listing(path, tmp_path):
+    """The gfx950 instructions of an object file, in order."""
+    if not os.path.exists(path) or not os.path.exists(LLVM + "/llvm-objdump"):
+        pytest.skip("%s is not there: the library was built elsewhere" % path)
+    fat, code = str(tmp_path / "fat"), str(tmp_path / "code")
+    subprocess.check_call([LLVM + "/llvm-objcopy", "--dump-section", ".hip_fatbin=" + fat, path, os.devnull])
+    subprocess.check_call([LLVM + "/clang-offload-bundler", "--unbundle", "--type=o", "--targets=hipv4-amdgcn-amd-amdhsa--gfx950", "--input=" + fat,
+                           "--output=" + code])
+    text = subprocess.run([LLVM + "/llvm-objdump", "-d", code], check=True, capture_output=True, text=True).stdout
+    return [line.split("//")[0].strip() for line in text.splitlines() if line.startswith("\t")]
+
+
+@pytest.mark.parametrize("objects", OBJECTS, ids=os.path.basename)
+def test_nothing_but_the_lds_loads_uses_m0_in_newton_schulz(objects, tmp_path):
+    """ns_dma writes M0 in inline asm, which cannot name it as overwritten: right as long as the compiler keeps nothing of its own there."""
+    code = listing(os.path.join(objects, "newton_schulz.o"), tmp_path)
+    loads = 0
+    for i, line in enumerate(code):
+        if re.search(r"\bm0\b", line):
+            assert re.match(r"s_mov_b32 m0, s\d+$", line), line
+            assert code[i + 1] == "s_nop 0" and code[i + 2].startswith("global_load_lds_dwordx4 "), code[i:i + 3]
+            loads += 1
+        assert not re.match(r"[sv]_movrel|s_sendmsg|ds_gws|ds_\w*_gs_|v_interp|buffer_load_\w+ .*\blds\b", line), line
+    assert loads == sum(line.startswith("global_load_lds") for line in code) > 0
+
+
+@pytest.mark.parametrize("objects", OBJECTS, ids=os.path.basename)
+@pytest.mark.parametrize("name", ["newton_schulz", "rotary", "rowops", "attention"])
+def test_no_packed_fp32_instructions(name, objects, tmp_path):
+    for line in listing(os.path.join(objects, name + ".o"), tmp_path):
+        assert not re.match(r"v_pk_(add|mul|fma)_f32", line), line
