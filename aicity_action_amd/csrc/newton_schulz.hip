@@ -1164,27 +1164,27 @@ static int ns_launch(NsGemmArgs& g, hipStream_t st) {
     }
     if (t128 < slots || rest > 64 || longest_rest < 16) rest = 0;
     const bool even = 4 * work >= 3 * t128 * longest;
-    if (SPLIT) {
+    if constexpr (SPLIT) {
         if (t128 - rest > 192 * ((t128 - rest + 255) / 256) && (even || t128 >= 512)) {
-            const int rc = ns_launch_as<128, 1, 2, PHASE, SPLIT>(g, st, rest);
-            return rc != MVIT_OK || !rest ? rc : ns_launch_as<64, 2, 2, PHASE, SPLIT>(g, st, rest);
+            const int rc = ns_launch_as<128, 1, 2, PHASE, true>(g, st, rest);
+            return rc != MVIT_OK || !rest ? rc : ns_launch_as<64, 2, 2, PHASE, true>(g, st, rest);
         }
-        if constexpr (PHASE == NS_GRAM && SPLIT) {
+        if constexpr (PHASE == NS_GRAM) {
             const int64_t cuts = std::min<int64_t>(std::min<int64_t>(8, NS_SUMS / t64), longest / 4);
             if (cuts >= 2 && longest >= 16) {
                 g.cuts = (uint32_t)cuts;
-                const int rc = ns_launch_as<64, 2, 2, NS_PART, SPLIT>(g, st);
-                return rc != MVIT_OK ? rc : ns_launch_as<64, 1, 2, NS_JOIN, SPLIT>(g, st);
+                const int rc = ns_launch_as<64, 2, 2, NS_PART, true>(g, st);
+                return rc != MVIT_OK ? rc : ns_launch_as<64, 1, 2, NS_JOIN, true>(g, st);
             }
         }
-        if (longest >= 8 && t64 <= 256) return ns_launch_as<64, 2, 2, PHASE, SPLIT>(g, st);
+        if (longest >= 8 && t64 <= 256) return ns_launch_as<64, 2, 2, PHASE, true>(g, st);
     } else {
         if (t128 >= 512 || (t128 >= 192 && even)) {
-            const int rc = ns_launch_as<128, 1, 2, PHASE, SPLIT>(g, st, rest);
-            return rc != MVIT_OK || !rest ? rc : ns_launch_as<64, 2, SPLIT ? 2 : 5, PHASE, SPLIT>(g, st, rest);
+            const int rc = ns_launch_as<128, 1, 2, PHASE, false>(g, st, rest);
+            return rc != MVIT_OK || !rest ? rc : ns_launch_as<64, 2, 5, PHASE, false>(g, st, rest);
         }
-        if (longest >= 8 && t64 <= 256) return ns_launch_as<64, 2, SPLIT ? 2 : 5, PHASE, SPLIT>(g, st);
-        if (t64 <= 512) return ns_launch_as<64, 1, SPLIT ? 2 : 5, PHASE, SPLIT>(g, st);
+        if (longest >= 8 && t64 <= 256) return ns_launch_as<64, 2, 5, PHASE, false>(g, st);
+        if (t64 <= 512) return ns_launch_as<64, 1, 5, PHASE, false>(g, st);
     }
     return ns_launch_as<64, 1, 2, PHASE, SPLIT>(g, st);
 }

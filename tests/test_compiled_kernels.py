@@ -11,15 +11,20 @@ LLVM = "/opt/rocm/llvm/bin"
 OBJECTS = [os.path.join(os.path.dirname(_hip.LIB_PATH), d) for d in ("obj", "obj_f16")]
 
 
-def listing(path, tmp_path):
-    """The gfx950 instructions of an object file, in order."""
+def code_object(path, tmp_path):
+    """The gfx950 part of an object file."""
     if not os.path.exists(path) or not os.path.exists(LLVM + "/llvm-objdump"):
         pytest.skip("%s is not there: the library was built elsewhere" % path)
     fat, code = str(tmp_path / "fat"), str(tmp_path / "code")
     subprocess.check_call([LLVM + "/llvm-objcopy", "--dump-section", ".hip_fatbin=" + fat, path, os.devnull])
     subprocess.check_call([LLVM + "/clang-offload-bundler", "--unbundle", "--type=o", "--targets=hipv4-amdgcn-amd-amdhsa--gfx950", "--input=" + fat,
                            "--output=" + code])
-    text = subprocess.run([LLVM + "/llvm-objdump", "-d", code], check=True, capture_output=True, text=True).stdout
+    return code
+
+
+def listing(path, tmp_path):
+    """Its instructions, in order."""
+    text = subprocess.run([LLVM + "/llvm-objdump", "-d", code_object(path, tmp_path)], check=True, capture_output=True, text=True).stdout
     return [line.split("//")[0].strip() for line in text.splitlines() if line.startswith("\t")]
 
 
@@ -42,3 +47,15 @@ def test_nothing_but_the_lds_loads_uses_m0_in_newton_schulz(objects, tmp_path):
 def test_no_packed_fp32_instructions(name, objects, tmp_path):
     for line in listing(os.path.join(objects, name + ".o"), tmp_path):
         assert not re.match(r"v_pk_(add|mul|fma)_f32", line), line
+
+
+def test_newton_schulz_holds_the_tile_kernels_that_its_dispatch_names(tmp_path):
+    """ns_gemm_kernel<tile side, wave groups, stages, phase, split>: variants that no call reaches are not compiled."""
+    code = code_object(os.path.join(OBJECTS[0], "newton_schulz.o"), tmp_path)
+    names = subprocess.run([LLVM + "/llvm-nm", "-C", code], check=True, capture_output=True, text=True).stdout
+    found = set(re.findall(r"ns_gemm_kernel<(\d+), (\d+), (\d+), (\d+), (true|false)>", names))
+    phases = [str(p) for p in range(6)]           # the products of an iteration, and the last one to 16 bits, fp32 and the weights
+    want = {v + (p, s) for p in phases for s in ("true", "false") for v in (("128", "1", "2"), ("64", "1", "2"))}
+    want |= {v + (p, "false") for p in phases for v in (("64", "1", "5"), ("64", "2", "5"))}
+    want |= {("64", "2", "2", p, "true") for p in phases + ["6"]} | {("64", "1", "2", "7", "true")}       # 6, 7: pieces of long sums
+    assert found == want
