@@ -52,7 +52,7 @@ def test_no_packed_fp32_instructions(name, objects, tmp_path):
 def test_newton_schulz_holds_the_tile_kernels_that_its_dispatch_names(tmp_path):
     """ns_gemm_kernel<tile side, wave groups, stages, phase, split>: variants that no call reaches are not compiled."""
     code = code_object(os.path.join(OBJECTS[0], "newton_schulz.o"), tmp_path)
-    names = subprocess.run([LLVM + "/llvm-nm", "-C", code], check=True, capture_output=True, text=True).stdout
+    names = subprocess.run([LLVM + "/llvm-objdump", "-t", "-C", code], check=True, capture_output=True, text=True).stdout
     found = set(re.findall(r"ns_gemm_kernel<(\d+), (\d+), (\d+), (\d+), (true|false)>", names))
     phases = [str(p) for p in range(6)]           # the products of an iteration, and the last one to 16 bits, fp32 and the weights
     want = {v + (p, s) for p in phases for s in ("true", "false") for v in (("128", "1", "2"), ("64", "1", "2"))}
