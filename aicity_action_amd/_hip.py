@@ -5,6 +5,7 @@ caller gets an exception.  ``stream`` arguments are raw hipStream_t handles
 (``torch.cuda.current_stream().cuda_stream``).
 """
 import ctypes
+import functools
 import os
 import subprocess
 
@@ -139,6 +140,15 @@ def lib(half="bf16"):
     if _lib is None:
         _lib = _load(LIB_PATH)
     return _lib
+
+
+@functools.lru_cache(maxsize=None)
+def lib_with_record(half, entry, size):
+    """lib(half), whose struct that ``entry`` returns the bytes of is the one that the caller packs by hand (asked once)."""
+    L = lib(half)
+    if getattr(L, entry)() != size:
+        raise RuntimeError("%s: the library's record has %d bytes, the binding's %d; build it again" % (entry, getattr(L, entry)(), size))
+    return L
 
 
 # bench.py's in-step roofline: when this is a list, every fused-attention launch of the model is bracketed by two timing events on

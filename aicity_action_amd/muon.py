@@ -53,6 +53,10 @@ def _check_iteration(steps, coefficients, eps, arithmetic):
         raise ValueError("Newton-Schulz: arithmetic must be 'fp16' or 'split', got %r" % (arithmetic,))
 
 
+def _library(half):
+    return _hip.lib_with_record(half, "mvit_ns_matrix_bytes", _REC.itemsize)
+
+
 def _workspace(L, rec, split, device):
     n = L.mvit_newton_schulz_workspace_bytes(rec.ctypes.data, len(rec), split)
     _hip.check(min(int(n), 0), "newton_schulz (sizes)")
@@ -108,7 +112,7 @@ def orthogonalize(update, steps=5, coefficients=QUINTIC, eps=1e-7, dtype=torch.b
                              t.stride(-2), t.stride(-1), r, c, 0.0, 0))
         if rows:
             rec = np.array(rows, dtype=_REC)
-            L = _hip.lib("fp16" if half else "bf16")
+            L = _library("fp16" if half else "bf16")
             split = _ARITHMETIC[arithmetic]
             ws, n = _workspace(L, rec, split, ts[0].device)
             code = lambda d: _hip.F32 if d == torch.float32 else _hip.BF16  # noqa: E731
@@ -212,7 +216,7 @@ class MuonMatrices(object):
         if not self.params[0].is_cuda:
             raise RuntimeError("MuonMatrices needs its parameters on a gfx950 device; there is no CPU fallback")
         rec = np.array(rows, dtype=_REC)
-        L, split = _hip.lib(), _ARITHMETIC[self.arithmetic]
+        L, split = _library("bf16"), _ARITHMETIC[self.arithmetic]
         with torch.cuda.device(device):
             ws, n = _workspace(L, rec, split, device)
             _hip.check(L.mvit_muon_step(rec.ctypes.data, len(rec), float(lr or 0.0), self.weight_decay, self.momentum, int(self.nesterov),

@@ -185,7 +185,7 @@ def _records(xs, outs, adds, ps):
 
 def _launch(xs, outs, adds, ps, dim, axes, sections, turns, layout, inverse):
     x, rec = xs[0], _records(xs, outs, adds, ps)
-    lib = _hip.lib("fp16" if x.dtype == torch.float16 else "bf16")
+    lib = _hip.lib_with_record("fp16" if x.dtype == torch.float16 else "bf16", "mvit_rotary_tensor_bytes", _RECORD.size)
     act = _hip.F32 if x.dtype == torch.float32 else _hip.BF16
     args = (rec, len(xs), dim, axes, sections, turns, layout, 1 if inverse else 0, act)
     at = x.device.index

@@ -59,3 +59,22 @@ def test_newton_schulz_holds_the_tile_kernels_that_its_dispatch_names(tmp_path):
     want |= {v + (p, "false") for p in phases for v in (("64", "1", "5"), ("64", "2", "5"))}
     want |= {("64", "2", "2", p, "true") for p in phases + ["6"]} | {("64", "1", "2", "7", "true")}       # 6, 7: pieces of long sums
     assert found == want
+
+
+@pytest.mark.parametrize("half", ["bf16", "fp16"])
+def test_hand_packed_records_are_the_library_s(half):
+    """The sizes, and each record's fields by what the host side makes of them."""
+    import numpy as np
+
+    from aicity_action_amd import muon, rotary
+    L = _hip.lib_with_record(half, "mvit_rotary_tensor_bytes", rotary._RECORD.size)
+    assert L is _hip.lib(half) and muon._library(half) is L
+    with pytest.raises(RuntimeError, match="build it again"):
+        _hip.lib_with_record(half, "mvit_ns_matrix_bytes", muon._REC.itemsize - 4)
+    # rows and columns: a matrix of 65 rows and 200 columns is no one-workgroup matrix once its columns are far apart, and one of 65 x 2000 never is
+    size = lambda *m: L.mvit_newton_schulz_workspace_bytes(np.array([m], dtype=muon._REC).ctypes.data, 1, 0)  # noqa: E731
+    assert size(8, 8, 8, 8, 200, 1, 65, 200, 0.0, 0) == 0
+    tables = 72 * 256 * 8
+    assert size(8, 8, 8, 8, 200, 1 << 28, 65, 200, 0.0, 0) == tables + 2 * (3 * 128 * 256 + 2 * 128 * 128)
+    assert size(8, 8, 8, 8, 2000, 1, 65, 2000, 0.0, 0) == tables + 2 * (3 * 128 * 2048 + 2 * 128 * 128)
+    assert size(8, 8, 8, 8, 1, 1, 0, 5, 0.0, 0) < 0
