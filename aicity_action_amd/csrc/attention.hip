@@ -218,9 +218,9 @@ __global__ __launch_bounds__(64 * NW) void attn_fwd_bf16_kernel(const bf16_t* __
 #pragma unroll
                 for (int jj = 0; jj < 4; ++jj) {
                     const f32x2 sv = {s[kb][8 * sh + 2 * jj], s[kb][8 * sh + 2 * jj + 1]};
-                    const f32x2 t = __builtin_elementwise_fma(sv, c2, mc2);            // v_pk_fma_f32
+                    const f32x2 t = __builtin_elementwise_fma(sv, c2, mc2);
                     const f32x2 pp = {__builtin_amdgcn_exp2f(t[0]), __builtin_amdgcn_exp2f(t[1])};
-                    ps2 += pp;                                                          // v_pk_add_f32
+                    ps2 += pp;
                     pk[jj] = pack_bf16x2(pp[0], pp[1]);
                 }
                 uint4 u = make_uint4(pk[0], pk[1], pk[2], pk[3]);
