@@ -336,3 +336,63 @@ def test_a_loaded_state_brings_its_step_count():
         other = construct_optimizer(MViT(cfg), cfg)
         other.load_state_dict(sd)
         assert other.step_count == 7
+
+
+@gpu
+@pytest.mark.parametrize("name", ["tiny_even", "tiny_odd", "tiny_plain"])
+def test_rotary_model_gradients_relative_to_their_own_size(name, monkeypatch):
+    """Every gradient of the fp32 path against the oracle's in 64 bits, relative to that tensor's largest (the key-side norms' are 1e-4 of others').
+    The oracle's own fp32 gradients are within 2e-6 of them so measured, in every tensor of the three models; 1e-4 leaves room for other
+    orders of sums and functions good to a few units in the last place, 50 times that."""
+    cfg, meta, model, clip, labels = model_and_batch(name, "fp32")
+    monkeypatch.setattr(O, "attention", rotary_attention)
+    sd = {k: v.detach().cpu().double().requires_grad_(True) for k, v in model.state_dict().items()}
+    _, want = O.forward(sd, clip.double(), copy.deepcopy(cfg.MVIT.to_dict()), training=False, head_act=False)
+    O.soft_target_cross_entropy(want, labels.double()).backward()
+    model.train()
+    soft_target_cross_entropy(model([clip.cuda()]), labels.cuda()).backward()
+    for k, p in model.named_parameters():
+        ref = sd[k].grad
+        assert (p.grad.cpu().double() - ref).abs().max() <= 1e-4 * ref.abs().max(), k
+
+
+def _muon_rank(rank, world, port, results):
+    """A rank's own half of the batch, gradients averaged over the ranks (in host memory), three whole steps."""
+    import hashlib
+    import os
+
+    import torch.distributed as dist
+    os.environ["MASTER_ADDR"], os.environ["MASTER_PORT"] = "127.0.0.1", str(port)
+    torch.cuda.set_device(0)
+    dist.init_process_group("gloo", rank=rank, world_size=world)
+    cfg, meta, model, clip, labels = model_and_batch("tiny_even", "bf16")
+    opt = construct_optimizer(model.train(), cfg)
+    half = slice(rank * meta["batch"] // world, (rank + 1) * meta["batch"] // world)
+    for _ in range(3):
+        one_backward(model, clip[half], labels[half])
+        for p in model.parameters():
+            mean = p.grad.cpu()
+            dist.all_reduce(mean)
+            p.grad = (mean / world).to(p.grad.device)
+        opt.set_lr(1e-3)
+        opt.step()
+    digest = hashlib.sha256(b"".join(t.detach().cpu().numpy().tobytes() for t in list(model.parameters()) + opt._matrices.momenta)).hexdigest()
+    results.put((rank, half.stop - half.start, digest))
+    dist.barrier()
+    dist.destroy_process_group()
+
+
+@gpu
+def test_muon_ranks_stay_equal_bit_by_bit():
+    import torch.multiprocessing as mp
+    from test_hip_ddp import _free_port
+    ctx = mp.get_context("spawn")
+    results, port = ctx.Queue(), _free_port()
+    ranks = [ctx.Process(target=_muon_rank, args=(r, 2, port, results)) for r in range(2)]
+    for p in ranks:
+        p.start()
+    got = [results.get(timeout=100) for _ in ranks]
+    for p in ranks:
+        p.join(60)
+        assert p.exitcode == 0
+    assert sorted(r for r, _, _ in got) == [0, 1] and all(n > 0 for _, n, _ in got) and got[0][2] == got[1][2]
