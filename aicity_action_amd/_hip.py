@@ -103,14 +103,15 @@ EXPORTS = tuple(_SIGS)
 
 
 def build(force=False):
-    """Compile every HIP source for gfx950 into lib/libmvit_hip.so (hipcc cross-compiles without a GPU)."""
+    """Compile every HIP source for gfx950 into lib/libmvit_hip.so and libmvit_hip_f16.so (hipcc cross-compiles without a GPU): what is older
+    than its source, or with ``force`` all of them."""
     srcs = [os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith((".hip", ".h"))]
     srcs.append(os.path.join(os.path.dirname(_HERE), "include", "mvit_hip.h"))
     if not force and all(os.path.exists(p) and all(os.path.getmtime(p) >= os.path.getmtime(s) for s in srcs)
                          for p in (LIB_PATH, LIB_PATH_F16)):
         return LIB_PATH
     os.makedirs(os.path.dirname(LIB_PATH), exist_ok=True)
-    subprocess.check_call(["make", "-C", CSRC, "-j", str(min(8, os.cpu_count() or 1))])
+    subprocess.check_call(["make", "-C", CSRC, "-j", str(min(8, os.cpu_count() or 1))] + (["-B"] if force else []))
     return LIB_PATH
 
 

@@ -78,3 +78,13 @@ def test_hand_packed_records_are_the_library_s(half):
     assert size(8, 8, 8, 8, 200, 1 << 28, 65, 200, 0.0, 0) == tables + 2 * (3 * 128 * 256 + 2 * 128 * 128)
     assert size(8, 8, 8, 8, 2000, 1, 65, 2000, 0.0, 0) == tables + 2 * (3 * 128 * 2048 + 2 * 128 * 128)
     assert size(8, 8, 8, 8, 1, 1, 0, 5, 0.0, 0) < 0
+
+
+def test_the_build_entry_compiles_where_a_library_is_there(monkeypatch):
+    import __graft_entry__
+    calls = []
+    monkeypatch.setattr(_hip.subprocess, "check_call", lambda cmd, **kw: calls.append(cmd))
+    __graft_entry__.build()
+    assert len(calls) == 1 and calls[0][0] == "make" and "-B" in calls[0]
+    _hip.build()                       # the library is newer than its sources now
+    assert len(calls) == 1 or "-B" not in calls[1]
