@@ -139,7 +139,11 @@ class MuonMatrices(object):
 
     ``step``:  M <- mu M + (1 - mu) g;  U = (1 - mu) g + mu M (Nesterov) or M;  W <- W (1 - lr weight_decay) - lr rms sqrt(max(rows,
     columns)) NS(U).  ``rms`` 0.2 gives the update the size that AdamW's typically has, so that one learning rate and weight decay serve
-    both.  Weights and momenta: contiguous float32 matrices, updated in place; gradients: float32, any strides, in memory of their own."""
+    both.  Weights and momenta: contiguous float32 matrices, updated in place; gradients: float32, any strides, in memory of their own.
+
+    ``arithmetic`` of the orthogonalisation, as in ``orthogonalize``: "fp16" leaves NS(U) within 3e-3 of the exact one although everything around it
+    is float32 (an update is a small part of a weight, and the iteration itself stops up to 0.3 short of orthogonal), "split" within 1e-4 at twice
+    the time for a whole model's matrices (0.9 -> 1.7 ms for the video model's)."""
 
     def __init__(self, params, momenta=None, momentum=0.95, nesterov=True, weight_decay=0.0, rms=0.2, steps=5, coefficients=QUINTIC,
                  eps=1e-7, arithmetic="fp16"):
