@@ -16,11 +16,13 @@
 // both halves (high high + high low + low high, three times the matrix work): 5e-6 to 1e-5, for results wanted in single precision (4e-5 where one
 // direction dominates: a rounding of X_0 is amplified by those 485, in single precision throughout as well).
 //
-// Bound by the matrix cores where matrices are large: 4096 x 4096 takes 1.7 ms = 800 TFLOP/s counting A and A A half (a large library product of
+// Bound by the matrix cores where matrices are large: 4096 x 4096 takes 1.72 ms = 800 TFLOP/s counting A and A A half (a large library product of
 // this size: 1100), of which B X runs at 890; its LDS reads and LDS-DMA writes keep the LDS busy 1.5 times as long as the products the matrix
-// cores.  By memory as much as by them where they are many and shallow: the 34 M weights of the video model's blocks take 0.88 ms, of which a
-// launch of B X moves 360 MB in 79 us (4.5 TB/s, counted) beside its 33 GFLOP, the squares and X_0 406 MB each in 74 and 71 us (5.5 and 5.7).
-// By the latency of the chain of launches where they are few and small: 5 to 8 us each for three 1000 x 257.
+// cores.  By neither alone where they are many and shallow: the 34 M weights of the video model's blocks take 0.88 ms, of which a launch of B X moves
+// 359 MB in 81 us (4.4 TB/s, counted) with the matrix cores busy for a quarter of it -- tiles of six steps mostly, whose first loads and way out
+// do not overlap --, the squares and X_0 406 MB each in 74 and 72 us (5.5 and 5.6, what a copy reaches).
+// By the latency of the chain of launches where they are few and small: 5 to 8 us each for three 1000 x 257, of which 2 are the launch's and the
+// rest a first load, a few steps and the way out through LDS, one after the other.
 #include "common.h"
 #include <string.h>
 #include <algorithm>

@@ -2,7 +2,7 @@
 
 ``orthogonalize`` pushes the singular values of matrices to about one; ``MuonMatrices`` renews the momenta of a set of weights and steps
 each weight by its orthogonalised momentum, all matrices in the same launches whatever their sizes (one for a set of small ones, else 17 or a
-few more).  ``solver.construct_optimizer`` builds a train step on it (``SOLVER.OPTIMIZING_METHOD muon``); the reference's own methods are
+few more; matrices of few rows or columns run ahead of larger ones).  ``solver.construct_optimizer`` builds a train step on it (``SOLVER.OPTIMIZING_METHOD muon``); the reference's own methods are
 those of slowfast/models/optimizer.py:140-206.  Everything runs on the tensors' device and its current stream; there is no CPU fallback."""
 import bisect
 import functools
