@@ -1039,10 +1039,13 @@ static int ns_check(const mvit_ns_matrix* mats, int count) {
     return MVIT_OK;
 }
 
-// What a matrix is computed with is its own: matrices of at most 32 rows or columns always from pairs -- the rounding of their few entries of A and
-// B does not average out (2 x 7: up to 1.4 % from single fp16 values), and their products are short.  A call that has such matrices beside larger ones and
-// asks for fp16 products therefore runs as two parts, one behind the other in the same workspace; any other call is one part.
-// (18x768, 1x300 and 77x1 beside 130x70, 513x129 and 200x333, a Muon step: 138 us, from single values in one part 99.)
+// What a matrix is computed with: matrices of at most 32 rows or columns always from pairs -- the rounding of their few entries of A and B does not
+// average out (2 x 7: up to 1.4 % from single fp16 values), and their products are short.  A call that has such matrices beside larger ones and
+// asks for fp16 products runs as two parts, one behind the other in the same workspace; any other call is one part.  Where the matrices of few rows
+// need tiles, the second chain of launches costs more than pairs for larger matrices of up to 256 tiles (one per CU): then the call is one
+// part from pairs.  A Muon step in us, as two parts / one from pairs: 20x2500 beside 200x333 199 / 140, beside 384x1152 215 / 157, 1000x1000 (256
+// tiles) 245 / 246, 768x2304 (432) 265 / 227, 1500x1500 (576) 351 / 472; where they fit one workgroup the sides are about even (18x768, 1x300 and 77x1 beside
+// 130x70, 513x129 and 200x333 138 / 127, 384x1152 151 / 153, 768x2304 199 / 225), and it stays two.
 struct NsPart {
     const mvit_ns_matrix* mats;
     int count, only;             // only: -1 all matrices, 0 the larger ones, 1 those of few rows or columns
@@ -1072,7 +1075,12 @@ static int ns_parts(const mvit_ns_matrix* mats, int count, int asked, F f) {
     int few = 0;
     for (int i = 0; i < count; ++i) few += NsPart::few(mats[i]);
     if (asked || few == 0 || few == count) return f(NsPart(mats, count, -1, asked || few));
-    const int rc = f(NsPart(mats, count, 1, true));
+    const NsPart rows(mats, count, 1, true);
+    int64_t tiles = 0;             // of the larger ones
+    for (int i = 0; i < count; ++i)
+        if (!rows.has(i)) tiles += pad64(mats[i].rows) / 64 * (pad64(mats[i].cols) / 64);
+    if (!rows.small && tiles <= 256) return f(NsPart(mats, count, -1, true));
+    const int rc = f(rows);
     return rc != MVIT_OK ? rc : f(NsPart(mats, count, 0, false));
 }
 

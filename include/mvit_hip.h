@@ -395,14 +395,15 @@ int mvit_rotary(const mvit_rotary_tensor* tensors, int ntensors, int dim, int ax
  * caller's duty; those of X_0 are at most 1, and each step is one polynomial of every one).
  * mats: HOST array of count records; the matrices may have any sizes (MVIT_EUNSUPPORTED from 2^31 padded elements on) and run together,
  * in sets of 72.  u: in_dtype-typed, element strides given.
- *   mvit_newton_schulz: out [rows][cols] of out_dtype.
+ *   mvit_newton_schulz: out [rows][cols] of out_dtype; no out may overlap a u or another out.
  *   mvit_muon_step (fp32):  momentum <- mu momentum + (1 - mu) f u;  update = nesterov ? (1 - mu) f u + mu momentum : momentum;
- *       w <- w (1 - lr weight_decay) - lr scale NS(update);   w, momentum [rows][cols] contiguous, updated in place.
+ *       w <- w (1 - lr weight_decay) - lr scale NS(update);   w, momentum [rows][cols] contiguous, updated in place; no w or momentum may overlap
+ *       another one or a u.
  *       norm_coef: NULL (f = 1) or mvit_grad_norm's out2 (f = out2[1]; a non-finite norm or factor leaves w and momentum as they are);
  *       hyper: NULL or device memory whose first float is the learning rate (captured steps, as mvit_adamw_step_dev).
  * split 0: products from fp16 operands (result within 3e-3 of the exact one, relative to its norm, after five steps of the usual coefficients), 1: from pairs
- * of them (1e-4; three times the work).  Matrices of at most 32 rows or columns are always computed from pairs: beside larger ones they run
- * by themselves ahead of those.  Matrices that each fit a workgroup's LDS (about 48 K elements, 32 K from pairs, smaller side up to 128) are one launch and
+ * of them (1e-4; three times the work).  Matrices of at most 32 rows or columns are always computed from pairs: beside larger ones they run by
+ * themselves ahead of those, or take the whole call along where that is quicker.  Matrices that each fit a workgroup's LDS (about 48 K elements, 32 K from pairs, smaller side up to 128) are one launch and
  * need no workspace.
  * workspace: mvit_newton_schulz_workspace_bytes(mats, count, split) bytes (negative: MVIT_E*), 128-byte aligned, used by this call alone. */
 typedef struct {

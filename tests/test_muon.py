@@ -517,3 +517,15 @@ def test_coefficients_that_leave_the_products_range_are_refused():
     assert refused > 10
     MuonMatrices([torch.zeros(4, 6)], steps=1, coefficients=(40.0, 0.0, 0.0))      # (the result itself has single precision's range)
     MuonMatrices([torch.zeros(4, 6)], steps=100)
+
+
+@gpu
+@pytest.mark.parametrize("beside", [[(200, 333)], [(1000, 1000)], [(1024, 1088)], [(96, 288)] * 3], ids=str)
+def test_long_matrices_of_few_rows_beside_larger_ones(beside):
+    """The ones of few rows need tiles: one part from pairs up to 256 tiles of the larger ones, two parts above; more of them than a set holds."""
+    shapes = [(20, 2500), (1600, 28), (5, 40)] + beside
+    us = [u for i, shape in enumerate(shapes) for u in list(spectra(*shape, i))[:2]] + [gradient(1 + i % 30, 3 + i % 41, i) for i in range(150)]
+    for got, u in zip(orthogonalize(us, dtype=torch.float32, arithmetic="fp16"), us):
+        assert off(got, u) <= (FP16_BOUND if min(u.shape) > 32 else PAIRS_BOUND), u.shape
+    again = orthogonalize(us, dtype=torch.float32, arithmetic="fp16")
+    assert all(torch.equal(a, b) for a, b in zip(again, orthogonalize(us, dtype=torch.float32, arithmetic="fp16")))
