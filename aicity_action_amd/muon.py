@@ -2,8 +2,9 @@
 
 ``orthogonalize`` pushes the singular values of matrices to about one; ``MuonMatrices`` renews the momenta of a set of weights and steps
 each weight by its orthogonalised momentum, all matrices in the same launches whatever their sizes (one for a set of small ones, else 17 or a
-few more; matrices of few rows or columns run ahead of larger ones).  ``solver.construct_optimizer`` builds a train step on it (``SOLVER.OPTIMIZING_METHOD muon``); the reference's own methods are
-those of slowfast/models/optimizer.py:140-206.  Everything runs on the tensors' device and its current stream; there is no CPU fallback."""
+few more; matrices of few rows or columns run ahead of larger ones).  ``solver.construct_optimizer`` builds a train step on it
+(``SOLVER.OPTIMIZING_METHOD muon``); the reference's own methods are those of slowfast/models/optimizer.py:140-206.
+Everything runs on the tensors' device and its current stream; there is no CPU fallback."""
 import bisect
 import functools
 import math
@@ -69,8 +70,8 @@ def orthogonalize(update, steps=5, coefficients=QUINTIC, eps=1e-7, dtype=torch.b
     launches for all).  float32 / bfloat16 / float16, any strides.  Returns contiguous tensors of ``dtype``.  Coefficients under which a singular
     value or its polynomial would reach 15 on the way are refused.
 
-    ``arithmetic``: "fp16" (default for 16-bit results) computes the products from fp16 operands, which leaves the result within 3e-3 of the exact one
-    relative to its norm (five steps, these coefficients; about 1.4e-3 from a hundred rows on).  "split" (default for float32) computes them
+    ``arithmetic``: "fp16" (default for 16-bit results) computes the products from fp16 operands, which leaves the result within 3e-3 of the
+    exact one relative to its norm (five steps, these coefficients; about 1.4e-3 from a hundred rows on).  "split" (default for float32) computes them
     from pairs of fp16 values at three times the work: within 1e-4, and 1e-5 unless one direction of the update dominates all others.
     Matrices of at most 32 rows or columns always take pairs, whatever they stand beside.  A matrix of zeros stays zero; one with NaN or
     infinity gives NaN.  A matrix' last bits depend on the call it is in (which order its sums are taken in)."""
@@ -141,9 +142,9 @@ class MuonMatrices(object):
     columns)) NS(U).  ``rms`` 0.2 gives the update the size that AdamW's typically has, so that one learning rate and weight decay serve
     both.  Weights and momenta: contiguous float32 matrices, updated in place; gradients: float32, any strides, in memory of their own.
 
-    ``arithmetic`` of the orthogonalisation, as in ``orthogonalize``: "fp16" leaves NS(U) within 3e-3 of the exact one although everything around it
-    is float32 (an update is a small part of a weight, and the iteration itself stops up to 0.3 short of orthogonal), "split" within 1e-4 at twice
-    the time for a whole model's matrices (0.9 -> 1.7 ms for the video model's)."""
+    ``arithmetic`` of the orthogonalisation, as in ``orthogonalize``: "fp16" leaves NS(U) within 3e-3 of the exact one although everything
+    around it is float32 (an update is a small part of a weight, and the iteration itself stops up to 0.3 short of orthogonal), "split" within
+    1e-4 at twice the time for a whole model's matrices (0.9 -> 1.7 ms for the video model's)."""
 
     def __init__(self, params, momenta=None, momentum=0.95, nesterov=True, weight_decay=0.0, rms=0.2, steps=5, coefficients=QUINTIC,
                  eps=1e-7, arithmetic="fp16"):

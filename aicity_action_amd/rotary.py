@@ -77,9 +77,10 @@ class AxialRotary(object):
         return AxialRotary, (self.head_dim, self.sections, self.base, self.layout)
 
     def __call__(self, x, positions, k=None, k_positions=None):
-        """Turned copies of ``x`` (and ``k``), differentiable in reverse mode (a tensor with a forward-mode tangent is refused).  Tensors [batch, heads, tokens, head_dim], float32 / bfloat16 / float16, any
-        strides with contiguous channels (a token-major buffer goes in as its transposed view).  Positions: a TokenGrid, or a tensor
-        [tokens, axes] or [batch, tokens, axes] of int32 / int64 / float32 on the same device."""
+        """Turned copies of ``x`` (and ``k``), differentiable in reverse mode (a tensor or a gradient with a forward-mode tangent is refused).
+        Tensors [batch, heads, tokens, head_dim], float32 / bfloat16 / float16, any strides with contiguous channels (a token-major buffer goes
+        in as its transposed view).  Positions: a TokenGrid, or a tensor [tokens, axes] or [batch, tokens, axes] of int32 / int64 / float32 on
+        the same device."""
         xs, ps = self._arguments(x, positions, k, k_positions)
         if torch.is_grad_enabled() and any(t.requires_grad for t in xs):
             held = [_leaf_on_one_stream(t) for t in xs]
@@ -195,7 +196,8 @@ def _launch(xs, outs, adds, ps, dim, axes, sections, turns, layout, inverse):
         with torch.cuda.device(at):
             rc = lib.mvit_rotary(*args, _raw_stream(at))
     if rc == _hip.EINVAL and outs is xs:        # (everything else has been checked)
-        raise ValueError("AxialRotary.rotate_: the tensors are the same memory in part, or one of them shares elements with itself; they must not overlap")
+        raise ValueError("AxialRotary.rotate_: the tensors are the same memory in part, or one of them shares elements with itself; they "
+                         "must not overlap")
     _hip.check(rc, "rotary")
 
 
@@ -230,6 +232,8 @@ class _RotaryFn(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, *grads):
+        if forward_ad._current_level >= 0:
+            _hip.refuse_tangents("AxialRotary", *grads)
         ps = ctx.ps
         if None in ps:
             saved = iter(ctx.saved_tensors)

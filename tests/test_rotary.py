@@ -394,3 +394,21 @@ def test_in_place_turns_of_overlapping_views_are_refused():
     want = [rot(t, grid) for t in views(before)]
     rot.rotate_(q, grid, k, grid)
     assert torch.equal(q, want[0]) and torch.equal(k, want[2]) and torch.equal(buf[:, :, 5:], before[:, :, 5:])
+
+
+def test_gradients_with_a_forward_mode_tangent_are_refused(monkeypatch):
+    """Forward over reverse: the tangent comes with the gradient, not with the tensor."""
+    from torch.autograd import forward_ad
+
+    from aicity_action_amd import rotary
+    rot, grid = AxialRotary(96), TokenGrid((2, 2, 2))
+    monkeypatch.setattr(rotary, "_launch", lambda xs, outs, *a: [y.zero_() for y in outs])
+    monkeypatch.setattr(rotary, "_leaf_on_one_stream", lambda t: None)
+    monkeypatch.setattr(torch.Tensor, "is_cuda", True)
+    x, w = torch.zeros(1, 1, 8, 96, requires_grad=True), torch.ones(1, 1, 8, 96)
+    assert torch.autograd.grad(rot(x, grid), x, w)[0].shape == x.shape
+    with forward_ad.dual_level():
+        y = rot(x, grid)
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            torch.autograd.grad(y, x, forward_ad.make_dual(w, torch.ones_like(w)))
+        assert torch.autograd.grad(rot(x, grid), x, w)[0].shape == x.shape
